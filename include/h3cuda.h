@@ -39,6 +39,15 @@
  *                         Machine.swift:48-56), for CUDA devices and NVLink
  *   h3c_nvlink_query      the NVLink / NVSwitch part of that discovery
  *                         (Machine.swift:48-56 measures, never assumes)
+ *   h3c_cross_attn_fwd/bwd, h3c_prefix_attn_fwd  new: attention to an
+ *                         encoder's states and over a shared prefix, beside
+ *                         AttentionLayer.sdpa (DiTBlock.swift:293-328; the
+ *                         reference packs its conditioning rows into the one
+ *                         self-attention sequence, PackedSequence.swift:191-297)
+ *   h3c_qk_norm_rope_fwd/bwd  qNorm/kNorm + SplitHalfRoPE (DiTBlock.swift:
+ *                         346-352) with queries and keys of their own lengths
+ *                         and heads, and the gradients (the reference only
+ *                         infers)
  *   h3c_init/h3c_destroy  the backend instance AttentionRegistry.resolve
  *                         creates once per render (AttentionBackend.swift:255-259)
  */
@@ -291,6 +300,107 @@ h3c_status h3c_attn_fwd_noalloc(const h3c_attn_args* args, void* stream, char* e
  * bounded wait of the last call gave up (its output is invalid).  Allocates
  * nothing.  No counterpart in the reference (see h3c_attn_fwd_noalloc). */
 h3c_status h3c_attn_fwd_noalloc_status(void);
+
+/* --- conditioning: cross attention, shared prefix, q/k norm ------------------ */
+/* These calls keep no state between them: scratch is the caller's
+ * (`workspace`, device memory of at least the size the matching
+ * *_workspace_size call gives, 256-byte aligned; its contents need not be
+ * kept or cleared), so calls on several streams, host threads or captured
+ * graphs are independent as long as each has its own workspace and outputs.
+ * They are asynchronous on `stream`, allocate nothing and may be captured.
+ * Results are deterministic: no sum depends on the order of atomics. */
+
+/* A bf16 [batch, tokens, heads, 128] operand: element (b, s, h, d) sits at
+ * ptr[b * batch_stride + s * token_stride + h * head_stride + d].  A stride of
+ * an axis with one element is not read.  Inputs may be broadcast (stride 0)
+ * over the batch and the heads; outputs may not.  ptr and every stride are
+ * multiples of 16 bytes.  ptr may be NULL when the operand has no elements. */
+typedef struct h3c_bview {
+  void* ptr;
+  int64_t batch_stride;
+  int64_t token_stride;
+  int64_t head_stride;
+} h3c_bview;
+
+enum { H3C_OP_CROSS_FWD = 0, H3C_OP_CROSS_BWD = 1, H3C_OP_PREFIX_FWD = 2 };
+
+/* Query head h reads key head h / (heads / kv_heads).  Member b's queries
+ * attend to its first kv_lens[b] keys (clamped to [0, kv_len]; NULL: all),
+ * after the shared prefix where there is one; key and value rows past that
+ * length are not used whatever they hold (NaN included).  A row without keys
+ * gives an output of 0, a log-sum-exp of -inf and no gradient. */
+typedef struct h3c_cross_args {
+  h3c_bview q, out;           /* [batch, q_len, heads, 128]; out may not overlap an input */
+  h3c_bview k, v;             /* [batch, kv_len, kv_heads, 128] */
+  int32_t batch, q_len, kv_len;
+  int32_t heads, kv_heads;    /* heads divisible by kv_heads */
+  int32_t head_dim;           /* must be 128 */
+  float scale;                /* softmax scale */
+  const int32_t* kv_lens;     /* device [batch] or NULL */
+  float* lse;                 /* device fp32 [batch, heads, q_len]: natural log of the softmax
+                                 denominator; written by the forward calls (NULL: not wanted),
+                                 read by the backward call */
+  /* h3c_prefix_attn_fwd: keys and values all members share */
+  h3c_view prefix_k, prefix_v; /* [prefix_len, kv_heads, 128] */
+  int32_t prefix_len;
+  int32_t reserved;           /* 0 */
+  /* h3c_cross_attn_bwd */
+  h3c_bview out_grad, dq;     /* [batch, q_len, heads, 128] */
+  h3c_bview dk, dv;           /* [batch, kv_len, kv_heads, 128]; rows past kv_lens get 0 */
+  void* workspace;
+  size_t workspace_bytes;
+} h3c_cross_args;
+
+/* Checks the arguments of operator `op` (H3C_OP_*) and gives the bytes of
+ * workspace the call needs (0: workspace may be NULL).  Host only, no device
+ * needed.  err (optional) receives the reason of a refusal. */
+h3c_status h3c_cross_workspace_size(const h3c_cross_args* args, int32_t op, size_t* bytes, char* err,
+                                    size_t err_len);
+/* out = softmax(scale q k^T) v over an encoder's states. */
+h3c_status h3c_cross_attn_fwd(h3c_ctx* ctx, const h3c_cross_args* args, void* stream);
+/* dq, dk, dv of h3c_cross_attn_fwd from out_grad and the forward call's out
+ * and lse; dk and dv sum over the query heads that share a key head.  The
+ * gradients may not overlap any input. */
+h3c_status h3c_cross_attn_bwd(h3c_ctx* ctx, const h3c_cross_args* args, void* stream);
+/* Attention over the keys of the shared prefix followed by each member's own
+ * (kv_len may be 0).  With few queries a member the prefix is read once for
+ * the whole batch. */
+h3c_status h3c_prefix_attn_fwd(h3c_ctx* ctx, const h3c_cross_args* args, void* stream);
+
+/* Per-head RMSNorm of queries and keys and their rotation, one pass:
+ *   y = R (x / sqrt(mean(x^2) + eps) * w)
+ * in fp32 with one rounding at the end (h3c_prologue rounds after each step,
+ * as the reference's inference does).  R turns channel pairs (i, half + i) by
+ * the table's (t0, t1; t2, t3) entry of the token, as h3c_rope_table lays
+ * them out; channels from 2*half up pass.  A table may be NULL: norm only. */
+typedef struct h3c_qk_norm_args {
+  h3c_bview q, q_out;         /* [batch, q_len, heads, 128]; q_out may be q */
+  h3c_bview k, k_out;         /* [batch, k_len, kv_heads, 128]; k_out may be k */
+  int32_t batch, q_len, k_len, heads, kv_heads;
+  int32_t head_dim;           /* must be 128 */
+  const void* q_norm_weight;  /* bf16 [128] */
+  const void* k_norm_weight;  /* bf16 [128] */
+  const void* q_rope;         /* bf16 [q_len, q_rope_half, 4], or one such table a member */
+  const void* k_rope;         /* bf16 [k_len, k_rope_half, 4], likewise */
+  int64_t q_rope_batch_stride, k_rope_batch_stride; /* elements; 0: one table for the batch */
+  int32_t q_rope_half, k_rope_half;
+  float eps;
+  int32_t reserved;           /* 0 */
+  /* h3c_qk_norm_rope_bwd: gradients of the outputs in, of q, k and the weights out */
+  h3c_bview q_grad, dq;       /* dq may be q_grad */
+  h3c_bview k_grad, dk;       /* dk may be k_grad */
+  float* q_norm_grad;         /* device fp32 [128] */
+  float* k_norm_grad;         /* device fp32 [128] */
+  void* workspace;            /* h3c_qk_norm_rope_bwd only */
+  size_t workspace_bytes;
+} h3c_qk_norm_args;
+
+/* Checks the arguments of the forward (backward == 0) or backward call and
+ * gives the bytes of workspace it needs (0 for the forward call). */
+h3c_status h3c_qk_norm_workspace_size(const h3c_qk_norm_args* args, int32_t backward, size_t* bytes, char* err,
+                                      size_t err_len);
+h3c_status h3c_qk_norm_rope_fwd(h3c_ctx* ctx, const h3c_qk_norm_args* args, void* stream);
+h3c_status h3c_qk_norm_rope_bwd(h3c_ctx* ctx, const h3c_qk_norm_args* args, void* stream);
 
 /* --- sequence-sharded path (NCCL) ------------------------------------------ */
 /* Multi-GPU layout for the longest sequences (one process per GPU).  The

@@ -33,23 +33,18 @@
 // word and raises a CTA-wide abort flag; every role drains to the common
 // exit, where TMEM is freed, and the waits of every other CTA see the status
 // word and stop too.
-#include <cuda.h>
-
 #include <climits>
 #include <mutex>
 #include <cstdlib>
 #include <type_traits>
 
-#include "common.cuh"
+#include "tcgen05.cuh"
 
 namespace h3 {
 namespace {
 
 constexpr int kThreads = 384;
 constexpr int kStages = 4;
-constexpr int kTileBytes = 128 * 128 * 2;   // one 128x128 bf16 tile
-constexpr int kHalfBytes = kTileBytes / 2;  // one 128x64 swizzle box
-constexpr uint64_t kWaitLimitNs = 4000000000ull;  // 4 s
 
 struct __align__(8) Barriers {
   uint64_t q_full[2];
@@ -71,147 +66,6 @@ static_assert(sizeof(Barriers) <= 256, "barrier block");
 constexpr int kSmemTiles = 2 * kTileBytes + kStages * kTileBytes;
 constexpr int kSmemBytes = kSmemTiles + 1024 /*align slack*/ + 256 /*barriers*/;
 
-// ------------------------------------------------------------- primitives
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-__device__ __forceinline__ uint64_t globaltimer() {
-  uint64_t t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  return t;
-}
-
-__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
-}
-
-__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-
-// Bounded wait; false on abort/timeout.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int32_t* abort_flag,
-                                          int32_t* status, uint64_t limit_ns = kWaitLimitNs) {
-  for (int i = 0; i < 64; ++i)
-    if (mbar_try(bar, parity)) return true;
-  const uint64_t t0 = globaltimer();
-  while (true) {
-    if (mbar_try(bar, parity)) return true;
-    if (*abort_flag) return false;
-    // another CTA's wait already gave up: stop instead of timing out again
-    // (one status word per launch, so a systematic stall ends in one limit)
-    if (status && *(volatile int32_t*)status != 0) {
-      *abort_flag = 1;
-      return false;
-    }
-    if (globaltimer() - t0 > limit_ns) {
-      *abort_flag = 1;
-      if (status) atomicExch(status, (int32_t)H3C_ERR_TIMEOUT);
-      return false;
-    }
-  }
-}
-
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-
-__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-
-// 3D tiled TMA load (no multicast): coordinates (d, token, head).
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1,
-                                            int c2) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], "
-      "[%2];" ::"r"(dst),
-      "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
-      : "memory");
-}
-
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-__device__ __forceinline__ void tc_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-
-// D[tmem] (+)= A[smem desc] * B[smem desc]
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
-      : "memory");
-}
-
-// D[tmem] (+)= A[tmem] * B[smem desc]
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc)
-      : "memory");
-}
-
-// The same three operations issued by a whole converged warp, one lane
-// elected by elect.sync: the MMA warp runs its loop with all 32 lanes (no
-// divergent single-lane branch around the issue), which measured 3% faster
-// than a lane-0-only issuer (config 2 and dense).
-__device__ __forceinline__ void mma_ss_w(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
-      : "memory");
-}
-
-__device__ __forceinline__ void mma_ts_w(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc)
-      : "memory");
-}
-
-__device__ __forceinline__ void tc_commit_w(uint32_t bar) {
-  asm volatile(
-      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
-      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
-      : "memory");
-}
-
-#define H3_TMEM_LD16(addr, r)                                                                                 \
-  asm volatile(                                                                                               \
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];" \
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),       \
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])  \
-      : "r"(addr))
-
-#define H3_TMEM_ST16(addr, r)                                                                                  \
-  asm volatile(                                                                                                \
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" \
-      ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),       \
-      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])              \
-      : "memory")
-
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // 2^x on the FMA pipe, for the share of the exponentials that would
 // otherwise queue on the MUFU unit.  Cody-Waite split x = n + f with
 // n = round(x) (via the 1.5*2^23 rounding constant) and f in [-0.5, 0.5];
@@ -228,58 +82,6 @@ __device__ __forceinline__ float ex2_poly(float x) {
   const float f = __fsub_rn(x, __fsub_rn(t, kRound));
   const float p = fmaf(fmaf(fmaf(kC3, f, kC2), f, kC1), f, kC0);
   return __int_as_float(__float_as_int(p) + (__float_as_int(t) << 23));
-}
-
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-
-// (x0, x1) = (s0, s1) * k + b on the packed f32x2 pipe; k, b hold a scalar
-// in both halves.
-__device__ __forceinline__ void fma2(float& x0, float& x1, uint32_t s0, uint32_t s1, uint64_t k, uint64_t b) {
-  asm("{\n\t.reg .b64 a, d;\n\tmov.b64 a, {%2, %3};\n\t"
-      "fma.rn.ftz.f32x2 d, a, %4, %5;\n\tmov.b64 {%0, %1}, d;\n\t}"
-      : "=f"(x0), "=f"(x1)
-      : "r"(s0), "r"(s1), "l"(k), "l"(b));
-}
-
-__device__ __forceinline__ uint64_t add2(uint64_t acc, float a, float b) {
-  uint64_t r;
-  asm("{\n\t.reg .b64 t;\n\tmov.b64 t, {%2, %3};\n\tadd.rn.ftz.f32x2 %0, %1, t;\n\t}"
-      : "=l"(r)
-      : "l"(acc), "f"(a), "f"(b));
-  return r;
-}
-
-__device__ __forceinline__ uint64_t dup2(float v) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %1};" : "=l"(r) : "f"(v));
-  return r;
-}
-
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-  __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<uint32_t*>(&v);
-}
-
-// Shared-memory matrix descriptor, 128-byte swizzle (layout type 2),
-// descriptor version 1; lbo/sbo in bytes.
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
-  uint64_t d = 0;
-  d |= (uint64_t)((addr >> 4) & 0x3FFF);
-  d |= (uint64_t)((lbo >> 4) & 0x3FFF) << 16;
-  d |= (uint64_t)((sbo >> 4) & 0x3FFF) << 32;
-  d |= (uint64_t)1 << 46;
-  d |= (uint64_t)2 << 61;
-  return d;
-}
-
-// Instruction descriptor, kind::f16: bf16 x bf16 -> f32, M = 128, N = 128.
-constexpr uint32_t idesc_bf16(bool b_mn_major) {
-  return (1u << 4) | (1u << 7) | (1u << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((128u >> 3) << 17) |
-         ((128u >> 4) << 24);
 }
 
 // ------------------------------------------------------------------ kernel
@@ -670,23 +472,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // --------------------------------------------------------------- host side
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-// Looked up once per process (thread-safe static initialisation).
-EncodeTiledFn get_encode() {
-  static const EncodeTiledFn fn = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      return (EncodeTiledFn)p;
-    return (EncodeTiledFn) nullptr;
-  }();
-  return fn;
-}
-
 // (d, token, head) view of a strided bf16 operand, boxes of 64 x 128 x 1.
 bool make_map(CUtensorMap* m, const void* base, int64_t tok_stride, int64_t head_stride, int seq, int heads,
               std::string* err) {

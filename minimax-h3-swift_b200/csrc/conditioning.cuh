@@ -1,0 +1,62 @@
+// Internal types of the conditioning calls (cross attention, shared prefix,
+// q/k norm): normalised operands and the launchers of the kernel files.
+#pragma once
+
+#include "common.cuh"
+
+namespace h3 {
+
+// A [batch, tokens, heads, 128] operand; strides in elements, 0 on an axis of
+// one element or a broadcast axis.
+struct Rows {
+  uint16_t* p;
+  int64_t b, t, h;
+  __host__ __device__ uint16_t* at(int64_t ib, int64_t it, int64_t ih) const { return p + ib * b + it * t + ih * h; }
+};
+
+struct CrossShape {
+  int32_t batch, q_len, kv_len, prefix_len, heads, kv_heads, group;
+};
+
+struct CrossLaunch {
+  CrossShape n;
+  Rows q, out, k, v, pk, pv;  // pk, pv: batch stride 0
+  Rows dout, dq, dk, dv;
+  float scale;
+  const int32_t* kv_lens;     // may be null
+  float* lse;                 // may be null (forward)
+  uint8_t* ws;
+  int32_t* status;            // status word of the context (bounded waits)
+  uint64_t wait_limit_ns;
+};
+
+__device__ __forceinline__ int kv_len_of(const int32_t* kv_lens, int kv_len, int b) {
+  return kv_lens ? max(0, min(kv_len, kv_lens[b])) : kv_len;
+}
+
+size_t cross_fwd_workspace(const CrossShape& n);
+size_t cross_bwd_workspace(const CrossShape& n);
+cudaError_t launch_cross_fwd(const CrossLaunch& a, cudaStream_t s, std::string* err);
+cudaError_t launch_cross_bwd(const CrossLaunch& a, cudaStream_t s, std::string* err);
+
+struct QkNormOperand {
+  Rows x, g, y;               // rows in; gradient of the output in (backward); result out
+  int32_t tokens, heads, half;
+  const uint16_t* w;
+  const uint16_t* table;      // null: no rotation
+  int64_t table_batch;        // elements; 0: one table for the batch
+  float* dw;                  // backward: fp32 [128]
+};
+
+struct QkNormLaunch {
+  QkNormOperand op[2];        // queries, keys
+  int32_t batch;
+  float eps;
+  float* ws;
+};
+
+size_t qk_norm_bwd_workspace();
+cudaError_t launch_qk_norm_fwd(const QkNormLaunch& a, cudaStream_t s);
+cudaError_t launch_qk_norm_bwd(const QkNormLaunch& a, cudaStream_t s);
+
+}  // namespace h3

@@ -31,6 +31,10 @@ H3C_FUSE_PROLOGUE = 1
 H3C_KERNEL_MMA_SYNC = 2
 H3C_NO_ROPE = 4
 
+H3C_OP_CROSS_FWD = 0
+H3C_OP_CROSS_BWD = 1
+H3C_OP_PREFIX_FWD = 2
+
 # Every exported symbol of include/h3cuda.h, checked by the CPU test suite.
 EXPORTS = (
     "h3c_abi_version", "h3c_init", "h3c_destroy", "h3c_last_error", "h3c_device_info",
@@ -41,6 +45,8 @@ EXPORTS = (
     "h3c_comm_unique_id", "h3c_comm_init", "h3c_comm_destroy", "h3c_attn_fwd_seqshard",
     "h3c_blockmask_validate", "h3c_attn_fwd_noalloc_status", "h3c_nvlink_query",
     "h3c_device_alloc", "h3c_device_free", "h3c_comm_wait",
+    "h3c_cross_workspace_size", "h3c_cross_attn_fwd", "h3c_cross_attn_bwd", "h3c_prefix_attn_fwd",
+    "h3c_qk_norm_workspace_size", "h3c_qk_norm_rope_fwd", "h3c_qk_norm_rope_bwd",
 )
 
 
@@ -115,6 +121,37 @@ class AttnArgs(C.Structure):
     ]
 
 
+class BView(C.Structure):
+    _fields_ = [("ptr", C.c_void_p), ("batch_stride", C.c_int64), ("token_stride", C.c_int64),
+                ("head_stride", C.c_int64)]
+
+
+class CrossArgs(C.Structure):
+    _fields_ = [
+        ("q", BView), ("out", BView), ("k", BView), ("v", BView),
+        ("batch", C.c_int32), ("q_len", C.c_int32), ("kv_len", C.c_int32),
+        ("heads", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("scale", C.c_float),
+        ("kv_lens", C.c_void_p), ("lse", C.c_void_p),
+        ("prefix_k", View), ("prefix_v", View), ("prefix_len", C.c_int32), ("reserved", C.c_int32),
+        ("out_grad", BView), ("dq", BView), ("dk", BView), ("dv", BView),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class QkNormArgs(C.Structure):
+    _fields_ = [
+        ("q", BView), ("q_out", BView), ("k", BView), ("k_out", BView),
+        ("batch", C.c_int32), ("q_len", C.c_int32), ("k_len", C.c_int32), ("heads", C.c_int32),
+        ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
+        ("q_norm_weight", C.c_void_p), ("k_norm_weight", C.c_void_p), ("q_rope", C.c_void_p),
+        ("k_rope", C.c_void_p), ("q_rope_batch_stride", C.c_int64), ("k_rope_batch_stride", C.c_int64),
+        ("q_rope_half", C.c_int32), ("k_rope_half", C.c_int32), ("eps", C.c_float), ("reserved", C.c_int32),
+        ("q_grad", BView), ("dq", BView), ("k_grad", BView), ("dk", BView),
+        ("q_norm_grad", C.c_void_p), ("k_norm_grad", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -161,6 +198,14 @@ def load() -> C.CDLL:
             "h3c_device_alloc": ([vp, C.c_size_t, C.POINTER(vp)], st),
             "h3c_comm_wait": ([vp, vp, i64], st),
             "h3c_device_free": ([vp, vp], st),
+            "h3c_cross_workspace_size": ([C.POINTER(CrossArgs), i32, C.POINTER(C.c_size_t), C.c_char_p, C.c_size_t], st),
+            "h3c_cross_attn_fwd": ([vp, C.POINTER(CrossArgs), vp], st),
+            "h3c_cross_attn_bwd": ([vp, C.POINTER(CrossArgs), vp], st),
+            "h3c_prefix_attn_fwd": ([vp, C.POINTER(CrossArgs), vp], st),
+            "h3c_qk_norm_workspace_size": ([C.POINTER(QkNormArgs), i32, C.POINTER(C.c_size_t), C.c_char_p,
+                                            C.c_size_t], st),
+            "h3c_qk_norm_rope_fwd": ([vp, C.POINTER(QkNormArgs), vp], st),
+            "h3c_qk_norm_rope_bwd": ([vp, C.POINTER(QkNormArgs), vp], st),
             "h3c_blockmask_validate": ([vp, vp, vp, i32, i64, vp], st),
         }
         for name, (args, res) in sig.items():

@@ -32,6 +32,45 @@ def view_of(t, layout: str) -> _lib.View:
     return _lib.View(t.data_ptr(), tok, head)
 
 
+def _bview(name, t, layout: str, device: int, shape=None):
+    """``(h3c_bview, (batch, tokens, heads))`` of a bf16 tensor on ``device``:
+    [B, S, H, 128] or [S, H, 128] ("SHD"), [B, H, S, 128] or [H, S, 128]
+    ("HSD").  ``shape``: the (batch, tokens, heads) it must have."""
+    import torch
+
+    if t.dtype is not torch.bfloat16 or t.device.type != "cuda" or t.device.index != device:
+        raise ValueError(f"{name} must be bfloat16 on cuda:{device}, got {t.dtype} on {t.device}")
+    size, stride = t.shape, t.stride()
+    if len(size) == 3:
+        size, stride = (1, *size), (0, *stride)
+    if len(size) != 4:
+        raise ValueError(f"{name} must have 3 or 4 axes, got {tuple(t.shape)}")
+    if layout == "SHD":
+        b, s, h, d = size
+        view = _lib.BView(t.data_ptr(), stride[0], stride[1], stride[2])
+    elif layout == "HSD":
+        b, h, s, d = size
+        view = _lib.BView(t.data_ptr(), stride[0], stride[2], stride[1])
+    else:
+        raise ValueError(layout)
+    if stride[3] != 1 and d > 1:
+        raise ValueError(f"{name}: head_dim must be contiguous")
+    if d != 128:
+        raise _lib.H3CError(_lib.H3C_ERR_UNSUPPORTED, f"{name}: head_dim must be 128, got {d}")
+    if shape is not None and (b, s, h) != shape:
+        raise ValueError(f"{name} must have {shape} (batch, tokens, heads), got {(b, s, h)}")
+    return view, (b, s, h)
+
+
+def _vector(name, t, dtype, shape, device: int) -> int:
+    """Device pointer of a contiguous tensor of the given type and shape."""
+    if t.dtype is not dtype or t.device.type != "cuda" or t.device.index != device or tuple(t.shape) != shape \
+            or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape} on cuda:{device}, got "
+                         f"{t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
 class Runtime:
     _lock = threading.Lock()
     _by_device: Dict[int, "Runtime"] = {}
@@ -148,6 +187,145 @@ class Runtime:
 
     def attn_fwd_args(self, a: _lib.AttnArgs, stream=None):
         self._check(self.L.h3c_attn_fwd(self.ctx, C.byref(a), _stream_ptr(stream)))
+
+    # --------------------------------------------------------- conditioning
+    def _launch(self, call, args, size_call, selector, stream):
+        """Run ``call`` with workspace of the size ``size_call`` gives, taken
+        from torch's allocator on the launching stream (so a captured call
+        keeps its own, and the memory is not reused before the call is done)."""
+        import torch
+
+        need, why = C.c_size_t(0), C.create_string_buffer(256)
+        st = size_call(C.byref(args), selector, C.byref(need), why, 256)
+        if st != _lib.H3C_OK:
+            raise _lib.H3CError(st, why.value.decode())
+        if stream is None:
+            stream = torch.cuda.current_stream(self.device)
+        ws = None
+        if need.value:
+            with torch.cuda.stream(stream):
+                ws = torch.empty(need.value, dtype=torch.uint8, device=f"cuda:{self.device}")
+            args.workspace, args.workspace_bytes = ws.data_ptr(), need.value
+        self._check(call(self.ctx, C.byref(args), stream.cuda_stream or None))
+
+    def _cross_args(self, q, k, v, out, layout, scale, kv_lens, lse):
+        import torch
+
+        a, dev = _lib.CrossArgs(), self.device
+        a.q, (B, S, H) = _bview("q", q, layout, dev)
+        a.out, _ = _bview("out", out, layout, dev, (B, S, H))
+        a.k, (kb, n, Hk) = _bview("k", k, layout, dev)
+        if kb != B:
+            raise ValueError(f"k must have the {B} members of q, got {kb}")
+        a.v, _ = _bview("v", v, layout, dev, (B, n, Hk))
+        a.batch, a.q_len, a.kv_len, a.heads, a.kv_heads, a.head_dim = B, S, n, H, Hk, 128
+        a.scale = scale
+        if kv_lens is not None:
+            a.kv_lens = _vector("kv_lens", kv_lens, torch.int32, (B,), dev)
+        if lse is not None:
+            shape = (B, H, S) if q.dim() == 4 or lse.dim() == 3 else (H, S)
+            a.lse = _vector("lse", lse, torch.float32, shape, dev)
+        return a
+
+    def cross_attn_fwd(self, *, q, k, v, out, scale, layout="SHD", kv_lens=None, lse=None, stream=None):
+        """``out = softmax(scale q k^T) v`` against encoder states of another
+        length.  q, out: [B, S, H, 128]; k, v: [B, N, Hk, 128] (or without
+        B; "HSD": [B, H, S, 128]), H a multiple of Hk.  kv_lens: int32 [B]
+        device tensor, the valid keys of each member; a member without keys
+        gives zeros.  lse: optional fp32 [B, H, S] result, needed by
+        ``cross_attn_bwd``."""
+        a = self._cross_args(q, k, v, out, layout, scale, kv_lens, lse)
+        self._launch(self.L.h3c_cross_attn_fwd, a, self.L.h3c_cross_workspace_size, _lib.H3C_OP_CROSS_FWD, stream)
+
+    def cross_attn_bwd(self, *, q, k, v, out, lse, out_grad, dq, dk, dv, scale, layout="SHD", kv_lens=None,
+                       stream=None):
+        """Gradients of ``cross_attn_fwd``: dq as q, dk and dv as k (summed
+        over the query heads of each key head, 0 past kv_lens), from the
+        forward call's out and lse.  Deterministic."""
+        a, dev = self._cross_args(q, k, v, out, layout, scale, kv_lens, lse), self.device
+        mine, keys = (a.batch, a.q_len, a.heads), (a.batch, a.kv_len, a.kv_heads)
+        a.out_grad, _ = _bview("out_grad", out_grad, layout, dev, mine)
+        a.dq, _ = _bview("dq", dq, layout, dev, mine)
+        a.dk, _ = _bview("dk", dk, layout, dev, keys)
+        a.dv, _ = _bview("dv", dv, layout, dev, keys)
+        self._launch(self.L.h3c_cross_attn_bwd, a, self.L.h3c_cross_workspace_size, _lib.H3C_OP_CROSS_BWD, stream)
+
+    def prefix_attn_fwd(self, *, q, prefix_k, prefix_v, k, v, out, scale, layout="SHD", kv_lens=None, lse=None,
+                        stream=None):
+        """Attention of every member's queries over the keys all members
+        share (prefix_k, prefix_v: [P, Hk, 128], "HSD": [Hk, P, 128]) and
+        then its own, as ``cross_attn_fwd``."""
+        a, dev = self._cross_args(q, k, v, out, layout, scale, kv_lens, lse), self.device
+        if prefix_k.dim() != 3 or prefix_v.dim() != 3:
+            raise ValueError("prefix_k and prefix_v have no batch axis")
+        pk, (_, P, _) = _bview("prefix_k", prefix_k, layout, dev)
+        _bview("prefix_k", prefix_k, layout, dev, (1, P, a.kv_heads))
+        pv, _ = _bview("prefix_v", prefix_v, layout, dev, (1, P, a.kv_heads))
+        a.prefix_k = _lib.View(pk.ptr, pk.token_stride, pk.head_stride)
+        a.prefix_v = _lib.View(pv.ptr, pv.token_stride, pv.head_stride)
+        a.prefix_len = P
+        self._launch(self.L.h3c_prefix_attn_fwd, a, self.L.h3c_cross_workspace_size, _lib.H3C_OP_PREFIX_FWD, stream)
+
+    def _rope_rows(self, name, table, batch, tokens):
+        """(pointer, half, batch stride) of a bf16 [S, half, 4] or [B, S, half, 4] table."""
+        import torch
+
+        if table is None:
+            return None, 0, 0
+        shape = (tokens,) if table.dim() == 3 else (batch, tokens)
+        if table.dtype is not torch.bfloat16 or table.device.type != "cuda" or table.device.index != self.device \
+                or table.dim() not in (3, 4) or table.shape[-1] != 4 or tuple(table.shape[:-2]) != shape \
+                or not table.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous bfloat16 {(*shape, 'half', 4)} tensor on cuda:{self.device}, "
+                             f"got {table.dtype} {tuple(table.shape)} on {table.device}")
+        return table.data_ptr(), table.shape[-2], tokens * table.shape[-2] * 4 if table.dim() == 4 else 0
+
+    def _norm_args(self, q, k, q_norm, k_norm, eps, q_rope, k_rope, layout):
+        import torch
+
+        a, dev = _lib.QkNormArgs(), self.device
+        a.q, (B, S, H) = _bview("q", q, layout, dev)
+        a.k, (kb, n, Hk) = _bview("k", k, layout, dev)
+        if kb != B:
+            raise ValueError(f"k must have the {B} members of q, got {kb}")
+        a.batch, a.q_len, a.k_len, a.heads, a.kv_heads, a.head_dim, a.eps = B, S, n, H, Hk, 128, eps
+        a.q_norm_weight = _vector("q_norm", q_norm, torch.bfloat16, (128,), dev)
+        a.k_norm_weight = _vector("k_norm", k_norm, torch.bfloat16, (128,), dev)
+        a.q_rope, a.q_rope_half, a.q_rope_batch_stride = self._rope_rows("q_rope", q_rope, B, S)
+        a.k_rope, a.k_rope_half, a.k_rope_batch_stride = self._rope_rows("k_rope", k_rope, B, n)
+        return a
+
+    def qk_norm_rope_fwd(self, *, q, k, q_out, k_out, q_norm, k_norm, eps=1e-6, q_rope=None, k_rope=None,
+                         layout="SHD", stream=None):
+        """Per-head RMSNorm of queries and keys and their rotation in one
+        pass, fp32 with one rounding.  q: [B, S, H, 128], k: [B, N, Hk, 128];
+        q_out / k_out may be q / k.  Tables: bf16 [S, half, 4] (as
+        ``rope_table`` makes them) or [B, S, half, 4]; None: norm only."""
+        a, dev = self._norm_args(q, k, q_norm, k_norm, eps, q_rope, k_rope, layout), self.device
+        a.q_out, _ = _bview("q_out", q_out, layout, dev, (a.batch, a.q_len, a.heads))
+        a.k_out, _ = _bview("k_out", k_out, layout, dev, (a.batch, a.k_len, a.kv_heads))
+        if stream is None:
+            import torch
+
+            stream = torch.cuda.current_stream(dev)
+        self._check(self.L.h3c_qk_norm_rope_fwd(self.ctx, C.byref(a), stream.cuda_stream or None))
+
+    def qk_norm_rope_bwd(self, *, q, k, q_grad, k_grad, q_norm, k_norm, dq, dk, dq_norm, dk_norm, eps=1e-6,
+                         q_rope=None, k_rope=None, layout="SHD", stream=None):
+        """Gradients of ``qk_norm_rope_fwd`` from those of its outputs
+        (q_grad, k_grad): dq, dk (may be q_grad, k_grad) and the fp32 [128]
+        gradients of the two weights.  Deterministic."""
+        import torch
+
+        a, dev = self._norm_args(q, k, q_norm, k_norm, eps, q_rope, k_rope, layout), self.device
+        mine, keys = (a.batch, a.q_len, a.heads), (a.batch, a.k_len, a.kv_heads)
+        a.q_grad, _ = _bview("q_grad", q_grad, layout, dev, mine)
+        a.k_grad, _ = _bview("k_grad", k_grad, layout, dev, keys)
+        a.dq, _ = _bview("dq", dq, layout, dev, mine)
+        a.dk, _ = _bview("dk", dk, layout, dev, keys)
+        a.q_norm_grad = _vector("dq_norm", dq_norm, torch.float32, (128,), dev)
+        a.k_norm_grad = _vector("dk_norm", dk_norm, torch.float32, (128,), dev)
+        self._launch(self.L.h3c_qk_norm_rope_bwd, a, self.L.h3c_qk_norm_workspace_size, 1, stream)
 
     # ------------------------------------------------------------- prologue
     def prologue(self, x, out, weight, eps, rope_table=None, layout="SHD", stream=None):
