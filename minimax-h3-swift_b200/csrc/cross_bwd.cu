@@ -1,5 +1,4 @@
-// Cross attention, its gradient and attention over a shared prefix: the plain
-// kernels.  One warp per row, lane l holds channels 4l..4l+3; softmax
+// Gradient of cross attention: the plain kernels.  One warp per row, lane l holds channels 4l..4l+3; softmax
 // statistics and sums in fp32.
 #include <cmath>
 
@@ -42,35 +41,6 @@ struct Walk {
   __device__ Walk()
       : i(((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5), step(((int64_t)gridDim.x * blockDim.x) >> 5) {}
 };
-
-__global__ void __launch_bounds__(256) cross_fwd_kernel(CrossLaunch a) {
-  const CrossShape n = a.n;
-  for (Walk w; w.i < (int64_t)n.batch * n.heads * n.q_len; w.i += w.step) {
-    const int t = (int)(w.i % n.q_len), h = (int)(w.i / n.q_len % n.heads), b = (int)(w.i / n.q_len / n.heads);
-    const int hk = h / n.group, own = kv_len_of(a.kv_lens, n.kv_len, b);
-    const F4 q = load4(a.q.at(b, t, h));
-    F4 o{};
-    float m = -INFINITY, l = 0.f;
-    for (int j = 0; j < n.prefix_len + own; ++j) {
-      const bool pre = j < n.prefix_len;
-      const F4 k = load4(pre ? a.pk.at(0, j, hk) : a.k.at(b, j - n.prefix_len, hk));
-      const F4 v = load4(pre ? a.pv.at(0, j, hk) : a.v.at(b, j - n.prefix_len, hk));
-      const float s = dot(q, k) * a.scale;
-      if (s > m) {
-        const float f = expf(m - s);
-        l *= f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o.v[i] *= f;
-        m = s;
-      }
-      const float p = expf(s - m);
-      l += p;
-      axpy(o, p, v);
-    }
-    store4(a.out.at(b, t, h), o, l > 0.f ? 1.f / l : 0.f);
-    if (a.lse && (threadIdx.x & 31) == 0) a.lse[w.i] = l > 0.f ? m + logf(l) : -INFINITY;
-  }
-}
 
 __global__ void __launch_bounds__(256) cross_dq_kernel(CrossLaunch a, float* delta) {
   const CrossShape n = a.n;
@@ -116,16 +86,7 @@ unsigned warps_grid(int64_t rows) { return (unsigned)((rows + 7) / 8 < 148 * 8 ?
 
 }  // namespace
 
-size_t cross_fwd_workspace(const CrossShape&) { return 0; }
-
 size_t cross_bwd_workspace(const CrossShape& n) { return (size_t)n.batch * n.heads * n.q_len * sizeof(float); }
-
-cudaError_t launch_cross_fwd(const CrossLaunch& a, cudaStream_t s, std::string*) {
-  const int64_t rows = (int64_t)a.n.batch * a.n.heads * a.n.q_len;
-  if (rows == 0) return cudaSuccess;
-  cross_fwd_kernel<<<warps_grid(rows), 256, 0, s>>>(a);
-  return cudaGetLastError();
-}
 
 cudaError_t launch_cross_bwd(const CrossLaunch& a, cudaStream_t s, std::string*) {
   const int64_t rows = (int64_t)a.n.batch * a.n.heads * a.n.q_len;

@@ -1,0 +1,901 @@
+// Cross attention and attention over a shared prefix on the Blackwell tensor
+// cores: tcgen05.mma with TMEM accumulators, TMA-staged K/V tiles, a
+// persistent CTA an SM.
+//
+//   o_i = sum_j 2^(s_ij - m_i) v_j / l_i,  s_ij = scale log2(e) q_i.k_j
+//
+// one pass over the keys with a running maximum m and sum l (fp32); weights
+// enter the second product in bf16, everything else is fp32 until the output.
+//
+// Work is cut into units: a block of query rows against all keys of one
+// source.  A CTA takes whole units in turn, or, where there are too few units
+// for the SMs, an equal share of all (unit, key tile) pairs in a row; a unit
+// that is cut, or whose rows have two sources, leaves fp32 partial results
+// (o, m, l) that combine_kernel joins in a fixed order.  Row blocks:
+//   dense   q_len >= 128: 2 x 128 tokens of one head, Q tiles by TMA; keys are
+//           the prefix's and then the member's own
+//   folded  q_len < 128: a row is (member, token, head of the group), so one
+//           K/V tile serves all query heads of its key head and, for the
+//           prefix, the whole batch; rows are gathered by two warps.  The
+//           prefix and each member's own keys are units of their own.
+//           More than 128 rows: two row tiles share each K/V tile (dual).
+//           Up to 128: the two halves of the CTA take alternate K/V tiles of
+//           the same rows (single) and their results are joined through TMEM;
+//           one half alone reaches 5.3 of the 6.5 TB/s that HBM gives.
+//
+// Roles of a CTA's 12 warps: 0 TMA producer; 1 MMA issuer; 2-3 gather folded
+// query rows (2 also owns TMEM); 4-7 and 8-11 softmax and epilogue of half 0
+// and 1, thread = row = TMEM lane.  TMEM: half t has S (then P, packed bf16,
+// over its first 64 columns) at 256t and O at 256t + 128.  K/V entries run
+// through a ring of 2 (3 in single mode, where each entry is needed for two
+// steps); the producer hands each entry's flags to the issuer through shared
+// memory.  The next unit's Q and K/V loads and its first S overlap the
+// epilogue of this one.  Every wait is bounded (see attn_tc.cu).
+#include <climits>
+#include <mutex>
+#include <type_traits>
+
+#include "conditioning.cuh"
+#include "tcgen05.cuh"
+
+namespace h3 {
+namespace {
+
+constexpr int kThreads = 384;
+constexpr int kSms = 148;
+
+enum { kDense = 0, kSingle = 1, kDual = 2 };
+
+struct FwdPlan {
+  int32_t mode;
+  int32_t np, nb;             // key tiles of the prefix and of kv_len
+  int32_t per_p, per_o;       // row blocks of a key head (prefix), of a member's (key) head (own)
+  int32_t units_p, units_o;   // units of the prefix (folded only) and the others
+  int32_t tiles_p, tiles_o;   // key tiles of such a unit
+  int32_t unit_rows;          // rows of a block: 128 or 256
+  int32_t fold_rows;          // folded: rows of a key head over the batch
+  int32_t tpc;                // key tiles a CTA in the linear split; 0: whole units in turn
+  int32_t ctas;
+  int32_t slots_p, slots;     // partial results a row, at most: from the prefix's units, in all
+  int32_t combine;
+  int64_t part_rows;
+};
+
+struct FwdArgs {
+  CrossShape n;
+  FwdPlan p;
+  Rows q, out;
+  const int32_t* kv_lens;
+  float* lse;
+  float scale_log2;
+  float* part_o;              // [part_rows, slots, 128]
+  float2* part_ml;            // [part_rows, slots]
+  int32_t* status;
+  uint64_t wait_limit_ns;
+  // 1 where an operand's tensor map has the axis, 0 where it is broadcast
+  int32_t q_b, q_h, k_b, k_h, v_b, v_h, pk_h, pv_h;
+};
+
+// One run of key tiles of one unit.
+struct Seg {
+  int b, hk, h;               // h: dense only
+  int row0, row_end;          // tokens (dense) or folded rows
+  int npre, len;              // tiles of the unit that are the prefix's; valid own keys
+  int j0, n;                  // first tile, tiles with valid keys (0: nothing to do)
+  int slot;                   // partial slot
+  bool direct;                // the whole result of its rows
+};
+
+struct SegIter {
+  int64_t pos, end;
+  __device__ explicit SegIter(const FwdPlan& p) {
+    if (p.tpc) {
+      const int64_t total = (int64_t)p.units_p * p.tiles_p + (int64_t)p.units_o * p.tiles_o;
+      pos = (int64_t)blockIdx.x * p.tpc;
+      end = min(total, pos + p.tpc);
+    } else {
+      pos = blockIdx.x;
+      end = p.units_p + p.units_o;
+    }
+  }
+  __device__ bool next(const FwdArgs& a, Seg& s) {
+    if (pos >= end) return false;
+    const FwdPlan& p = a.p;
+    int u, j1, tiles;
+    s.slot = 0;
+    if (p.tpc) {
+      const int64_t pre = (int64_t)p.units_p * p.tiles_p;
+      const bool own = pos >= pre;
+      const int64_t off = own ? pos - pre : pos;
+      tiles = own ? p.tiles_o : p.tiles_p;
+      const int v = (int)(off / tiles);
+      u = own ? p.units_p + v : v;
+      s.j0 = (int)(off - (int64_t)v * tiles);
+      j1 = (int)min((int64_t)tiles, s.j0 + (end - pos));
+      s.slot = (int)(blockIdx.x - (pos - s.j0) / p.tpc);
+      pos += j1 - s.j0;
+    } else {
+      u = (int)pos;
+      tiles = u < p.units_p ? p.tiles_p : p.tiles_o;
+      s.j0 = 0;
+      j1 = tiles;
+      pos += gridDim.x;
+    }
+    int limit;
+    if (u < p.units_p) {
+      s.hk = u / p.per_p;
+      s.row0 = (u - s.hk * p.per_p) * p.unit_rows;
+      s.row_end = min(p.fold_rows, s.row0 + p.unit_rows);
+      s.b = 0;
+      s.len = 0;
+      s.npre = limit = p.np;
+    } else {
+      const int v = u - p.units_p, x = v / p.per_o, rt = v - x * p.per_o;
+      if (p.mode == kDense) {
+        s.b = x / a.n.heads;
+        s.h = x - s.b * a.n.heads;
+        s.hk = s.h / a.n.group;
+        s.row0 = rt * p.unit_rows;
+        s.row_end = min(a.n.q_len, s.row0 + p.unit_rows);
+        s.npre = p.np;
+      } else {
+        s.b = x / a.n.kv_heads;
+        s.hk = x - s.b * a.n.kv_heads;
+        const int rows = a.n.q_len * a.n.group;
+        s.row0 = s.b * rows + rt * p.unit_rows;
+        s.row_end = min((s.b + 1) * rows, s.row0 + p.unit_rows);
+        s.npre = 0;
+        s.slot += p.slots_p;
+      }
+      s.len = kv_len_of(a.kv_lens, a.n.kv_len, s.b);
+      limit = s.npre + ((s.len + 127) >> 7);
+    }
+    s.n = max(0, min(j1, limit) - s.j0);
+    s.direct = s.j0 == 0 && j1 == tiles && (p.units_p == 0 || p.units_o == 0);
+    return true;
+  }
+  // valid keys of tile j of the segment's unit
+  static __device__ int valid(const FwdArgs& a, const Seg& s, int j) {
+    return min(128, j < s.npre ? a.n.prefix_len - 128 * j : s.len - 128 * (j - s.npre));
+  }
+};
+
+template <bool SINGLE>
+struct Layout {
+  static constexpr int kRing = SINGLE ? 3 : 2;      // K/V entries
+  static constexpr int kQTiles = SINGLE ? 1 : 2;
+  static constexpr int kTiles = (kQTiles + 2 * kRing) * kTileBytes;
+};
+
+struct __align__(8) Barriers {
+  uint64_t q_full[2], q_empty[2];
+  uint64_t kv_full[3], k_empty[3], v_empty[3];
+  uint64_t s_full[2], p_half[2], p_full[2], o_full[2], o_empty[2];
+  uint64_t ml_full;
+  uint64_t done;              // every MMA has retired
+  uint32_t tmem_base;
+  int32_t abort;
+  int32_t info[16];           // flags of entry e at [e & 15]
+  float2 ml[128];             // single mode: maximum and sum of half 1
+};
+
+// flags of an entry: bit t: half t takes it; 2 + t / 4 + t: first / last of the segment for half t
+enum { kFirst = 2, kLast = 4, kSegFirst = 1 << 6, kSegLast = 1 << 7, kEnd = 1 << 8, kZeroShift = 16 };
+
+template <bool SINGLE>
+constexpr int smem_bytes() {
+  return Layout<SINGLE>::kTiles + 1024 + (int)sizeof(Barriers);
+}
+static_assert(smem_bytes<true>() <= 227 * 1024 && smem_bytes<false>() <= 227 * 1024, "shared memory");
+
+// Instruction descriptor, kind::f16: bf16 x bf16 -> f32, M = N = 128.
+constexpr uint32_t kIdS = idesc_bf16(false), kIdPV = idesc_bf16(true);
+
+__device__ __forceinline__ void store_row32(uint16_t* p, const float* v, float f) {
+  uint32_t w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = pack_bf16(v[2 * i] * f, v[2 * i + 1] * f);
+  reinterpret_cast<uint4*>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+  reinterpret_cast<uint4*>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+}
+
+template <bool SINGLE>
+__global__ void __launch_bounds__(kThreads, 1)
+    cross_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                     const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_pk,
+                     const __grid_constant__ CUtensorMap tm_pv, const __grid_constant__ FwdArgs a) {
+  using L = Layout<SINGLE>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* sQ = smem;
+  uint8_t* sKV = smem + L::kQTiles * kTileBytes;  // entry r: K at 2r, V at 2r + 1
+  Barriers* bars = (Barriers*)(smem + L::kTiles);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile int32_t* abort_flag = &bars->abort;
+  const bool dense = a.p.mode == kDense;
+
+  if (threadIdx.x == 0) {
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(smem_u32(&bars->q_full[t]), dense ? 1 : 64);
+      mbar_init(smem_u32(&bars->q_empty[t]), 1);
+      mbar_init(smem_u32(&bars->s_full[t]), 1);
+      mbar_init(smem_u32(&bars->p_half[t]), 128);
+      mbar_init(smem_u32(&bars->p_full[t]), 128);
+      mbar_init(smem_u32(&bars->o_full[t]), 1);
+      mbar_init(smem_u32(&bars->o_empty[t]), 128);
+    }
+    for (int r = 0; r < 3; ++r) {
+      mbar_init(smem_u32(&bars->kv_full[r]), 1);
+      mbar_init(smem_u32(&bars->k_empty[r]), 1);
+      mbar_init(smem_u32(&bars->v_empty[r]), 1);
+    }
+    mbar_init(smem_u32(&bars->ml_full), 128);
+    mbar_init(smem_u32(&bars->done), 1);
+    bars->abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(
+                     smem_u32(&bars->tmem_base)));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem_base;
+  asm volatile("griddepcontrol.launch_dependents;");
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    return mbar_wait(smem_u32(bar), parity, abort_flag, a.status, a.wait_limit_ns);
+  };
+
+  // Register split of the launch's 384 x 168: 128 x 72 + 256 x 216.
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 0) {
+      // ------------------------------------------------------- TMA producer
+      if (lane == 0) {
+        SegIter it(a.p);
+        Seg s;
+        int ec = 0, r = 0, issued = 0;
+        uint32_t ph = 0;
+        int qn[2] = {0, 0};
+        bool ok = true;
+        while (ok && it.next(a, s)) {
+          if (s.n == 0) continue;
+          const bool act1 = !SINGLE && s.row0 + 128 < s.row_end;
+          if (!SINGLE && dense) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              if (!ok || (t && !act1)) continue;
+              if (!wait(&bars->q_empty[t], (qn[t] & 1) ^ 1)) {
+                ok = false;
+                continue;
+              }
+              const uint32_t bar = smem_u32(&bars->q_full[t]), dst = smem_u32(sQ + t * kTileBytes);
+              mbar_expect_tx(bar, kTileBytes);
+              tma_load_4d(dst, &tm_q, bar, 0, s.row0 + 128 * t, s.h * a.q_h, s.b * a.q_b);
+              tma_load_4d(dst + kHalfBytes, &tm_q, bar, 64, s.row0 + 128 * t, s.h * a.q_h, s.b * a.q_b);
+              ++qn[t];
+            }
+          }
+          for (int i = 0; ok && i < s.n; ++i) {
+            const int j = s.j0 + i;
+            int info;
+            if (SINGLE) {
+              const int t = ec & 1;
+              info = (1 << t) | (i < 2 ? 1 << (kFirst + t) : 0) | (i >= s.n - 2 ? 1 << (kLast + t) : 0) |
+                     (i == 0 ? kSegFirst : 0) | (i == s.n - 1 ? kSegLast : 0);
+            } else {
+              const int act = act1 ? 3 : 1;
+              info = act | (i == 0 ? act << kFirst : 0) | (i == s.n - 1 ? act << kLast : 0);
+            }
+            const bool pre = j < s.npre;
+            // value rows past the member's length hold whatever the caller
+            // left there, and 0 x NaN would reach the result: the issuer
+            // clears them (TMA itself clears rows past the operand's end)
+            const int valid = SegIter::valid(a, s, j);
+            if (!pre && valid < 128 && s.len < a.n.kv_len) info |= valid << kZeroShift;
+            if (!wait(&bars->k_empty[r], ph ^ 1) || !wait(&bars->v_empty[r], ph ^ 1)) {
+              ok = false;
+              break;
+            }
+            const uint32_t bar = smem_u32(&bars->kv_full[r]);
+            bars->info[ec & 15] = info;
+            mbar_expect_tx(bar, 2 * kTileBytes);
+            const uint32_t dk = smem_u32(sKV + 2 * r * kTileBytes), dv = dk + kTileBytes;
+            if (pre) {
+              tma_load_4d(dk, &tm_pk, bar, 0, 128 * j, s.hk * a.pk_h, 0);
+              tma_load_4d(dk + kHalfBytes, &tm_pk, bar, 64, 128 * j, s.hk * a.pk_h, 0);
+              tma_load_4d(dv, &tm_pv, bar, 0, 128 * j, s.hk * a.pv_h, 0);
+              tma_load_4d(dv + kHalfBytes, &tm_pv, bar, 64, 128 * j, s.hk * a.pv_h, 0);
+            } else {
+              const int tok = 128 * (j - s.npre);
+              tma_load_4d(dk, &tm_k, bar, 0, tok, s.hk * a.k_h, s.b * a.k_b);
+              tma_load_4d(dk + kHalfBytes, &tm_k, bar, 64, tok, s.hk * a.k_h, s.b * a.k_b);
+              tma_load_4d(dv, &tm_v, bar, 0, tok, s.hk * a.v_h, s.b * a.v_b);
+              tma_load_4d(dv + kHalfBytes, &tm_v, bar, 64, tok, s.hk * a.v_h, s.b * a.v_b);
+            }
+            ++issued;
+            ++ec;
+            if (++r == L::kRing) {
+              r = 0;
+              ph ^= 1;
+            }
+          }
+        }
+        if (ok && wait(&bars->k_empty[r], ph ^ 1) && wait(&bars->v_empty[r], ph ^ 1)) {
+          bars->info[ec & 15] = kEnd;
+          mbar_arrive(smem_u32(&bars->kv_full[r]));
+        } else {
+          // abort: every load in flight lands before anyone may exit
+          volatile int32_t zero = 0;
+          for (int e = max(0, issued - L::kRing); e < issued; ++e)
+            mbar_wait(smem_u32(&bars->kv_full[e % L::kRing]), (e / L::kRing) & 1, &zero, nullptr);
+          if (dense)
+            for (int t = 0; t < 2; ++t)
+              if (qn[t]) mbar_wait(smem_u32(&bars->q_full[t]), (qn[t] - 1) & 1, &zero, nullptr);
+        }
+      }
+    } else if (warp == 1) {
+      // ------------------------------------------------------------ MMA issuer
+      // Per entry and half: the PV of the half's previous entry (its P is
+      // ready once its softmax arrives), then its S of this entry, so that
+      // the halves alternate between tensor pipe and softmax.
+      auto iwait = [&](uint64_t* bar, uint32_t par) -> bool {
+        int got = 0;
+        if (lane == 0) got = wait(bar, par) ? 1 : 0;
+        return __shfl_sync(0xffffffff, got, 0) != 0;
+      };
+      int pend0 = -1, pend1 = -1;    // entry whose PV is due
+      int pr0 = 0, pr1 = 0;          // its ring slot
+      int pf0 = 0, pf1 = 0;          // bit 0 first, bit 1 last of its segment
+      int ns0 = 0, ns1 = 0;          // S issued
+      int no0 = 0, no1 = 0;          // segments begun (O in use)
+      int nq0 = 0, nq1 = 0;          // Q tiles taken
+      int ec = 0, r = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      using T0 = std::integral_constant<int, 0>;
+      using T1 = std::integral_constant<int, 1>;
+      auto issue_pv = [&](auto tile) -> bool {
+        constexpr int t = decltype(tile)::value;
+        int& pend = t == 0 ? pend0 : pend1;
+        int& no = t == 0 ? no0 : no1;
+        const int pr = t == 0 ? pr0 : pr1, pf = t == 0 ? pf0 : pf1, ns = t == 0 ? ns0 : ns1;
+        const int other = t == 0 ? pend1 : pend0;
+        if (pf & 1) {  // the epilogue of the half's last segment has read O
+          if (no > 0 && !iwait(&bars->o_empty[t], (no - 1) & 1)) return false;
+          ++no;
+        }
+        if (!iwait(&bars->p_half[t], (ns - 1) & 1)) return false;
+        tc_fence_after();
+        const uint64_t vdesc = smem_desc(smem_u32(sKV + (2 * pr + 1) * kTileBytes), kHalfBytes, 1024);
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) {
+          if (kk == 6) {
+            if (!iwait(&bars->p_full[t], (ns - 1) & 1)) return false;
+            tc_fence_after();
+          }
+          mma_ts_w(tmem + 256 * t + 128, tmem + 256 * t + kk * 8, vdesc + (uint64_t)((kk * 2048) >> 4), kIdPV,
+                   (!(pf & 1) || kk > 0) ? 1u : 0u);
+        }
+        if (pf & 2) tc_commit_w(smem_u32(&bars->o_full[t]));
+        if (other != pend) tc_commit_w(smem_u32(&bars->v_empty[pr]));
+        pend = -1;
+        return true;
+      };
+      auto issue_s = [&](auto tile, int info) -> bool {
+        constexpr int t = decltype(tile)::value;
+        if (!SINGLE && (info & (1 << (kFirst + t)))) {
+          int& nq = t == 0 ? nq0 : nq1;
+          if (!iwait(&bars->q_full[t], nq & 1)) return false;
+          tc_fence_after();
+          ++nq;
+        }
+        const uint64_t qdesc = smem_desc(smem_u32(sQ + (SINGLE ? 0 : t) * kTileBytes), 16, 1024);
+        const uint64_t kdesc = smem_desc(smem_u32(sKV + 2 * r * kTileBytes), 16, 1024);
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) {
+          const uint32_t off = (kk >> 2) * kHalfBytes + (kk & 3) * 32;
+          mma_ss_w(tmem + 256 * t, qdesc + (uint64_t)(off >> 4), kdesc + (uint64_t)(off >> 4), kIdS, kk > 0 ? 1u : 0u);
+        }
+        tc_commit_w(smem_u32(&bars->s_full[t]));
+        if (!SINGLE && (info & (1 << (kLast + t)))) tc_commit_w(smem_u32(&bars->q_empty[t]));
+        (t == 0 ? pend0 : pend1) = ec;
+        (t == 0 ? pr0 : pr1) = r;
+        (t == 0 ? pf0 : pf1) = ((info >> (kFirst + t)) & 1) | (((info >> (kLast + t)) & 1) << 1);
+        ++(t == 0 ? ns0 : ns1);
+        return true;
+      };
+      while (true) {
+        if (SINGLE) {
+          if (ec & 1) ok = pend1 < 0 || issue_pv(T1{});
+          else ok = pend0 < 0 || issue_pv(T0{});
+        } else {
+          ok = pend0 < 0 || issue_pv(T0{});
+        }
+        if (!ok || !iwait(&bars->kv_full[r], ph)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const int info = ((volatile int32_t*)bars->info)[ec & 15];
+        if (info & kEnd) break;
+        if (info >> kZeroShift) {
+          // rows [valid, 128) of V; a row is 128 bytes of either half tile
+          uint4* v = reinterpret_cast<uint4*>(sKV + (2 * r + 1) * kTileBytes);
+          const int lo = (info >> kZeroShift) * 8;
+          for (int x = lo + lane; x < 1024; x += 32) v[x] = v[1024 + x] = make_uint4(0, 0, 0, 0);
+          fence_async_shared();
+          __syncwarp();
+        }
+        if (SINGLE && (info & kSegFirst)) {
+          if (!iwait(&bars->q_full[0], nq0 & 1)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          ++nq0;
+        }
+        if (info & 1) ok = issue_s(T0{}, info);
+        if (!SINGLE && ok && pend1 >= 0) ok = issue_pv(T1{});
+        if (ok && (info & 2)) ok = issue_s(T1{}, info);
+        if (!ok) break;
+        tc_commit_w(smem_u32(&bars->k_empty[r]));
+        if (SINGLE && (info & kSegLast)) tc_commit_w(smem_u32(&bars->q_empty[0]));
+        ++ec;
+        if (++r == L::kRing) {
+          r = 0;
+          ph ^= 1;
+        }
+      }
+      if (ok && pend0 >= 0) ok = issue_pv(T0{});
+      if (ok && pend1 >= 0) ok = issue_pv(T1{});
+      // aborted or not: MMAs retire in order, so this covers all of them
+      tc_commit_w(smem_u32(&bars->done));
+    } else if (!dense) {
+      // -------------------------------------------- gather of folded Q rows
+      // 16 lanes take a row, 4 rows a pass of the 64 threads; rows past the
+      // block are zero.  Swizzle: 16-byte chunk c of row r sits at c ^ (r & 7).
+      const int g = threadIdx.x - 64, c = g & 15;
+      SegIter it(a.p);
+      Seg s;
+      int qn[2] = {0, 0};
+      bool ok = true;
+      while (ok && it.next(a, s)) {
+        if (s.n == 0) continue;
+#pragma unroll
+        for (int t = 0; t < L::kQTiles; ++t) {
+          if (!ok || (t && s.row0 + 128 >= s.row_end)) continue;
+          if (!wait(&bars->q_empty[t], (qn[t] & 1) ^ 1)) {
+            ok = false;
+            continue;
+          }
+          ++qn[t];
+          uint8_t* dst = sQ + t * kTileBytes + (c >> 3) * kHalfBytes;
+          for (int r0 = g >> 4; r0 < 128; r0 += 32) {
+            uint4 v[8];
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+              const int row = s.row0 + 128 * t + r0 + 4 * x;
+              v[x] = make_uint4(0, 0, 0, 0);
+              if (row < s.row_end) {
+                const int tok = row / a.n.group, b = tok / a.n.q_len;
+                v[x] = *reinterpret_cast<const uint4*>(
+                    a.q.at(b, tok - b * a.n.q_len, s.hk * a.n.group + (row - tok * a.n.group)) + 8 * c);
+              }
+            }
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+              const int r = r0 + 4 * x;
+              *reinterpret_cast<uint4*>(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[x];
+            }
+          }
+          fence_async_shared();
+          mbar_arrive(smem_u32(&bars->q_full[t]));
+        }
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    // ----------------------------------------------------- softmax + epilogue
+    const int t = (warp - 4) >> 2, q = warp & 3;
+    const int r = 32 * q + lane;  // row of the tile = TMEM lane
+    const uint32_t lane_base = tmem + ((uint32_t)(32 * q) << 16);
+    const uint32_t tS = lane_base + 256 * t, tO = tS + 128;
+    const float sl2 = a.scale_log2;
+    const uint64_t sl2x2 = dup2(sl2);
+    SegIter it(a.p);
+    Seg s;
+    int ec = 0, ns = 0, no = 0, no1 = 0, nml = 0;
+    bool ok = true;
+    while (ok && it.next(a, s)) {
+      const int row = s.row0 + (SINGLE ? 0 : 128 * t) + r;
+      const int i0 = SINGLE ? ((ec ^ t) & 1) : 0;
+      const int step = SINGLE ? 2 : 1;
+      const int nt = SINGLE ? (s.n - i0 + 1) / 2 : (s.row0 + 128 * t < s.row_end ? s.n : 0);
+      ec += s.n;
+      float m = -1e30f, l = 0.f;
+      for (int x = 0; x < nt; ++x) {
+        const int valid = SegIter::valid(a, s, s.j0 + i0 + x * step);
+        if (!wait(&bars->s_full[t], ns & 1)) {
+          ok = false;
+          break;
+        }
+        ++ns;
+        tc_fence_after();
+        uint32_t v[128];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) H3_TMEM_LD16(tS + 16 * c, (&v[16 * c]));
+        tmem_wait_ld();
+        if (valid < 128) {
+#pragma unroll
+          for (int c = 0; c < 128; ++c)
+            if (c >= valid) v[c] = __float_as_uint(-INFINITY);
+        }
+        float mxa[8];
+#pragma unroll
+        for (int g = 0; g < 8; ++g) {
+          float w = __uint_as_float(v[16 * g]);
+#pragma unroll
+          for (int c = 1; c < 15; c += 2)
+            w = max3(w, __uint_as_float(v[16 * g + c]), __uint_as_float(v[16 * g + c + 1]));
+          mxa[g] = fmaxf(w, __uint_as_float(v[16 * g + 15]));
+        }
+        const float mx = max3(max3(mxa[0], mxa[1], mxa[2]), max3(mxa[3], mxa[4], mxa[5]), fmaxf(mxa[6], mxa[7]));
+        // finite even where every logit so far is -inf (its weights are then 0)
+        const float mxs = fmaxf(mx * sl2, -1e30f);
+        // the running maximum moves only when the new one is over 8 above it
+        // (a factor 256 in the weights), so O is rarely rescaled
+        const bool need = x > 0 && mxs > m + 8.0f;
+        if (x == 0) m = mxs;
+        if (__any_sync(0xffffffff, need)) {
+          const float f = need ? ex2(m - mxs) : 1.0f;
+          if (need) {
+            l *= f;
+            m = mxs;
+          }
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            uint32_t o[16];
+            H3_TMEM_LD16(tO + 16 * c, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            H3_TMEM_ST16(tO + 16 * c, o);
+          }
+        }
+        const uint64_t negm = dup2(-m);
+        uint64_t sum2 = 0;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float x0, x1;
+            fma2(x0, x1, v[32 * c + 2 * e], v[32 * c + 2 * e + 1], sl2x2, negm);
+            const float p0 = ex2(x0), p1 = ex2(x1);
+            sum2 = add2(sum2, p0, p1);
+            pk[e] = pack_bf16(p0, p1);
+          }
+          H3_TMEM_ST16(tS + 16 * c, pk);
+          if (c == 2) {  // keys 0-95 of P are in TMEM: the first six PV steps may start
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(smem_u32(&bars->p_half[t]));
+          }
+        }
+        l += __uint_as_float((uint32_t)sum2) + __uint_as_float((uint32_t)(sum2 >> 32));
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(smem_u32(&bars->p_full[t]));
+      }
+      if (!ok) break;
+      // ---------------------------------------------------------- epilogue
+      bool has0 = nt > 0, has1 = false;  // this half's O; single mode: half 1's
+      float w0 = 1.f, w1 = 0.f;
+      if (SINGLE) {
+        if (t == 1) {
+          if (nt > 0) {
+            // half 0 has read the last segment's
+            if (nml > 0 && !wait(&bars->o_empty[1], (nml - 1) & 1)) break;
+            bars->ml[r] = make_float2(m, l);
+            ++nml;
+            mbar_arrive(smem_u32(&bars->ml_full));
+          }
+          continue;
+        }
+        has1 = s.n - nt > 0;
+        if (has1) {
+          if (!wait(&bars->ml_full, nml & 1)) break;
+          const float2 ml = bars->ml[r];
+          ++nml;
+          const float top = fmaxf(m, ml.x);
+          w0 = ex2(m - top);
+          w1 = ex2(ml.x - top);
+          m = top;
+          l = l * w0 + ml.y * w1;
+          if (!wait(&bars->o_full[1], no1 & 1)) break;
+          ++no1;
+        }
+      }
+      if (has0) {
+        if (!wait(&bars->o_full[t], no & 1)) break;
+        ++no;
+      }
+      tc_fence_after();
+      const bool live = row < s.row_end;
+      int tok = row, b = s.b, h = s.h;
+      if (!dense) {
+        const int bt = row / a.n.group;
+        b = bt / a.n.q_len;
+        tok = bt - b * a.n.q_len;
+        h = s.hk * a.n.group + (row - bt * a.n.group);
+      }
+      const int64_t rid = dense ? ((int64_t)b * a.n.heads + h) * a.n.q_len + tok
+                                : (int64_t)s.hk * a.p.fold_rows + row;
+      const int64_t part = rid * a.p.slots + s.slot;
+      uint16_t* go = a.out.p + (live ? b * a.out.b + tok * a.out.t + h * a.out.h : 0);
+      if (s.direct) {
+        const float inv = 1.0f / fmaxf(l, 1e-30f);
+        w0 *= inv;
+        w1 *= inv;
+        if (live && a.lse)
+          a.lse[((int64_t)b * a.n.heads + h) * a.n.q_len + tok] =
+              l == 0.f ? -INFINITY : (m + lg2(l)) * 0.69314718055994531f;
+      } else if (live) {
+        a.part_ml[part] = make_float2(m, l);
+      }
+      if (has0 || has1 || s.direct) {
+#pragma unroll 2
+        for (int c = 0; c < 8; ++c) {
+          uint32_t o0[16], o1[16];
+          float o[16];
+          if (has0) H3_TMEM_LD16(tO + 16 * c, o0);
+          if (has1) H3_TMEM_LD16(tO + 256 + 16 * c, o1);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            o[e] = has0 ? __uint_as_float(o0[e]) * w0 : 0.f;
+            if (has1) o[e] += __uint_as_float(o1[e]) * w1;
+          }
+          if (live && s.direct) {
+            store_row32(go + 16 * c, o, 1.0f);
+          } else if (live) {
+            float4* po = reinterpret_cast<float4*>(a.part_o + part * 128 + 16 * c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) po[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          }
+        }
+      }
+      tc_fence_before();
+      if (has0) mbar_arrive(smem_u32(&bars->o_empty[t]));
+      if (has1) mbar_arrive(smem_u32(&bars->o_empty[1]));
+    }
+  }
+
+  // ------------------------------------------------------------------ exit
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 2) {
+    if (bars->abort) {  // no MMA may still write TMEM when it is released
+      volatile int32_t zero = 0;
+      mbar_wait(smem_u32(&bars->done), 0, &zero, nullptr);
+      __syncwarp();
+    }
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  }
+}
+
+// Joins the partial results of a row: o = sum 2^(m_s - M) o_s / sum 2^(m_s - M) l_s.
+// One warp a row, lane l holds channels 4l..4l+3.
+__global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ FwdArgs a) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const FwdPlan& p = a.p;
+  const int lane = threadIdx.x & 31;
+  const int64_t rows = (int64_t)a.n.batch * a.n.heads * a.n.q_len;
+  for (int64_t row = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5; row < rows;
+       row += ((int64_t)gridDim.x * blockDim.x) >> 5) {
+    const int tok = (int)(row % a.n.q_len);
+    const int64_t bh = row / a.n.q_len;
+    const int h = (int)(bh % a.n.heads), b = (int)(bh / a.n.heads), hk = h / a.n.group;
+    int64_t rid, start_o;      // partial row; first position of its own unit in the linear split
+    int np = 0, no = 0;        // partial results of either source
+    if (p.mode == kDense) {
+      rid = row;
+      start_o = (bh * p.per_o + tok / p.unit_rows) * p.tiles_o;
+    } else {
+      const int in_b = tok * a.n.group + (h - hk * a.n.group);
+      const int fr = b * a.n.q_len * a.n.group + in_b;
+      rid = (int64_t)hk * p.fold_rows + fr;
+      start_o = (int64_t)p.units_p * p.tiles_p +
+                (((int64_t)b * a.n.kv_heads + hk) * p.per_o + in_b / p.unit_rows) * p.tiles_o;
+      if (p.units_p) {
+        const int64_t start = ((int64_t)hk * p.per_p + fr / p.unit_rows) * p.tiles_p;
+        np = p.tpc ? (int)((start + p.tiles_p - 1) / p.tpc - start / p.tpc) + 1 : 1;
+      }
+    }
+    if (p.units_o) no = p.tpc ? (int)((start_o + p.tiles_o - 1) / p.tpc - start_o / p.tpc) + 1 : 1;
+    if (np + no == 1) continue;  // written by its unit
+    const float2* ml = a.part_ml + rid * p.slots;
+    float m = -1e30f;
+    for (int i = lane; i < np + no; i += 32) m = fmaxf(m, ml[i < np ? i : p.slots_p + i - np].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int i = 0; i < np + no; ++i) {
+      const int slot = i < np ? i : p.slots_p + i - np;
+      const float2 e = ml[slot];
+      if (e.y == 0.f) continue;  // no keys: its o was not written
+      const float w = ex2(e.x - m);
+      const float4 v = *reinterpret_cast<const float4*>(a.part_o + (rid * p.slots + slot) * 128 + 4 * lane);
+      l += e.y * w;
+      acc.x = fmaf(v.x, w, acc.x);
+      acc.y = fmaf(v.y, w, acc.y);
+      acc.z = fmaf(v.z, w, acc.z);
+      acc.w = fmaf(v.w, w, acc.w);
+    }
+    const float inv = 1.0f / fmaxf(l, 1e-30f);
+    *reinterpret_cast<uint2*>(a.out.at(b, tok, h) + 4 * lane) =
+        make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+    if (a.lse && lane == 0) a.lse[row] = l == 0.f ? -INFINITY : (m + lg2(l)) * 0.69314718055994531f;
+  }
+}
+
+// No keys at all: zeros and -inf.
+__global__ void __launch_bounds__(256) no_keys_kernel(CrossShape n, Rows out, float* lse) {
+  const int64_t rows = (int64_t)n.batch * n.heads * n.q_len;
+  for (int64_t row = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5; row < rows;
+       row += ((int64_t)gridDim.x * blockDim.x) >> 5) {
+    const int64_t bh = row / n.q_len;
+    *reinterpret_cast<uint2*>(out.at(bh / n.heads, row % n.q_len, bh % n.heads) + 4 * (threadIdx.x & 31)) =
+        make_uint2(0, 0);
+    if (lse && (threadIdx.x & 31) == 0) lse[row] = -INFINITY;
+  }
+}
+
+FwdPlan plan_fwd(const CrossShape& n) {
+  FwdPlan p{};
+  p.np = (n.prefix_len + 127) / 128;
+  p.nb = (n.kv_len + 127) / 128;
+  if (n.q_len >= 128) {
+    p.mode = kDense;
+    p.unit_rows = 256;
+    p.per_o = (n.q_len + 255) / 256;
+    p.units_o = p.np + p.nb ? n.batch * n.heads * p.per_o : 0;
+    p.tiles_o = p.np + p.nb;
+  } else {
+    const int own_rows = n.q_len * n.group;
+    p.fold_rows = n.batch * own_rows;
+    p.mode = (p.np ? p.fold_rows : own_rows) <= 128 ? kSingle : kDual;
+    p.unit_rows = p.mode == kSingle ? 128 : 256;
+    p.per_p = (p.fold_rows + p.unit_rows - 1) / p.unit_rows;
+    p.per_o = (own_rows + p.unit_rows - 1) / p.unit_rows;
+    p.units_p = p.np ? n.kv_heads * p.per_p : 0;
+    p.units_o = p.nb ? n.batch * n.kv_heads * p.per_o : 0;
+    p.tiles_p = p.np;
+    p.tiles_o = p.nb;
+  }
+  const int64_t units = (int64_t)p.units_p + p.units_o;
+  const int64_t total = (int64_t)p.units_p * p.tiles_p + (int64_t)p.units_o * p.tiles_o;
+  const int64_t longest = p.units_p ? (p.tiles_p > p.tiles_o ? p.tiles_p : p.tiles_o) : p.tiles_o;
+  const int64_t share = (total + kSms - 1) / kSms;
+  // whole units in turn cost up to one unit more than the even share; the
+  // linear split costs the partial results' traffic and the combine launch,
+  // about the time of 4 tiles
+  if ((units + kSms - 1) / kSms * longest > share + share / 10 + 4) p.tpc = (int32_t)share;
+  p.ctas = (int32_t)(p.tpc ? (total + p.tpc - 1) / p.tpc : (units < kSms ? units : kSms));
+  p.slots_p = p.units_p ? (p.tpc ? (p.tiles_p - 1) / p.tpc + 2 : 1) : 0;
+  p.slots = p.slots_p + (p.units_o ? (p.tpc ? (p.tiles_o - 1) / p.tpc + 2 : 1) : 0);
+  p.combine = (p.units_p && p.units_o) || (p.tpc && p.tpc % (int32_t)longest != 0);
+  p.part_rows = p.combine ? (p.mode == kDense ? (int64_t)n.batch * n.heads * n.q_len : (int64_t)n.kv_heads * p.fold_rows)
+                          : 0;
+  return p;
+}
+
+// (d, token, head, batch) map of an operand, boxes of 64 x 128; a broadcast
+// axis has one element.
+bool make_map4(CUtensorMap* m, const Rows& r, int tokens, int heads, int batch, std::string* err) {
+  EncodeTiledFn enc = get_encode();
+  if (!enc) {
+    *err += "cuTensorMapEncodeTiled unavailable; ";
+    return false;
+  }
+  cuuint64_t dims[4] = {128, (cuuint64_t)tokens, r.h ? (cuuint64_t)heads : 1, r.b ? (cuuint64_t)batch : 1};
+  cuuint64_t strides[3] = {r.t ? (cuuint64_t)r.t * 2 : 256, r.h ? (cuuint64_t)r.h * 2 : 256,
+                           r.b ? (cuuint64_t)r.b * 2 : 256};
+  cuuint32_t box[4] = {64, 128, 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult res = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, r.p, dims, strides, box, estr,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (res != CUDA_SUCCESS) {
+    *err += "cuTensorMapEncodeTiled failed (" + std::to_string((int)res) + "); ";
+    return false;
+  }
+  return true;
+}
+
+template <bool SINGLE>
+cudaError_t launch_fwd(const FwdArgs& a, const CUtensorMap* m, cudaStream_t s) {
+  static std::once_flag once[64];
+  static cudaError_t set_result[64];
+  int dev = 0;
+  cudaError_t de = cudaGetDevice(&dev);
+  if (de != cudaSuccess) return de;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  std::call_once(once[dev], [dev] {
+    cudaError_t e =
+        cudaFuncSetAttribute(cross_fwd_kernel<SINGLE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<SINGLE>());
+    // the register split needs exactly 168 a thread at launch
+    cudaFuncAttributes fa;
+    if (e == cudaSuccess) e = cudaFuncGetAttributes(&fa, cross_fwd_kernel<SINGLE>);
+    if (e == cudaSuccess && fa.numRegs != 168) e = cudaErrorInvalidConfiguration;
+    set_result[dev] = e;
+  });
+  if (set_result[dev] != cudaSuccess) return set_result[dev];
+  cross_fwd_kernel<SINGLE><<<a.p.ctas, kThreads, smem_bytes<SINGLE>(), s>>>(m[0], m[1], m[2], m[3], m[4], a);
+  return cudaGetLastError();
+}
+
+unsigned warps_grid(int64_t rows) { return (unsigned)((rows + 7) / 8 < kSms * 8 ? (rows + 7) / 8 : kSms * 8); }
+
+}  // namespace
+
+size_t cross_fwd_workspace(const CrossShape& n) {
+  if (!n.batch || !n.q_len) return 0;
+  const FwdPlan p = plan_fwd(n);
+  return (size_t)(p.part_rows * p.slots) * (128 * sizeof(float) + sizeof(float2));
+}
+
+cudaError_t launch_cross_fwd(const CrossLaunch& L, cudaStream_t s, std::string* err) {
+  const int64_t rows = (int64_t)L.n.batch * L.n.heads * L.n.q_len;
+  if (rows == 0) return cudaSuccess;
+  FwdArgs a{};
+  a.n = L.n;
+  a.p = plan_fwd(L.n);
+  if (a.p.units_p + a.p.units_o == 0) {
+    no_keys_kernel<<<warps_grid(rows), 256, 0, s>>>(L.n, L.out, L.lse);
+    return cudaGetLastError();
+  }
+  a.q = L.q;
+  a.out = L.out;
+  a.kv_lens = L.kv_lens;
+  a.lse = L.lse;
+  a.scale_log2 = L.scale * 1.4426950408889634f;
+  a.part_o = (float*)L.ws;
+  a.part_ml = (float2*)(a.part_o + a.p.part_rows * a.p.slots * 128);
+  a.status = L.status;
+  a.wait_limit_ns = L.wait_limit_ns;
+  a.q_b = L.q.b != 0, a.q_h = L.q.h != 0;
+  a.k_b = L.k.b != 0, a.k_h = L.k.h != 0;
+  a.v_b = L.v.b != 0, a.v_h = L.v.h != 0;
+  a.pk_h = L.pk.h != 0, a.pv_h = L.pv.h != 0;
+  CUtensorMap m[5] = {};
+  const CrossShape& n = L.n;
+  if (a.p.mode == kDense && !make_map4(&m[0], L.q, n.q_len, n.heads, n.batch, err)) return cudaErrorInvalidValue;
+  if (n.kv_len && (!make_map4(&m[1], L.k, n.kv_len, n.kv_heads, n.batch, err) ||
+                   !make_map4(&m[2], L.v, n.kv_len, n.kv_heads, n.batch, err)))
+    return cudaErrorInvalidValue;
+  if (n.prefix_len && (!make_map4(&m[3], L.pk, n.prefix_len, n.kv_heads, 1, err) ||
+                       !make_map4(&m[4], L.pv, n.prefix_len, n.kv_heads, 1, err)))
+    return cudaErrorInvalidValue;
+  cudaError_t e = a.p.mode == kSingle ? launch_fwd<true>(a, m, s) : launch_fwd<false>(a, m, s);
+  if (e != cudaSuccess || !a.p.combine) return e;
+  // placed while the attention kernel runs; waits for its end before it reads
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(warps_grid(rows));
+  cfg.blockDim = dim3(256);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, combine_kernel, a);
+}
+
+}  // namespace h3
