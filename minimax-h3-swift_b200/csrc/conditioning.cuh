@@ -2,7 +2,7 @@
 // q/k norm): normalised operands and the launchers of the kernel files.
 #pragma once
 
-#include "common.cuh"
+#include "tcgen05.cuh"
 
 namespace h3 {
 
@@ -32,6 +32,29 @@ struct CrossLaunch {
 
 __device__ __forceinline__ int kv_len_of(const int32_t* kv_lens, int kv_len, int b) {
   return kv_lens ? max(0, min(kv_len, kv_lens[b])) : kv_len;
+}
+
+// (d, token, head, batch) map of an operand, boxes of 64 x 128; a broadcast
+// axis has one element.
+inline bool make_map4(CUtensorMap* m, const Rows& r, int tokens, int heads, int batch, std::string* err) {
+  EncodeTiledFn enc = get_encode();
+  if (!enc) {
+    *err += "cuTensorMapEncodeTiled unavailable; ";
+    return false;
+  }
+  cuuint64_t dims[4] = {128, (cuuint64_t)tokens, r.h ? (cuuint64_t)heads : 1, r.b ? (cuuint64_t)batch : 1};
+  cuuint64_t strides[3] = {r.t ? (cuuint64_t)r.t * 2 : 256, r.h ? (cuuint64_t)r.h * 2 : 256,
+                           r.b ? (cuuint64_t)r.b * 2 : 256};
+  cuuint32_t box[4] = {64, 128, 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult res = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, r.p, dims, strides, box, estr,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (res != CUDA_SUCCESS) {
+    *err += "cuTensorMapEncodeTiled failed (" + std::to_string((int)res) + "); ";
+    return false;
+  }
+  return true;
 }
 
 size_t cross_fwd_workspace(const CrossShape& n);

@@ -1,98 +1,868 @@
-// Gradient of cross attention: the plain kernels.  One warp per row, lane l holds channels 4l..4l+3; softmax
-// statistics and sums in fp32.
-#include <cmath>
+// Gradient of cross attention on the Blackwell tensor cores.
+//
+//   P = 2^(scale log2(e) q.k - lse2);  delta_i = do_i.o_i;  dS = P (do v^T - delta)
+//   dq = scale dS k;  dk = scale dS^T q;  dv = P^T do   (sums over the heads of a group)
+//
+// Two passes, so that every sum has one owner and a fixed order (no atomics):
+//   dq_kernel    a CTA holds 128 queries and walks the keys: S, dP, dq += dS K
+//   dkv_kernel   a CTA holds 128 keys and walks the queries of all heads of
+//                the group: S^T, dP^T, dv += P^T do, dk += dS^T Q
+// Seven products of 128x128x128 a tile pair instead of the five that a single
+// pass with atomics on dq would make.  P and dS enter their products in bf16
+// from TMEM (they never touch shared memory); sums are fp32.  dq_kernel also
+// writes delta and -lse2 for dkv_kernel, padded to whole blocks of queries
+// (-inf there, so that P is 0).
+//
+// Roles of a CTA's 12 warps: 0 TMA producer, 1 MMA issuer, 2 TMEM owner,
+// 4-7 and 8-11 elementwise: each warpgroup takes 64 of a tile's 128 columns of
+// every row (thread = row = TMEM lane).  Every wait is bounded (attn_tc.cu).
+//
+// dkv_kernel's work, all (key tile, query block) pairs in a row, is cut into
+// equal runs, one a CTA; a key tile that is cut leaves fp32 partial sums that
+// dkv_join_kernel adds in the order of the queries.
+#include <climits>
+#include <mutex>
 
 #include "conditioning.cuh"
 
 namespace h3 {
 namespace {
 
-struct F4 {
-  float v[4];
+constexpr int kThreads = 384;
+constexpr int kSms = 148;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr uint32_t kIdKK = idesc_bf16(false), kIdKM = idesc_bf16(true);
+
+struct BwdArgs {
+  CrossShape n;
+  Rows out, dout, dq, dk, dv;
+  const int32_t* kv_lens;
+  const float* lse;
+  float scale;
+  float* nl2;                 // [batch * heads, query blocks * 128]: -lse log2(e)
+  float* delta;
+  float* part;                // [ctas, 2 (head, tail), 2 (dk, dv), 128 * 128]
+  int32_t q_blocks;
+  int32_t* status;
+  uint64_t wait_limit_ns;
+  int32_t q_b, q_h, k_b, k_h, v_b, v_h, g_b, g_h;
 };
 
-__device__ __forceinline__ F4 load4(const uint16_t* p) {
-  const uint2 u = *reinterpret_cast<const uint2*>(p + 4 * (threadIdx.x & 31));
-  return {{__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
-           __uint_as_float(u.y & 0xffff0000u)}};
+__device__ __forceinline__ uint64_t pair2(uint32_t lo, uint32_t hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+  return r;
 }
 
-__device__ __forceinline__ void store4(uint16_t* p, const F4& f, float m) {
-  *reinterpret_cast<uint2*>(p + 4 * (threadIdx.x & 31)) =
-      make_uint2((uint32_t)f2bf(f.v[0] * m) | ((uint32_t)f2bf(f.v[1] * m) << 16),
-                 (uint32_t)f2bf(f.v[2] * m) | ((uint32_t)f2bf(f.v[3] * m) << 16));
+// (s0, s1) * k + b, two fp32 at a time
+__device__ __forceinline__ uint64_t fma_2(uint64_t a, uint64_t k, uint64_t b) {
+  uint64_t r;
+  asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(k), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul_2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float lo2(uint64_t v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float hi2(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
+
+__device__ __forceinline__ void tma_tile(uint32_t dst, const CUtensorMap* m, uint32_t bar, int tok, int h, int b) {
+  tma_load_4d(dst, m, bar, 0, tok, h, b);
+  tma_load_4d(dst + kHalfBytes, m, bar, 64, tok, h, b);
 }
 
-__device__ __forceinline__ float dot(const F4& a, const F4& b) {
-  float s = a.v[0] * b.v[0] + a.v[1] * b.v[1] + a.v[2] * b.v[2] + a.v[3] * b.v[3];
+// 512 bytes of a float array into shared memory
+__device__ __forceinline__ void bulk_512(uint32_t dst, const float* src, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], 512, [%2];" ::"r"(dst), "l"(src),
+      "r"(bar)
+      : "memory");
+}
+
+// D (+)= A B^T over 128 channels, A and B K-major tiles in shared memory
+__device__ __forceinline__ void mma_tile_ss(uint32_t d, uint32_t a, uint32_t b) {
+  const uint64_t da = smem_desc(a, 16, 1024), db = smem_desc(b, 16, 1024);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  return s;
-}
-
-__device__ __forceinline__ void axpy(F4& y, float a, const F4& x) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) y.v[i] = fmaf(a, x.v[i], y.v[i]);
-}
-
-// this warp's row numbers
-struct Walk {
-  int64_t i, step;
-  __device__ Walk()
-      : i(((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5), step(((int64_t)gridDim.x * blockDim.x) >> 5) {}
-};
-
-__global__ void __launch_bounds__(256) cross_dq_kernel(CrossLaunch a, float* delta) {
-  const CrossShape n = a.n;
-  for (Walk w; w.i < (int64_t)n.batch * n.heads * n.q_len; w.i += w.step) {
-    const int t = (int)(w.i % n.q_len), h = (int)(w.i / n.q_len % n.heads), b = (int)(w.i / n.q_len / n.heads);
-    const int hk = h / n.group, own = kv_len_of(a.kv_lens, n.kv_len, b);
-    const F4 q = load4(a.q.at(b, t, h)), g = load4(a.dout.at(b, t, h));
-    const float dl = dot(g, load4(a.out.at(b, t, h))), lse = own ? a.lse[w.i] : 0.f;
-    F4 dq{};
-    for (int j = 0; j < own; ++j) {
-      const F4 k = load4(a.k.at(b, j, hk));
-      const float p = expf(dot(q, k) * a.scale - lse);
-      axpy(dq, p * (dot(g, load4(a.v.at(b, j, hk))) - dl), k);
-    }
-    store4(a.dq.at(b, t, h), dq, a.scale);
-    if ((threadIdx.x & 31) == 0) delta[w.i] = dl;
+  for (int kk = 0; kk < 8; ++kk) {
+    const uint32_t off = (kk >> 2) * kHalfBytes + (kk & 3) * 32;
+    mma_ss_w(d, da + (uint64_t)(off >> 4), db + (uint64_t)(off >> 4), kIdKK, kk > 0 ? 1u : 0u);
   }
 }
 
-__global__ void __launch_bounds__(256) cross_dkv_kernel(CrossLaunch a, const float* delta) {
-  const CrossShape n = a.n;
-  for (Walk w; w.i < (int64_t)n.batch * n.kv_heads * n.kv_len; w.i += w.step) {
-    const int j = (int)(w.i % n.kv_len), hk = (int)(w.i / n.kv_len % n.kv_heads),
-              b = (int)(w.i / n.kv_len / n.kv_heads);
-    F4 dk{}, dv{};
-    if (j < kv_len_of(a.kv_lens, n.kv_len, b)) {
-      const F4 k = load4(a.k.at(b, j, hk)), v = load4(a.v.at(b, j, hk));
-      for (int h = hk * n.group; h < (hk + 1) * n.group; ++h)
-        for (int t = 0; t < n.q_len; ++t) {
-          const int64_t r = ((int64_t)b * n.heads + h) * n.q_len + t;
-          const F4 q = load4(a.q.at(b, t, h)), g = load4(a.dout.at(b, t, h));
-          const float p = expf(dot(q, k) * a.scale - a.lse[r]);
-          axpy(dv, p, g);
-          axpy(dk, p * (dot(g, v) - delta[r]), q);
+// D (+)= A B, A packed bf16 in TMEM (steps 0-3 at a0, 4-7 at a1), B a tile
+// with the summed axis along its rows
+__device__ __forceinline__ void mma_tile_ts(uint32_t d, uint32_t a0, uint32_t a1, uint32_t b, bool acc) {
+  const uint64_t db = smem_desc(b, kHalfBytes, 1024);
+#pragma unroll
+  for (int kk = 0; kk < 8; ++kk)
+    mma_ts_w(d, (kk < 4 ? a0 : a1) + (kk & 3) * 8, db + (uint64_t)((kk * 2048) >> 4), kIdKM, acc || kk > 0 ? 1u : 0u);
+}
+
+__device__ __forceinline__ void load64(uint32_t addr, uint32_t* v) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c) H3_TMEM_LD16(addr + 16 * c, (&v[16 * c]));
+  tmem_wait_ld();
+}
+
+enum { kFirst = 1, kLast = 2, kEnd = 4, kZeroShift = 8 };
+
+__device__ __forceinline__ uint32_t alloc_tmem(int warp, uint32_t* slot) {
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(slot)));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  return *slot;
+}
+
+// Common exit: no MMA may still write TMEM when it is released.
+__device__ __forceinline__ void release_tmem(int warp, uint32_t tmem, volatile int32_t* abort_flag, uint64_t* done) {
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 2) {
+    if (*abort_flag) {
+      volatile int32_t zero = 0;
+      mbar_wait(smem_u32(done), 0, &zero, nullptr);
+      __syncwarp();
+    }
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  }
+}
+
+// --------------------------------------------------------------------- dq
+// Shared memory: q and do of two units (128 KB), two K tiles, one V tile.
+// TMEM columns: dq 0, S 128, dP 256, dS (two buffers) 384 and 448.  Of block
+// e+1, S and dP run while block e is in the elementwise warps; dq of e follows.
+struct __align__(8) DqBarriers {
+  uint64_t qd_full[2], qd_empty[2];  // unit u on [u & 1]
+  uint64_t k_full[2], k_empty[2], v_full, v_empty;
+  uint64_t s_full, s_empty, dp_full, dp_empty, dq_full, dq_empty, red_full, done;
+  // block e on [e & 1]: S and dP of e + 1 are issued before the issuer waits
+  // for dS of e, so one barrier could complete twice before that wait
+  uint64_t ds_full[2];
+  uint32_t tmem_base;
+  int32_t abort;
+  int32_t info[8];
+  float red[2][128];                 // halves of delta
+};
+constexpr int kDqTiles = 7 * kTileBytes;
+constexpr int kDqSmem = kDqTiles + 1024 + (int)sizeof(DqBarriers);
+static_assert(kDqSmem <= 227 * 1024, "shared memory");
+
+struct DqUnit {
+  int b, h, t0, len, n;
+  __device__ DqUnit(const BwdArgs& a, int u) {
+    const int x = u / a.q_blocks;
+    t0 = (u - x * a.q_blocks) * 128;
+    b = x / a.n.heads;
+    h = x - b * a.n.heads;
+    len = kv_len_of(a.kv_lens, a.n.kv_len, b);
+    n = (len + 127) >> 7;
+  }
+};
+
+__global__ void __launch_bounds__(kThreads, 1)
+    dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+              const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_g,
+              const __grid_constant__ BwdArgs a, int units) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t *sQ = smem, *sG = smem + 2 * kTileBytes, *sK = smem + 4 * kTileBytes, *sV = smem + 6 * kTileBytes;
+  DqBarriers* bars = (DqBarriers*)(smem + kDqTiles);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile int32_t* abort_flag = &bars->abort;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&bars->qd_full[i]), 1);
+      mbar_init(smem_u32(&bars->qd_empty[i]), 257);  // the unit's last product and 256 readers of do
+      mbar_init(smem_u32(&bars->k_full[i]), 1);
+      mbar_init(smem_u32(&bars->k_empty[i]), 1);
+      mbar_init(smem_u32(&bars->ds_full[i]), 256);
+    }
+    mbar_init(smem_u32(&bars->v_full), 1);
+    mbar_init(smem_u32(&bars->v_empty), 1);
+    mbar_init(smem_u32(&bars->s_full), 1);
+    mbar_init(smem_u32(&bars->s_empty), 256);
+    mbar_init(smem_u32(&bars->dp_full), 1);
+    mbar_init(smem_u32(&bars->dp_empty), 256);
+    mbar_init(smem_u32(&bars->dq_full), 1);
+    mbar_init(smem_u32(&bars->dq_empty), 256);
+    mbar_init(smem_u32(&bars->red_full), 256);
+    mbar_init(smem_u32(&bars->done), 1);
+    bars->abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  const uint32_t tmem = alloc_tmem(warp, &bars->tmem_base);
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    return mbar_wait(smem_u32(bar), parity, abort_flag, a.status, a.wait_limit_ns);
+  };
+  // Register split of the launch's 384 x 168: 128 x 72 + 256 x 216.
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 0 && lane == 0) {
+      int e = 0, qn = 0;           // key tiles and units loaded
+      bool ok = true;
+      auto next_unit = [&](int u) {  // the next unit with keys
+        while (u < units && DqUnit(a, u).n == 0) u += gridDim.x;
+        return u;
+      };
+      auto load_q = [&](int u) {
+        const DqUnit x(a, u);
+        const int i = qn & 1;
+        if (!wait(&bars->qd_empty[i], ((qn >> 1) & 1) ^ 1)) return false;
+        const uint32_t bar = smem_u32(&bars->qd_full[i]);
+        mbar_expect_tx(bar, 2 * kTileBytes);
+        tma_tile(smem_u32(sQ + i * kTileBytes), &tm_q, bar, x.t0, x.h * a.q_h, x.b * a.q_b);
+        tma_tile(smem_u32(sG + i * kTileBytes), &tm_g, bar, x.t0, x.h * a.g_h, x.b * a.g_b);
+        ++qn;
+        return true;
+      };
+      int u = next_unit(blockIdx.x);
+      if (u < units) ok = load_q(u);
+      while (ok && u < units) {
+        const DqUnit x(a, u);
+        const int hk = x.h / a.n.group;
+        const int following = next_unit(u + gridDim.x);
+        for (int j = 0; ok && j < x.n; ++j, ++e) {
+          const int i = e & 1;
+          if (!wait(&bars->k_empty[i], ((e >> 1) & 1) ^ 1)) {
+            ok = false;
+            break;
+          }
+          const int valid = x.len - 128 * j;
+          // key rows past the member's length hold whatever the caller left
+          // there: the issuer clears them (0 x NaN would reach dq)
+          bars->info[e & 7] = (j == 0 ? kFirst : 0) | (j == x.n - 1 ? kLast : 0) |
+                              (valid < 128 && x.len < a.n.kv_len ? valid << kZeroShift : 0);
+          uint32_t bar = smem_u32(&bars->k_full[i]);
+          mbar_expect_tx(bar, kTileBytes);
+          tma_tile(smem_u32(sK + i * kTileBytes), &tm_k, bar, 128 * j, hk * a.k_h, x.b * a.k_b);
+          if (!wait(&bars->v_empty, (e & 1) ^ 1)) {
+            ++e;
+            ok = false;
+            break;
+          }
+          bar = smem_u32(&bars->v_full);
+          mbar_expect_tx(bar, kTileBytes);
+          tma_tile(smem_u32(sV), &tm_v, bar, 128 * j, hk * a.v_h, x.b * a.v_b);
+          if (j == 0 && following < units) ok = load_q(following);
         }
+        u = following;
+      }
+      if (ok && wait(&bars->k_empty[e & 1], ((e >> 1) & 1) ^ 1)) {
+        bars->info[e & 7] = kEnd;
+        mbar_arrive(smem_u32(&bars->k_full[e & 1]));
+      } else {  // abort: every load in flight lands before anyone may exit
+        volatile int32_t zero = 0;
+        for (int i = 0; i < 2; ++i) {
+          const int ke = e - 1 - ((e - 1 - i) & 1), qe = qn - 1 - ((qn - 1 - i) & 1);
+          if (ke >= 0) mbar_wait(smem_u32(&bars->k_full[i]), (ke >> 1) & 1, &zero, nullptr);
+          if (qe >= 0) mbar_wait(smem_u32(&bars->qd_full[i]), (qe >> 1) & 1, &zero, nullptr);
+        }
+        // of the last two V loads at least the older one was issued
+        if (e >= 2) mbar_wait(smem_u32(&bars->v_full), e & 1, &zero, nullptr, 1000000);
+        if (e >= 1) mbar_wait(smem_u32(&bars->v_full), (e - 1) & 1, &zero, nullptr, 1000000);
+      }
+    } else if (warp == 1) {
+      auto iwait = [&](uint64_t* bar, uint32_t par) -> bool {
+        int got = 0;
+        if (lane == 0) got = wait(bar, par) ? 1 : 0;
+        return __shfl_sync(0xffffffff, got, 0) != 0;
+      };
+      int e = 0, pinfo = 0, units_s = 0, units_q = 0;
+      bool ok = true;
+      auto issue_dq = [&](int p, int info) -> bool {  // dq += dS_p K_p
+        if (info & kFirst) {
+          if (units_q > 0 && !iwait(&bars->dq_empty, (units_q - 1) & 1)) return false;
+          ++units_q;
+        }
+        if (!iwait(&bars->ds_full[p & 1], (p >> 1) & 1)) return false;
+        tc_fence_after();
+        const uint32_t ds = tmem + 384 + 64 * (p & 1);
+        mma_tile_ts(tmem, ds, ds + 32, smem_u32(sK + (p & 1) * kTileBytes), !(info & kFirst));
+        tc_commit_w(smem_u32(&bars->k_empty[p & 1]));
+        if (info & kLast) tc_commit_w(smem_u32(&bars->dq_full));
+        return true;
+      };
+      while (true) {
+        const int i = e & 1;
+        ok = iwait(&bars->k_full[i], (e >> 1) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        const int info = ((volatile int32_t*)bars->info)[e & 7];
+        if (info & kEnd) break;
+        if (info >> kZeroShift) {
+          uint4* k = reinterpret_cast<uint4*>(sK + i * kTileBytes);
+          for (int x = (info >> kZeroShift) * 8 + lane; x < 1024; x += 32) k[x] = k[1024 + x] = make_uint4(0, 0, 0, 0);
+          fence_async_shared();
+          __syncwarp();
+        }
+        if (info & kFirst) {
+          ok = iwait(&bars->qd_full[units_s & 1], (units_s >> 1) & 1);
+          if (!ok) break;
+          ++units_s;
+        }
+        const int qi = (units_s - 1) & 1;
+        ok = e == 0 || iwait(&bars->s_empty, (e - 1) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        mma_tile_ss(tmem + 128, smem_u32(sQ + qi * kTileBytes), smem_u32(sK + i * kTileBytes));
+        tc_commit_w(smem_u32(&bars->s_full));
+        ok = iwait(&bars->v_full, e & 1) && (e == 0 || iwait(&bars->dp_empty, (e - 1) & 1));
+        if (!ok) break;
+        tc_fence_after();
+        mma_tile_ss(tmem + 256, smem_u32(sG + qi * kTileBytes), smem_u32(sV));
+        tc_commit_w(smem_u32(&bars->dp_full));
+        tc_commit_w(smem_u32(&bars->v_empty));
+        if (info & kLast) tc_commit_w(smem_u32(&bars->qd_empty[qi]));
+        ok = e == 0 || issue_dq(e - 1, pinfo);
+        if (!ok) break;
+        pinfo = info;
+        ++e;
+      }
+      if (ok && e > 0) issue_dq(e - 1, pinfo);
+      tc_commit_w(smem_u32(&bars->done));
     }
-    store4(a.dk.at(b, j, hk), dk, a.scale);
-    store4(a.dv.at(b, j, hk), dv, 1.f);
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    // one outcome a warp: the TMEM accesses need its lanes together
+    auto wait_w = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
+    const int w = (warp - 4) >> 2, q = warp & 3, r = 32 * q + lane;
+    const uint32_t lane_base = tmem + ((uint32_t)(32 * q) << 16);
+    const uint64_t sl2 = dup2(a.scale * kLog2e);
+    int e = 0, un = 0;
+    bool ok = true;
+    for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
+      const DqUnit x(a, u);
+      const int tok = x.t0 + r;
+      const bool live = tok < a.n.q_len;
+      uint4* go = reinterpret_cast<uint4*>(live ? a.dq.at(x.b, tok, x.h) + 64 * w : nullptr);
+      if (x.n == 0) {
+        if (live)
+#pragma unroll
+          for (int c = 0; c < 8; ++c) go[c] = make_uint4(0, 0, 0, 0);
+        continue;
+      }
+      // delta: this warpgroup's 64 channels, then both halves
+      const int64_t pad = ((int64_t)x.b * a.n.heads + x.h) * a.q_blocks * 128 + tok;
+      float nl2 = -INFINITY, half = 0.f;
+      uint4 o[8];
+      if (live) {
+        nl2 = a.lse[((int64_t)x.b * a.n.heads + x.h) * a.n.q_len + tok] * -kLog2e;
+        const uint4* po = reinterpret_cast<const uint4*>(a.out.at(x.b, tok, x.h) + 64 * w);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) o[c] = po[c];
+      }
+      if (!wait_w(&bars->qd_full[un & 1], (un >> 1) & 1)) break;
+      if (live) {
+        const uint8_t* pg = sG + (un & 1) * kTileBytes + w * kHalfBytes + r * 128;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const uint4 g = *reinterpret_cast<const uint4*>(pg + ((c ^ (r & 7)) << 4));
+          const uint32_t gw[4] = {g.x, g.y, g.z, g.w}, ow[4] = {o[c].x, o[c].y, o[c].z, o[c].w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            half = fmaf(__uint_as_float(gw[i] << 16), __uint_as_float(ow[i] << 16), half);
+            half = fmaf(__uint_as_float(gw[i] & 0xffff0000u), __uint_as_float(ow[i] & 0xffff0000u), half);
+          }
+        }
+      }
+      mbar_arrive(smem_u32(&bars->qd_empty[un & 1]));
+      // every reader of the last unit's halves arrived on ds_full before this
+      // thread saw that unit's dq_full
+      bars->red[w][r] = half;
+      mbar_arrive(smem_u32(&bars->red_full));
+      if (!wait_w(&bars->red_full, un & 1)) break;
+      const float delta = bars->red[0][r] + bars->red[1][r];
+      if (w == 0) {
+        a.nl2[pad] = nl2;
+        a.delta[pad] = delta;
+      }
+      const uint64_t nl2x2 = dup2(nl2), ndelta = dup2(-delta);
+      for (int j = 0; j < x.n; ++j, ++e) {
+        if (!wait_w(&bars->s_full, e & 1)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        uint32_t s[64];
+        load64(lane_base + 128 + 64 * w, s);
+        tc_fence_before();
+        mbar_arrive(smem_u32(&bars->s_empty));
+        float p[64];
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          const uint64_t v = fma_2(pair2(s[2 * c], s[2 * c + 1]), sl2, nl2x2);
+          p[2 * c] = ex2(lo2(v));
+          p[2 * c + 1] = ex2(hi2(v));
+        }
+        if (!wait_w(&bars->dp_full, e & 1)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        uint32_t d[64];
+        load64(lane_base + 256 + 64 * w, d);
+        tc_fence_before();
+        mbar_arrive(smem_u32(&bars->dp_empty));
+        const int valid = x.len - 128 * j - 64 * w;  // this half's
+        uint32_t pk[32];
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          const uint64_t v = mul_2(add_2(pair2(d[2 * c], d[2 * c + 1]), ndelta),
+                                   pair2(__float_as_uint(p[2 * c]), __float_as_uint(p[2 * c + 1])));
+          pk[c] = pack_bf16(lo2(v), hi2(v));
+        }
+        if (valid < 64) {  // keys past the length, whatever their values gave
+#pragma unroll
+          for (int c = 0; c < 32; ++c) pk[c] = 2 * c + 1 < valid ? pk[c] : 2 * c < valid ? pk[c] & 0xffffu : 0u;
+        }
+        const uint32_t ds = lane_base + 384 + 64 * (e & 1) + 32 * w;
+        H3_TMEM_ST16(ds, (&pk[0]));
+        H3_TMEM_ST16(ds + 16, (&pk[16]));
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(smem_u32(&bars->ds_full[e & 1]));
+      }
+      if (!ok || !wait_w(&bars->dq_full, un & 1)) break;
+      ++un;
+      tc_fence_after();
+      uint32_t v[64];
+      load64(lane_base + 64 * w, v);
+      tc_fence_before();
+      mbar_arrive(smem_u32(&bars->dq_empty));
+      if (live) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          uint32_t k[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            k[i] = pack_bf16(__uint_as_float(v[8 * c + 2 * i]) * a.scale, __uint_as_float(v[8 * c + 2 * i + 1]) * a.scale);
+          go[c] = make_uint4(k[0], k[1], k[2], k[3]);
+        }
+      }
+    }
+  }
+  release_tmem(warp, tmem, abort_flag, &bars->done);
+}
+
+// ------------------------------------------------------------------ dk, dv
+// Shared memory: K and V of the unit (64 KB), q and do of two query blocks
+// (128 KB) with their -lse2 and delta.  TMEM columns: dk 0, dv 128, S^T 256,
+// dP^T 384; a warpgroup writes its half of P^T (dS^T) over its own half of
+// S^T (dP^T), so neither waits for the other's loads.
+struct __align__(16) DkvBarriers {
+  float nl2[2][128], delta[2][128];
+  uint64_t kv_full, kv_empty;
+  uint64_t q_full[2], q_empty[2], g_empty[2];
+  uint64_t s_full, dp_full, p_full, ds_full, acc_full, acc_empty, done;
+  uint32_t tmem_base;
+  int32_t abort;
+  int32_t info[8];
+};
+constexpr int kDkvTiles = 6 * kTileBytes;
+constexpr int kDkvSmem = kDkvTiles + 1024 + (int)sizeof(DkvBarriers);
+
+// The run of (key tile, query block) pairs of one CTA, over key tiles that
+// hold valid keys: tile order member, key head, tile.
+struct DkvWalk {
+  int64_t pos, end;
+  int b, len, tiles;          // current member
+  int64_t base;               // its first position
+  int steps;                  // query blocks of a key tile: those of all heads of the group
+  // current segment
+  int hk, tile, it0, it1;
+  __device__ DkvWalk(const BwdArgs& a, int cta, int ctas) {
+    steps = a.n.group * a.q_blocks;
+    int64_t all = 0;
+    for (int i = 0; i < a.n.batch; ++i) all += (kv_len_of(a.kv_lens, a.n.kv_len, i) + 127) >> 7;
+    all *= (int64_t)a.n.kv_heads * steps;
+    const int64_t share = (all + ctas - 1) / ctas;
+    pos = min(all, share * cta);
+    end = min(all, pos + share);
+    b = -1;
+    base = 0;
+    len = tiles = 0;
+  }
+  __device__ bool next(const BwdArgs& a) {
+    if (pos >= end) return false;
+    while (b < 0 || pos >= base + (int64_t)tiles * a.n.kv_heads * steps) {
+      if (b >= 0) base += (int64_t)tiles * a.n.kv_heads * steps;
+      ++b;
+      len = kv_len_of(a.kv_lens, a.n.kv_len, b);
+      tiles = (len + 127) >> 7;
+    }
+    const int64_t off = pos - base;
+    const int u = (int)(off / steps);
+    hk = u / tiles;
+    tile = u - hk * tiles;
+    it0 = (int)(off - (int64_t)u * steps);
+    it1 = (int)min((int64_t)steps, it0 + (end - pos));
+    pos += it1 - it0;
+    return true;
+  }
+};
+
+__global__ void __launch_bounds__(kThreads, 1)
+    dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+               const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_g,
+               const __grid_constant__ BwdArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t *sK = smem, *sV = smem + kTileBytes, *sQ = smem + 2 * kTileBytes, *sG = smem + 4 * kTileBytes;
+  DkvBarriers* bars = (DkvBarriers*)(smem + kDkvTiles);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile int32_t* abort_flag = &bars->abort;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&bars->q_full[i]), 1);
+      mbar_init(smem_u32(&bars->q_empty[i]), 1);
+      mbar_init(smem_u32(&bars->g_empty[i]), 1);
+    }
+    mbar_init(smem_u32(&bars->kv_full), 1);
+    mbar_init(smem_u32(&bars->kv_empty), 1);
+    mbar_init(smem_u32(&bars->s_full), 1);
+    mbar_init(smem_u32(&bars->dp_full), 1);
+    mbar_init(smem_u32(&bars->p_full), 256);
+    mbar_init(smem_u32(&bars->ds_full), 256);
+    mbar_init(smem_u32(&bars->acc_full), 1);
+    mbar_init(smem_u32(&bars->acc_empty), 256);
+    mbar_init(smem_u32(&bars->done), 1);
+    bars->abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  const uint32_t tmem = alloc_tmem(warp, &bars->tmem_base);
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    return mbar_wait(smem_u32(bar), parity, abort_flag, a.status, a.wait_limit_ns);
+  };
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 0 && lane == 0) {
+      DkvWalk seg(a, blockIdx.x, gridDim.x);
+      int e = 0, sn = 0;           // query blocks and segments loaded
+      bool ok = true;
+      while (ok && seg.next(a)) {
+        if (!wait(&bars->kv_empty, (sn & 1) ^ 1)) {
+          ok = false;
+          break;
+        }
+        uint32_t bar = smem_u32(&bars->kv_full);
+        mbar_expect_tx(bar, 2 * kTileBytes);
+        tma_tile(smem_u32(sK), &tm_k, bar, 128 * seg.tile, seg.hk * a.k_h, seg.b * a.k_b);
+        tma_tile(smem_u32(sV), &tm_v, bar, 128 * seg.tile, seg.hk * a.v_h, seg.b * a.v_b);
+        ++sn;
+        int g = seg.it0 / a.q_blocks, qb = seg.it0 - g * a.q_blocks;
+        for (int it = seg.it0; it < seg.it1; ++it, ++e) {
+          const int i = e & 1, h = seg.hk * a.n.group + g;
+          if (!wait(&bars->g_empty[i], ((e >> 1) & 1) ^ 1) || !wait(&bars->q_empty[i], ((e >> 1) & 1) ^ 1)) {
+            ok = false;
+            break;
+          }
+          bars->info[e & 7] = (it == seg.it0 ? kFirst : 0) | (it == seg.it1 - 1 ? kLast : 0);
+          bar = smem_u32(&bars->q_full[i]);
+          mbar_expect_tx(bar, 2 * kTileBytes + 1024);
+          tma_tile(smem_u32(sQ + i * kTileBytes), &tm_q, bar, 128 * qb, h * a.q_h, seg.b * a.q_b);
+          tma_tile(smem_u32(sG + i * kTileBytes), &tm_g, bar, 128 * qb, h * a.g_h, seg.b * a.g_b);
+          const int64_t pad = (((int64_t)seg.b * a.n.heads + h) * a.q_blocks + qb) * 128;
+          bulk_512(smem_u32(bars->nl2[i]), a.nl2 + pad, bar);
+          bulk_512(smem_u32(bars->delta[i]), a.delta + pad, bar);
+          if (++qb == a.q_blocks) {
+            qb = 0;
+            ++g;
+          }
+        }
+      }
+      if (ok && wait(&bars->g_empty[e & 1], ((e >> 1) & 1) ^ 1) && wait(&bars->q_empty[e & 1], ((e >> 1) & 1) ^ 1)) {
+        bars->info[e & 7] = kEnd;
+        mbar_arrive(smem_u32(&bars->q_full[e & 1]));
+      } else {
+        volatile int32_t zero = 0;
+        for (int x = max(0, e - 2); x < e; ++x) mbar_wait(smem_u32(&bars->q_full[x & 1]), (x >> 1) & 1, &zero, nullptr);
+        if (sn) mbar_wait(smem_u32(&bars->kv_full), (sn - 1) & 1, &zero, nullptr);
+      }
+    } else if (warp == 1) {
+      auto iwait = [&](uint64_t* bar, uint32_t par) -> bool {
+        int got = 0;
+        if (lane == 0) got = wait(bar, par) ? 1 : 0;
+        return __shfl_sync(0xffffffff, got, 0) != 0;
+      };
+      int e = 0, pinfo = 0, segs = 0, accs = 0;
+      bool ok = true;
+      auto issue_dv = [&](int p, int info) -> bool {  // dv += P^T do
+        if (info & kFirst) {
+          if (accs > 0 && !iwait(&bars->acc_empty, (accs - 1) & 1)) return false;
+          ++accs;
+        }
+        if (!iwait(&bars->p_full, p & 1)) return false;
+        tc_fence_after();
+        mma_tile_ts(tmem + 128, tmem + 256, tmem + 320, smem_u32(sG + (p & 1) * kTileBytes), !(info & kFirst));
+        tc_commit_w(smem_u32(&bars->g_empty[p & 1]));
+        return true;
+      };
+      auto issue_dk = [&](int p, int info) -> bool {  // dk += dS^T q
+        if (!iwait(&bars->ds_full, p & 1)) return false;
+        tc_fence_after();
+        mma_tile_ts(tmem, tmem + 384, tmem + 448, smem_u32(sQ + (p & 1) * kTileBytes), !(info & kFirst));
+        tc_commit_w(smem_u32(&bars->q_empty[p & 1]));
+        if (info & kLast) tc_commit_w(smem_u32(&bars->acc_full));
+        return true;
+      };
+      while (true) {
+        const int i = e & 1;
+        ok = iwait(&bars->q_full[i], (e >> 1) & 1);
+        if (!ok) break;
+        const int info = ((volatile int32_t*)bars->info)[e & 7];
+        if (info & kEnd) break;
+        ok = e == 0 || issue_dv(e - 1, pinfo);
+        if (ok && (info & kFirst)) {
+          ok = iwait(&bars->kv_full, segs & 1);
+          ++segs;
+        }
+        if (!ok) break;
+        tc_fence_after();
+        mma_tile_ss(tmem + 256, smem_u32(sK), smem_u32(sQ + i * kTileBytes));
+        tc_commit_w(smem_u32(&bars->s_full));
+        ok = e == 0 || issue_dk(e - 1, pinfo);
+        if (!ok) break;
+        mma_tile_ss(tmem + 384, smem_u32(sV), smem_u32(sG + i * kTileBytes));
+        tc_commit_w(smem_u32(&bars->dp_full));
+        if (info & kLast) tc_commit_w(smem_u32(&bars->kv_empty));
+        pinfo = info;
+        ++e;
+      }
+      if (ok && e > 0) ok = issue_dv(e - 1, pinfo) && issue_dk(e - 1, pinfo);
+      tc_commit_w(smem_u32(&bars->done));
+    } else if (warp >= 2) {
+      // gradients of key tiles without a valid key: 0
+      const int64_t first = (int64_t)blockIdx.x * 2 + (warp - 2), step = (int64_t)gridDim.x * 2;
+      for (int b = 0; b < a.n.batch; ++b) {
+        const int t0 = (kv_len_of(a.kv_lens, a.n.kv_len, b) + 127) & ~127;
+        for (int64_t x = first; x < (int64_t)max(0, a.n.kv_len - t0) * a.n.kv_heads; x += step) {
+          const int64_t t = t0 + x / a.n.kv_heads, h = x % a.n.kv_heads;
+          uint16_t* row = lane < 16 ? a.dk.at(b, t, h) : a.dv.at(b, t, h);
+          reinterpret_cast<uint4*>(row)[lane & 15] = make_uint4(0, 0, 0, 0);
+        }
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    // one outcome a warp: the TMEM accesses need its lanes together
+    auto wait_w = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
+    const int w = (warp - 4) >> 2, q = warp & 3, r = 32 * q + lane;
+    const uint32_t lane_base = tmem + ((uint32_t)(32 * q) << 16);
+    const uint64_t sl2 = dup2(a.scale * kLog2e);
+    DkvWalk seg(a, blockIdx.x, gridDim.x);
+    int e = 0, sn = 0;
+    bool ok = true;
+    while (ok && seg.next(a)) {
+      for (int it = seg.it0; it < seg.it1; ++it, ++e) {
+        if (!wait_w(&bars->q_full[e & 1], (e >> 1) & 1) || !wait_w(&bars->s_full, e & 1)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        uint32_t s[64];
+        load64(lane_base + 256 + 64 * w, s);
+        const uint64_t* nl2 = reinterpret_cast<const uint64_t*>(bars->nl2[e & 1] + 64 * w);
+        float p[64];
+        uint32_t pk[32];
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          const uint64_t v = fma_2(pair2(s[2 * c], s[2 * c + 1]), sl2, nl2[c]);
+          p[2 * c] = ex2(lo2(v));
+          p[2 * c + 1] = ex2(hi2(v));
+          pk[c] = pack_bf16(p[2 * c], p[2 * c + 1]);
+        }
+        H3_TMEM_ST16(lane_base + 256 + 64 * w, (&pk[0]));
+        H3_TMEM_ST16(lane_base + 256 + 64 * w + 16, (&pk[16]));
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(smem_u32(&bars->p_full));
+        if (!wait_w(&bars->dp_full, e & 1)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        load64(lane_base + 384 + 64 * w, s);
+        const uint64_t* delta = reinterpret_cast<const uint64_t*>(bars->delta[e & 1] + 64 * w);
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          const uint64_t v = mul_2(add_2(pair2(s[2 * c], s[2 * c + 1]), delta[c] ^ 0x8000000080000000ull),
+                                   pair2(__float_as_uint(p[2 * c]), __float_as_uint(p[2 * c + 1])));
+          pk[c] = pack_bf16(lo2(v), hi2(v));
+        }
+        H3_TMEM_ST16(lane_base + 384 + 64 * w, (&pk[0]));
+        H3_TMEM_ST16(lane_base + 384 + 64 * w + 16, (&pk[16]));
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(smem_u32(&bars->ds_full));
+      }
+      if (!ok || !wait_w(&bars->acc_full, sn & 1)) break;
+      ++sn;
+      tc_fence_after();
+      // warpgroup 0 writes dk, 1 dv
+      const bool head = seg.it0 > 0, tail = seg.it1 < seg.steps;
+      const int key = seg.tile * 128 + r;
+      const bool valid = key < seg.len, live = key < a.n.kv_len;
+      const float f = w ? 1.0f : a.scale;
+      const Rows& out = w ? a.dv : a.dk;
+      uint16_t* go = live ? out.at(seg.b, key, seg.hk) : nullptr;
+      float4* po = reinterpret_cast<float4*>(a.part + (((int64_t)blockIdx.x * 2 + (head ? 0 : 1)) * 2 + w) * 16384);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        uint32_t v[16];
+        H3_TMEM_LD16(lane_base + 128 * w + 16 * c, v);
+        tmem_wait_ld();
+        if (head || tail) {
+          // column-major in groups of four, so that a warp's stores are contiguous
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            po[(4 * c + i) * 128 + r] = make_float4(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]),
+                                                    __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
+        } else if (live) {
+          uint32_t k[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            k[i] = valid ? pack_bf16(__uint_as_float(v[2 * i]) * f, __uint_as_float(v[2 * i + 1]) * f) : 0u;
+          reinterpret_cast<uint4*>(go + 16 * c)[0] = make_uint4(k[0], k[1], k[2], k[3]);
+          reinterpret_cast<uint4*>(go + 16 * c)[1] = make_uint4(k[4], k[5], k[6], k[7]);
+        }
+      }
+      tc_fence_before();
+      mbar_arrive(smem_u32(&bars->acc_empty));
+    }
+  }
+  release_tmem(warp, tmem, abort_flag, &bars->done);
+}
+
+// Adds the partial sums of the key tiles that were cut.  Block (x, y): the
+// tile that the start of CTA x + 1's run cuts (if it is the first such start
+// inside the tile), rows 16y..16y+15 of dk and dv.
+__global__ void __launch_bounds__(256) dkv_join_kernel(const __grid_constant__ BwdArgs a, int ctas) {
+  const int c = blockIdx.x + 1;
+  DkvWalk own(a, c, ctas);
+  const int64_t start = own.pos, share = DkvWalk(a, 1, ctas).pos;  // share: CTA 1 starts there
+  if (start >= own.end) return;
+  if (!own.next(a) || own.it0 == 0) return;
+  const int64_t first = start - own.it0, last = first + own.steps - 1;
+  const int c0 = (int)(first / share), c1 = (int)(last / share);
+  if (c0 != c - 1) return;  // an earlier start cuts the tile too
+  // 16 rows x 32 column groups x 2 results over 256 threads
+  const int r = blockIdx.y * 16 + (threadIdx.x & 15), key = own.tile * 128 + r;
+  if (key >= a.n.kv_len) return;
+  for (int k = threadIdx.x >> 4; k < 64; k += 16) {
+    const int which = k >> 5, cg = k & 31;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = c0; i <= c1; ++i) {
+      const float4 v = reinterpret_cast<const float4*>(
+          a.part + (((int64_t)i * 2 + (i == c0 ? 1 : 0)) * 2 + which) * 16384)[cg * 128 + r];
+      sum.x += v.x;
+      sum.y += v.y;
+      sum.z += v.z;
+      sum.w += v.w;
+    }
+    const float f = which ? 1.0f : a.scale;
+    uint2 o = make_uint2(pack_bf16(sum.x * f, sum.y * f), pack_bf16(sum.z * f, sum.w * f));
+    if (key >= own.len) o = make_uint2(0, 0);
+    *reinterpret_cast<uint2*>((which ? a.dv : a.dk).at(own.b, key, own.hk) + 4 * cg) = o;
   }
 }
 
-unsigned warps_grid(int64_t rows) { return (unsigned)((rows + 7) / 8 < 148 * 8 ? (rows + 7) / 8 : 148 * 8); }
+__global__ void __launch_bounds__(256) zero_kv_kernel(CrossShape n, Rows dk, Rows dv) {
+  const int64_t rows = (int64_t)n.batch * n.kv_len * n.kv_heads;
+  const int lane = threadIdx.x & 31;
+  for (int64_t x = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5; x < rows;
+       x += ((int64_t)gridDim.x * blockDim.x) >> 5) {
+    const int64_t h = x % n.kv_heads, bt = x / n.kv_heads;
+    uint16_t* row = (lane < 16 ? dk : dv).at(bt / n.kv_len, bt % n.kv_len, h);
+    reinterpret_cast<uint4*>(row)[lane & 15] = make_uint4(0, 0, 0, 0);
+  }
+}
+
+unsigned warps_grid(int64_t rows) { return (unsigned)((rows + 7) / 8 < kSms * 8 ? (rows + 7) / 8 : kSms * 8); }
+
+int dkv_ctas(const CrossShape& n) {
+  const int64_t steps = (int64_t)n.group * ((n.q_len + 127) / 128);
+  const int64_t all = (int64_t)n.batch * n.kv_heads * ((n.kv_len + 127) / 128) * steps;
+  return (int)(all < kSms ? all : kSms);
+}
+
+// Attributes of a kernel, set once a device; the register split needs exactly
+// 168 registers a thread at launch.
+template <typename K>
+cudaError_t prepare(K* kernel, int smem, std::once_flag* once, cudaError_t* result) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  std::call_once(once[dev], [&] {
+    cudaError_t r = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaFuncAttributes fa;
+    if (r == cudaSuccess) r = cudaFuncGetAttributes(&fa, kernel);
+    if (r == cudaSuccess && fa.numRegs != 168) r = cudaErrorInvalidConfiguration;
+    result[dev] = r;
+  });
+  return result[dev];
+}
 
 }  // namespace
 
-size_t cross_bwd_workspace(const CrossShape& n) { return (size_t)n.batch * n.heads * n.q_len * sizeof(float); }
+size_t cross_bwd_workspace(const CrossShape& n) {
+  if (!n.batch || !n.q_len || !n.kv_len) return 0;
+  const size_t rows = (size_t)n.batch * n.heads * ((n.q_len + 127) / 128) * 128;
+  return 2 * rows * sizeof(float) + (size_t)dkv_ctas(n) * 4 * 16384 * sizeof(float);
+}
 
-cudaError_t launch_cross_bwd(const CrossLaunch& a, cudaStream_t s, std::string*) {
-  const int64_t rows = (int64_t)a.n.batch * a.n.heads * a.n.q_len;
-  const int64_t keys = (int64_t)a.n.batch * a.n.kv_heads * a.n.kv_len;
-  if (rows) cross_dq_kernel<<<warps_grid(rows), 256, 0, s>>>(a, (float*)a.ws);
-  if (keys) cross_dkv_kernel<<<warps_grid(keys), 256, 0, s>>>(a, (const float*)a.ws);
+cudaError_t launch_cross_bwd(const CrossLaunch& L, cudaStream_t s, std::string* err) {
+  const CrossShape& n = L.n;
+  if (n.q_len == 0) {
+    const int64_t rows = (int64_t)n.batch * n.kv_len * n.kv_heads;
+    if (rows) zero_kv_kernel<<<warps_grid(rows), 256, 0, s>>>(n, L.dk, L.dv);
+    return cudaGetLastError();
+  }
+  BwdArgs a{};
+  a.n = n;
+  a.out = L.out, a.dout = L.dout, a.dq = L.dq, a.dk = L.dk, a.dv = L.dv;
+  a.kv_lens = L.kv_lens;
+  a.lse = L.lse;
+  a.scale = L.scale;
+  a.q_blocks = (n.q_len + 127) / 128;
+  const int64_t rows = (int64_t)n.batch * n.heads * a.q_blocks * 128;
+  a.nl2 = (float*)L.ws;
+  a.delta = a.nl2 + rows;
+  a.part = a.delta + rows;
+  a.status = L.status;
+  a.wait_limit_ns = L.wait_limit_ns;
+  a.q_b = L.q.b != 0, a.q_h = L.q.h != 0;
+  a.k_b = L.k.b != 0, a.k_h = L.k.h != 0;
+  a.v_b = L.v.b != 0, a.v_h = L.v.h != 0;
+  a.g_b = L.dout.b != 0, a.g_h = L.dout.h != 0;
+  CUtensorMap mq, mk{}, mv{}, mg;
+  if (!make_map4(&mq, L.q, n.q_len, n.heads, n.batch, err) || !make_map4(&mg, L.dout, n.q_len, n.heads, n.batch, err))
+    return cudaErrorInvalidValue;
+  if (n.kv_len && (!make_map4(&mk, L.k, n.kv_len, n.kv_heads, n.batch, err) ||
+                   !make_map4(&mv, L.v, n.kv_len, n.kv_heads, n.batch, err)))
+    return cudaErrorInvalidValue;
+  static std::once_flag once_q[64], once_kv[64];
+  static cudaError_t res_q[64], res_kv[64];
+  cudaError_t e = prepare(dq_kernel, kDqSmem, once_q, res_q);
+  if (e == cudaSuccess) e = prepare(dkv_kernel, kDkvSmem, once_kv, res_kv);
+  if (e != cudaSuccess) return e;
+  const int units = n.batch * n.heads * a.q_blocks;
+  dq_kernel<<<units < kSms ? units : kSms, kThreads, kDqSmem, s>>>(mq, mk, mv, mg, a, units);
+  const int ctas = n.kv_len ? dkv_ctas(n) : 0;
+  if (ctas) dkv_kernel<<<ctas, kThreads, kDkvSmem, s>>>(mq, mk, mv, mg, a);
+  if (ctas > 1) dkv_join_kernel<<<dim3(ctas - 1, 8), 256, 0, s>>>(a, ctas);
   return cudaGetLastError();
 }
 

@@ -36,7 +36,6 @@
 #include <type_traits>
 
 #include "conditioning.cuh"
-#include "tcgen05.cuh"
 
 namespace h3 {
 namespace {
@@ -498,6 +497,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    // one outcome a warp: the TMEM accesses need its lanes together
+    auto wait_w = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
     // ----------------------------------------------------- softmax + epilogue
     const int t = (warp - 4) >> 2, q = warp & 3;
     const int r = 32 * q + lane;  // row of the tile = TMEM lane
@@ -518,7 +519,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       float m = -1e30f, l = 0.f;
       for (int x = 0; x < nt; ++x) {
         const int valid = SegIter::valid(a, s, s.j0 + i0 + x * step);
-        if (!wait(&bars->s_full[t], ns & 1)) {
+        if (!wait_w(&bars->s_full[t], ns & 1)) {
           ok = false;
           break;
         }
@@ -598,7 +599,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (t == 1) {
           if (nt > 0) {
             // half 0 has read the last segment's
-            if (nml > 0 && !wait(&bars->o_empty[1], (nml - 1) & 1)) break;
+            if (nml > 0 && !wait_w(&bars->o_empty[1], (nml - 1) & 1)) break;
             bars->ml[r] = make_float2(m, l);
             ++nml;
             mbar_arrive(smem_u32(&bars->ml_full));
@@ -607,7 +608,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         has1 = s.n - nt > 0;
         if (has1) {
-          if (!wait(&bars->ml_full, nml & 1)) break;
+          if (!wait_w(&bars->ml_full, nml & 1)) break;
           const float2 ml = bars->ml[r];
           ++nml;
           const float top = fmaxf(m, ml.x);
@@ -615,12 +616,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           w1 = ex2(ml.x - top);
           m = top;
           l = l * w0 + ml.y * w1;
-          if (!wait(&bars->o_full[1], no1 & 1)) break;
+          if (!wait_w(&bars->o_full[1], no1 & 1)) break;
           ++no1;
         }
       }
       if (has0) {
-        if (!wait(&bars->o_full[t], no & 1)) break;
+        if (!wait_w(&bars->o_full[t], no & 1)) break;
         ++no;
       }
       tc_fence_after();
@@ -794,29 +795,6 @@ FwdPlan plan_fwd(const CrossShape& n) {
   p.part_rows = p.combine ? (p.mode == kDense ? (int64_t)n.batch * n.heads * n.q_len : (int64_t)n.kv_heads * p.fold_rows)
                           : 0;
   return p;
-}
-
-// (d, token, head, batch) map of an operand, boxes of 64 x 128; a broadcast
-// axis has one element.
-bool make_map4(CUtensorMap* m, const Rows& r, int tokens, int heads, int batch, std::string* err) {
-  EncodeTiledFn enc = get_encode();
-  if (!enc) {
-    *err += "cuTensorMapEncodeTiled unavailable; ";
-    return false;
-  }
-  cuuint64_t dims[4] = {128, (cuuint64_t)tokens, r.h ? (cuuint64_t)heads : 1, r.b ? (cuuint64_t)batch : 1};
-  cuuint64_t strides[3] = {r.t ? (cuuint64_t)r.t * 2 : 256, r.h ? (cuuint64_t)r.h * 2 : 256,
-                           r.b ? (cuuint64_t)r.b * 2 : 256};
-  cuuint32_t box[4] = {64, 128, 1, 1};
-  cuuint32_t estr[4] = {1, 1, 1, 1};
-  CUresult res = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, r.p, dims, strides, box, estr,
-                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (res != CUDA_SUCCESS) {
-    *err += "cuTensorMapEncodeTiled failed (" + std::to_string((int)res) + "); ";
-    return false;
-  }
-  return true;
 }
 
 template <bool SINGLE>

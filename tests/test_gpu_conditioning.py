@@ -162,6 +162,9 @@ CROSS = [
     (1, 255, 383, 2, 2, None), (2, 256, 33, 3, 1, [33, 0]), (3, 257, 77, 8, 2, [77, 58, 0]), (1, 300, 600, 2, 1, [513]),
     (1, 1000, 332, 4, 4, None), (2, 515, 1024, 6, 2, [1024, 385]), (1, 64, 3001, 8, 2, None), (1, 16, 5000, 3, 3, [4999]),
     (70, 3, 20, 1, 1, [i % 21 for i in range(70)]), (1, 700, 2048, 1, 1, None),
+    # several units and cut key tiles a CTA
+    (2, 2500, 400, 10, 5, [400, 200]), (1, 4000, 332, 14, 14, None), (300, 2, 70, 4, 4, [i % 71 for i in range(300)]),
+    (40, 40, 300, 8, 2, [300 - 7 * i for i in range(40)]),
 ]
 
 
