@@ -216,6 +216,24 @@ def load() -> C.CDLL:
         return L
 
 
+_packed = None
+
+
+def load_packed() -> C.CDLL:
+    """The conditioning calls with their argument structure as packed bytes."""
+    global _packed
+    load()
+    with _lock:
+        if _packed is None:
+            L = C.CDLL(LIB_PATH)
+            for name in ("h3c_cross_attn_fwd", "h3c_cross_attn_bwd", "h3c_prefix_attn_fwd", "h3c_qk_norm_rope_fwd",
+                         "h3c_qk_norm_rope_bwd"):
+                fn = getattr(L, name)
+                fn.argtypes, fn.restype = [C.c_void_p, C.c_char_p, C.c_void_p], C.c_int
+            _packed = L
+        return _packed
+
+
 def check(status: int, ctx=None, what: str = "") -> None:
     if status != H3C_OK:
         msg = load().h3c_last_error(ctx).decode() if ctx is not None else what

@@ -6,6 +6,8 @@ shapes and strides cross the boundary.
 from __future__ import annotations
 
 import ctypes as C
+import functools
+import struct
 import threading
 from typing import Dict, Optional
 
@@ -32,43 +34,78 @@ def view_of(t, layout: str) -> _lib.View:
     return _lib.View(t.data_ptr(), tok, head)
 
 
-def _bview(name, t, layout: str, device: int, shape=None):
-    """``(h3c_bview, (batch, tokens, heads))`` of a bf16 tensor on ``device``:
-    [B, S, H, 128] or [S, H, 128] ("SHD"), [B, H, S, 128] or [H, S, 128]
-    ("HSD").  ``shape``: the (batch, tokens, heads) it must have."""
+# h3c_cross_args and h3c_qk_norm_args, packed in one call: a small operator's
+# time is mostly that of its Python call, and filling the ctypes structures
+# field by field took 12 of its 20 us.
+_CROSS = struct.Struct("@" + "Pqqq" * 4 + "6if" + "PP" + "Pqq" * 2 + "ii" + "Pqqq" * 4 + "PN")
+_NORM = struct.Struct("@" + "Pqqq" * 4 + "6i" + "4P" + "qq" + "iifi" + "Pqqq" * 4 + "PPPN")
+_NO_ROWS = (0, 0, 0, 0)
+
+
+def _rows(name, t, hsd: bool, device: int, want=None):
+    """``((pointer, batch, token and head stride), (batch, tokens, heads))``
+    of a bf16 tensor on ``device``: [B, S, H, 128] or [S, H, 128], with
+    ``hsd`` [B, H, S, 128] or [H, S, 128].  ``want``: the (batch, tokens,
+    heads) it must have."""
     import torch
 
-    if t.dtype is not torch.bfloat16 or t.device.type != "cuda" or t.device.index != device:
+    if t.dtype is not torch.bfloat16 or t.get_device() != device:
         raise ValueError(f"{name} must be bfloat16 on cuda:{device}, got {t.dtype} on {t.device}")
     size, stride = t.shape, t.stride()
-    if len(size) == 3:
-        size, stride = (1, *size), (0, *stride)
-    if len(size) != 4:
-        raise ValueError(f"{name} must have 3 or 4 axes, got {tuple(t.shape)}")
-    if layout == "SHD":
-        b, s, h, d = size
-        view = _lib.BView(t.data_ptr(), stride[0], stride[1], stride[2])
-    elif layout == "HSD":
-        b, h, s, d = size
-        view = _lib.BView(t.data_ptr(), stride[0], stride[2], stride[1])
+    if len(size) == 4:
+        (b, s, h, d), (sb, ss, sh, sd) = size, stride
+    elif len(size) == 3:
+        (s, h, d), (ss, sh, sd), b, sb = size, stride, 1, 0
     else:
-        raise ValueError(layout)
-    if stride[3] != 1 and d > 1:
+        raise ValueError(f"{name} must have 3 or 4 axes, got {tuple(size)}")
+    if hsd:
+        s, h, ss, sh = h, s, sh, ss
+    if sd != 1 and d > 1:
         raise ValueError(f"{name}: head_dim must be contiguous")
     if d != 128:
         raise _lib.H3CError(_lib.H3C_ERR_UNSUPPORTED, f"{name}: head_dim must be 128, got {d}")
-    if shape is not None and (b, s, h) != shape:
-        raise ValueError(f"{name} must have {shape} (batch, tokens, heads), got {(b, s, h)}")
-    return view, (b, s, h)
+    if want is not None and (b, s, h) != want:
+        raise ValueError(f"{name} must have {want} (batch, tokens, heads), got {(b, s, h)}")
+    return (t.data_ptr(), sb, ss, sh), (b, s, h)
 
 
 def _vector(name, t, dtype, shape, device: int) -> int:
     """Device pointer of a contiguous tensor of the given type and shape."""
-    if t.dtype is not dtype or t.device.type != "cuda" or t.device.index != device or tuple(t.shape) != shape \
-            or not t.is_contiguous():
+    if t.dtype is not dtype or t.get_device() != device or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape} on cuda:{device}, got "
                          f"{t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
+
+
+def _hsd(layout: str) -> bool:
+    if layout != "SHD" and layout != "HSD":
+        raise ValueError(layout)
+    return layout == "HSD"
+
+
+@functools.lru_cache(maxsize=4096)
+def _cross_workspace(op, batch, q_len, kv_len, prefix_len, heads, kv_heads) -> int:
+    """Bytes of workspace of a call of these sizes.  It depends on nothing
+    else, so the operands are stood in for by aligned pointers; a call whose
+    sizes are refused is refused by itself."""
+    a, n = _lib.CrossArgs(), C.c_size_t(0)
+    a.batch, a.q_len, a.kv_len, a.heads, a.kv_heads, a.head_dim = batch, q_len, kv_len, heads, kv_heads, 128
+    a.scale, a.lse, a.prefix_len = 1.0, 256, prefix_len
+    for names, s, h in ((("q", "out", "out_grad", "dq"), q_len, heads), (("k", "v", "dk", "dv"), kv_len, kv_heads)):
+        for name in names:
+            setattr(a, name, _lib.BView(256, s * h * 128, h * 128, 128))
+    a.prefix_k = a.prefix_v = _lib.View(256, kv_heads * 128, 128)
+    _lib.load().h3c_cross_workspace_size(C.byref(a), op, C.byref(n), None, 0)
+    return n.value
+
+
+@functools.lru_cache(maxsize=None)
+def _norm_workspace() -> int:
+    a, n = _lib.QkNormArgs(), C.c_size_t(0)
+    a.heads = a.kv_heads = 1
+    a.head_dim, a.q_norm_weight, a.k_norm_weight, a.q_norm_grad, a.k_norm_grad = 128, 256, 256, 256, 256
+    _lib.check(_lib.load().h3c_qk_norm_workspace_size(C.byref(a), 1, C.byref(n), None, 0), what="workspace size")
+    return n.value
 
 
 class Runtime:
@@ -77,6 +114,7 @@ class Runtime:
 
     def __init__(self, device: int):
         self.L = _lib.load()
+        self._packed = _lib.load_packed()
         self.device = device
         h = C.c_void_p()
         _lib.check(self.L.h3c_init(device, C.byref(h)), what=f"h3c_init(device={device})")
@@ -189,43 +227,60 @@ class Runtime:
         self._check(self.L.h3c_attn_fwd(self.ctx, C.byref(a), _stream_ptr(stream)))
 
     # --------------------------------------------------------- conditioning
-    def _launch(self, call, args, size_call, selector, stream):
-        """Run ``call`` with workspace of the size ``size_call`` gives, taken
-        from torch's allocator on the launching stream (so a captured call
-        keeps its own, and the memory is not reused before the call is done)."""
+    def _workspace(self, size: int, stream):
+        """Scratch from torch's allocator on the launching stream (None: the
+        current one), so a captured call keeps its own and the memory is not
+        reused before the call is done."""
         import torch
 
-        need, why = C.c_size_t(0), C.create_string_buffer(256)
-        st = size_call(C.byref(args), selector, C.byref(need), why, 256)
-        if st != _lib.H3C_OK:
-            raise _lib.H3CError(st, why.value.decode())
         if stream is None:
-            stream = torch.cuda.current_stream(self.device)
-        ws = None
-        if need.value:
-            with torch.cuda.stream(stream):
-                ws = torch.empty(need.value, dtype=torch.uint8, device=f"cuda:{self.device}")
-            args.workspace, args.workspace_bytes = ws.data_ptr(), need.value
-        self._check(call(self.ctx, C.byref(args), stream.cuda_stream or None))
+            return torch.empty(size, dtype=torch.uint8, device=self._torch_device())
+        with torch.cuda.stream(stream):
+            return torch.empty(size, dtype=torch.uint8, device=self._torch_device())
 
-    def _cross_args(self, q, k, v, out, layout, scale, kv_lens, lse):
+    def _torch_device(self):
         import torch
 
-        a, dev = _lib.CrossArgs(), self.device
-        a.q, (B, S, H) = _bview("q", q, layout, dev)
-        a.out, _ = _bview("out", out, layout, dev, (B, S, H))
-        a.k, (kb, n, Hk) = _bview("k", k, layout, dev)
-        if kb != B:
-            raise ValueError(f"k must have the {B} members of q, got {kb}")
-        a.v, _ = _bview("v", v, layout, dev, (B, n, Hk))
-        a.batch, a.q_len, a.kv_len, a.heads, a.kv_heads, a.head_dim = B, S, n, H, Hk, 128
-        a.scale = scale
-        if kv_lens is not None:
-            a.kv_lens = _vector("kv_lens", kv_lens, torch.int32, (B,), dev)
-        if lse is not None:
-            shape = (B, H, S) if q.dim() == 4 or lse.dim() == 3 else (H, S)
-            a.lse = _vector("lse", lse, torch.float32, shape, dev)
-        return a
+        return torch.device("cuda", self.device)
+
+    def _raw_stream(self, stream):
+        import torch
+
+        return (torch.cuda.current_stream(self.device) if stream is None else stream).cuda_stream or None
+
+    def _cross(self, op, call, q, k, v, out, layout, scale, kv_lens, lse, stream, prefix=None, grads=None):
+        import torch
+
+        hsd, dev = _hsd(layout), self.device
+        vq, mine = _rows("q", q, hsd, dev)
+        vo, _ = _rows("out", out, hsd, dev, mine)
+        B, S, H = mine
+        vk, keys = _rows("k", k, hsd, dev)
+        vv, _ = _rows("v", v, hsd, dev, keys)
+        if keys[0] != B:
+            raise ValueError(f"k must have the {B} members of q, got {keys[0]}")
+        Hk = keys[2]
+        P, vp = 0, (0, 0, 0, 0, 0, 0)
+        if prefix is not None:
+            if prefix[0].dim() != 3 or prefix[1].dim() != 3:
+                raise ValueError("prefix_k and prefix_v have no batch axis")
+            (pk, _, pks, pkh), (_, P, ph) = _rows("prefix_k", prefix[0], hsd, dev)
+            (pv, _, pvs, pvh), _ = _rows("prefix_v", prefix[1], hsd, dev, (1, P, ph))
+            if ph != Hk:
+                raise ValueError(f"prefix_k must have the {Hk} heads of k, got {ph}")
+            vp = (pk, pks, pkh, pv, pvs, pvh)
+        vg = (_NO_ROWS,) * 4
+        if grads is not None:
+            vg = (_rows("out_grad", grads[0], hsd, dev, mine)[0], _rows("dq", grads[1], hsd, dev, mine)[0],
+                  _rows("dk", grads[2], hsd, dev, keys)[0], _rows("dv", grads[3], hsd, dev, keys)[0])
+        lens = 0 if kv_lens is None else _vector("kv_lens", kv_lens, torch.int32, (B,), dev)
+        plse = 0 if lse is None else _vector("lse", lse, torch.float32, (B, H, S) if lse.dim() == 3 or B > 1 else (H, S),
+                                             dev)
+        size = _cross_workspace(op, B, S, keys[1], P, H, Hk)
+        ws = self._workspace(size, stream) if size else None
+        args = _CROSS.pack(*vq, *vo, *vk, *vv, B, S, keys[1], H, Hk, 128, scale, lens, plse, *vp, P, 0, *vg[0], *vg[1],
+                           *vg[2], *vg[3], ws.data_ptr() if size else 0, size)
+        self._check(call(self.ctx, args, self._raw_stream(stream)))
 
     def cross_attn_fwd(self, *, q, k, v, out, scale, layout="SHD", kv_lens=None, lse=None, stream=None):
         """``out = softmax(scale q k^T) v`` against encoder states of another
@@ -234,66 +289,70 @@ class Runtime:
         device tensor, the valid keys of each member; a member without keys
         gives zeros.  lse: optional fp32 [B, H, S] result, needed by
         ``cross_attn_bwd``."""
-        a = self._cross_args(q, k, v, out, layout, scale, kv_lens, lse)
-        self._launch(self.L.h3c_cross_attn_fwd, a, self.L.h3c_cross_workspace_size, _lib.H3C_OP_CROSS_FWD, stream)
+        self._cross(_lib.H3C_OP_CROSS_FWD, self._packed.h3c_cross_attn_fwd, q, k, v, out, layout, scale, kv_lens, lse,
+                    stream)
 
     def cross_attn_bwd(self, *, q, k, v, out, lse, out_grad, dq, dk, dv, scale, layout="SHD", kv_lens=None,
                        stream=None):
         """Gradients of ``cross_attn_fwd``: dq as q, dk and dv as k (summed
         over the query heads of each key head, 0 past kv_lens), from the
         forward call's out and lse.  Deterministic."""
-        a, dev = self._cross_args(q, k, v, out, layout, scale, kv_lens, lse), self.device
-        mine, keys = (a.batch, a.q_len, a.heads), (a.batch, a.kv_len, a.kv_heads)
-        a.out_grad, _ = _bview("out_grad", out_grad, layout, dev, mine)
-        a.dq, _ = _bview("dq", dq, layout, dev, mine)
-        a.dk, _ = _bview("dk", dk, layout, dev, keys)
-        a.dv, _ = _bview("dv", dv, layout, dev, keys)
-        self._launch(self.L.h3c_cross_attn_bwd, a, self.L.h3c_cross_workspace_size, _lib.H3C_OP_CROSS_BWD, stream)
+        self._cross(_lib.H3C_OP_CROSS_BWD, self._packed.h3c_cross_attn_bwd, q, k, v, out, layout, scale, kv_lens, lse,
+                    stream, grads=(out_grad, dq, dk, dv))
 
     def prefix_attn_fwd(self, *, q, prefix_k, prefix_v, k, v, out, scale, layout="SHD", kv_lens=None, lse=None,
                         stream=None):
         """Attention of every member's queries over the keys all members
         share (prefix_k, prefix_v: [P, Hk, 128], "HSD": [Hk, P, 128]) and
         then its own, as ``cross_attn_fwd``."""
-        a, dev = self._cross_args(q, k, v, out, layout, scale, kv_lens, lse), self.device
-        if prefix_k.dim() != 3 or prefix_v.dim() != 3:
-            raise ValueError("prefix_k and prefix_v have no batch axis")
-        pk, (_, P, _) = _bview("prefix_k", prefix_k, layout, dev)
-        _bview("prefix_k", prefix_k, layout, dev, (1, P, a.kv_heads))
-        pv, _ = _bview("prefix_v", prefix_v, layout, dev, (1, P, a.kv_heads))
-        a.prefix_k = _lib.View(pk.ptr, pk.token_stride, pk.head_stride)
-        a.prefix_v = _lib.View(pv.ptr, pv.token_stride, pv.head_stride)
-        a.prefix_len = P
-        self._launch(self.L.h3c_prefix_attn_fwd, a, self.L.h3c_cross_workspace_size, _lib.H3C_OP_PREFIX_FWD, stream)
+        self._cross(_lib.H3C_OP_PREFIX_FWD, self._packed.h3c_prefix_attn_fwd, q, k, v, out, layout, scale, kv_lens,
+                    lse, stream, prefix=(prefix_k, prefix_v))
 
     def _rope_rows(self, name, table, batch, tokens):
         """(pointer, half, batch stride) of a bf16 [S, half, 4] or [B, S, half, 4] table."""
         import torch
 
         if table is None:
-            return None, 0, 0
-        shape = (tokens,) if table.dim() == 3 else (batch, tokens)
-        if table.dtype is not torch.bfloat16 or table.device.type != "cuda" or table.device.index != self.device \
-                or table.dim() not in (3, 4) or table.shape[-1] != 4 or tuple(table.shape[:-2]) != shape \
-                or not table.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous bfloat16 {(*shape, 'half', 4)} tensor on cuda:{self.device}, "
-                             f"got {table.dtype} {tuple(table.shape)} on {table.device}")
-        return table.data_ptr(), table.shape[-2], tokens * table.shape[-2] * 4 if table.dim() == 4 else 0
+            return 0, 0, 0
+        shape = table.shape
+        each = len(shape) == 4
+        if table.dtype is not torch.bfloat16 or table.get_device() != self.device or not 3 <= len(shape) <= 4 \
+                or shape[-1] != 4 or shape[:-2] != ((batch, tokens) if each else (tokens,)) or not table.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous bfloat16 [{tokens}, half, 4] or [{batch}, {tokens}, half, 4] "
+                             f"tensor on cuda:{self.device}, got {table.dtype} {tuple(shape)} on {table.device}")
+        return table.data_ptr(), shape[-2], tokens * shape[-2] * 4 if each else 0
 
-    def _norm_args(self, q, k, q_norm, k_norm, eps, q_rope, k_rope, layout):
+    def _norm(self, call, q, k, outs, q_norm, k_norm, eps, q_rope, k_rope, layout, stream, grads=None):
         import torch
 
-        a, dev = _lib.QkNormArgs(), self.device
-        a.q, (B, S, H) = _bview("q", q, layout, dev)
-        a.k, (kb, n, Hk) = _bview("k", k, layout, dev)
-        if kb != B:
-            raise ValueError(f"k must have the {B} members of q, got {kb}")
-        a.batch, a.q_len, a.k_len, a.heads, a.kv_heads, a.head_dim, a.eps = B, S, n, H, Hk, 128, eps
-        a.q_norm_weight = _vector("q_norm", q_norm, torch.bfloat16, (128,), dev)
-        a.k_norm_weight = _vector("k_norm", k_norm, torch.bfloat16, (128,), dev)
-        a.q_rope, a.q_rope_half, a.q_rope_batch_stride = self._rope_rows("q_rope", q_rope, B, S)
-        a.k_rope, a.k_rope_half, a.k_rope_batch_stride = self._rope_rows("k_rope", k_rope, B, n)
-        return a
+        hsd, dev = _hsd(layout), self.device
+        vq, mine = _rows("q", q, hsd, dev)
+        vk, keys = _rows("k", k, hsd, dev)
+        B, S, H = mine
+        if keys[0] != B:
+            raise ValueError(f"k must have the {B} members of q, got {keys[0]}")
+        wq = _vector("q_norm", q_norm, torch.bfloat16, (128,), dev)
+        wk = _vector("k_norm", k_norm, torch.bfloat16, (128,), dev)
+        tq, hq, bq = self._rope_rows("q_rope", q_rope, B, S)
+        tk, hk, bk = self._rope_rows("k_rope", k_rope, B, keys[1])
+        size, ws, back, dw = 0, None, (_NO_ROWS,) * 4, (0, 0)
+        if grads is None:
+            names, given = ("q_out", "k_out"), outs
+        else:
+            names, given = ("dq", "dk"), grads[2:4]
+            size = _norm_workspace()
+            ws = self._workspace(size, stream)
+            dw = (_vector("dq_norm", grads[4], torch.float32, (128,), dev),
+                  _vector("dk_norm", grads[5], torch.float32, (128,), dev))
+        yq, _ = _rows(names[0], given[0], hsd, dev, mine)
+        yk, _ = _rows(names[1], given[1], hsd, dev, keys)
+        fwd = (yq, yk)
+        if grads is not None:
+            back = (_rows("q_grad", grads[0], hsd, dev, mine)[0], yq, _rows("k_grad", grads[1], hsd, dev, keys)[0], yk)
+            fwd = (_NO_ROWS, _NO_ROWS)
+        args = _NORM.pack(*vq, *fwd[0], *vk, *fwd[1], B, S, keys[1], H, keys[2], 128, wq, wk, tq, tk, bq, bk, hq, hk, eps,
+                          0, *back[0], *back[1], *back[2], *back[3], *dw, ws.data_ptr() if size else 0, size)
+        self._check(call(self.ctx, args, self._raw_stream(stream)))
 
     def qk_norm_rope_fwd(self, *, q, k, q_out, k_out, q_norm, k_norm, eps=1e-6, q_rope=None, k_rope=None,
                          layout="SHD", stream=None):
@@ -301,31 +360,16 @@ class Runtime:
         pass, fp32 with one rounding.  q: [B, S, H, 128], k: [B, N, Hk, 128];
         q_out / k_out may be q / k.  Tables: bf16 [S, half, 4] (as
         ``rope_table`` makes them) or [B, S, half, 4]; None: norm only."""
-        a, dev = self._norm_args(q, k, q_norm, k_norm, eps, q_rope, k_rope, layout), self.device
-        a.q_out, _ = _bview("q_out", q_out, layout, dev, (a.batch, a.q_len, a.heads))
-        a.k_out, _ = _bview("k_out", k_out, layout, dev, (a.batch, a.k_len, a.kv_heads))
-        if stream is None:
-            import torch
-
-            stream = torch.cuda.current_stream(dev)
-        self._check(self.L.h3c_qk_norm_rope_fwd(self.ctx, C.byref(a), stream.cuda_stream or None))
+        self._norm(self._packed.h3c_qk_norm_rope_fwd, q, k, (q_out, k_out), q_norm, k_norm, eps, q_rope, k_rope,
+                   layout, stream)
 
     def qk_norm_rope_bwd(self, *, q, k, q_grad, k_grad, q_norm, k_norm, dq, dk, dq_norm, dk_norm, eps=1e-6,
                          q_rope=None, k_rope=None, layout="SHD", stream=None):
         """Gradients of ``qk_norm_rope_fwd`` from those of its outputs
         (q_grad, k_grad): dq, dk (may be q_grad, k_grad) and the fp32 [128]
         gradients of the two weights.  Deterministic."""
-        import torch
-
-        a, dev = self._norm_args(q, k, q_norm, k_norm, eps, q_rope, k_rope, layout), self.device
-        mine, keys = (a.batch, a.q_len, a.heads), (a.batch, a.k_len, a.kv_heads)
-        a.q_grad, _ = _bview("q_grad", q_grad, layout, dev, mine)
-        a.k_grad, _ = _bview("k_grad", k_grad, layout, dev, keys)
-        a.dq, _ = _bview("dq", dq, layout, dev, mine)
-        a.dk, _ = _bview("dk", dk, layout, dev, keys)
-        a.q_norm_grad = _vector("dq_norm", dq_norm, torch.float32, (128,), dev)
-        a.k_norm_grad = _vector("dk_norm", dk_norm, torch.float32, (128,), dev)
-        self._launch(self.L.h3c_qk_norm_rope_bwd, a, self.L.h3c_qk_norm_workspace_size, 1, stream)
+        self._norm(self._packed.h3c_qk_norm_rope_bwd, q, k, None, q_norm, k_norm, eps, q_rope, k_rope, layout, stream,
+                   grads=(q_grad, k_grad, dq, dk, dq_norm, dk_norm))
 
     # ------------------------------------------------------------- prologue
     def prologue(self, x, out, weight, eps, rope_table=None, layout="SHD", stream=None):

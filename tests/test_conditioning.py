@@ -186,13 +186,46 @@ def test_struct_sizes_match_the_header(lib, tmp_path):
     assert got == want
 
 
+def test_packed_arguments_match_the_structures(lib):
+    """The Python calls pack their arguments; every field lands where ctypes has it."""
+    from h3attention.runtime import _CROSS, _NORM
+
+    for packer, cls in ((_CROSS, lib.CrossArgs), (_NORM, lib.QkNormArgs)):
+        assert packer.size == C.sizeof(cls)
+        flat = []
+
+        def collect(o):
+            for name, t in o._fields_:
+                v = getattr(o, name)
+                if isinstance(v, C.Structure):
+                    collect(v)
+                else:
+                    flat.append(t)
+
+        collect(cls())
+        values = [float(i) if t is C.c_float else i for i, t in enumerate(flat, 1)]
+        a, got = cls.from_buffer_copy(packer.pack(*values)), []
+
+        def read(o):
+            for name, _ in o._fields_:
+                v = getattr(o, name)
+                read(v) if isinstance(v, C.Structure) else got.append(v)
+
+        read(a)
+        assert got == values
+
+
 def test_python_refuses_host_tensors_and_types(lib):
     """The tensor checks of the Python calls run before the library is entered."""
     import torch
 
-    from h3attention.runtime import _bview, _vector
+    from h3attention.runtime import _cross_workspace, _norm_workspace, _rows, _vector
 
     with pytest.raises(ValueError, match="must be bfloat16 on cuda:0"):
-        _bview("q", torch.zeros(2, 3, 128, dtype=torch.bfloat16), "SHD", 0)
+        _rows("q", torch.zeros(2, 3, 128, dtype=torch.bfloat16), False, 0)
     with pytest.raises(ValueError, match="must be a contiguous"):
         _vector("kv_lens", torch.zeros(2, dtype=torch.int64), torch.int32, (2,), 0)
+    a = _cross(lib)
+    for op in (0, 1, 2):
+        assert _cross_workspace(op, 2, 5, 7, 3, 4, 2) == _ask(lib, a, op)[1]
+    assert _norm_workspace() == _ask(lib, _norm(lib), 1)[1] > 0

@@ -613,13 +613,11 @@ def test_workspace_is_checked(gpu):
     rt = _rt()
     q, k, v, do = _inputs(1, 300, 300, 2, 1, 52)
     out, lse = torch.empty_like(q), torch.empty(1, 2, 300, device="cuda")
-    a = rt._cross_args(q, k, v, out, "SHD", SCALE, None, lse)
-    n = C.c_size_t()
-    from h3attention.runtime import _bview
-
-    grads = [torch.empty_like(x) for x in (q, k, v)]
-    a.out_grad, _ = _bview("do", do, "SHD", 0)
-    a.dq, a.dk, a.dv = (_bview("d", x, "SHD", 0)[0] for x in grads)
+    view = lambda x: _lib.BView(x.data_ptr(), x.stride(0), x.stride(1), x.stride(2))  # noqa: E731
+    a, n = _lib.CrossArgs(), C.c_size_t()
+    a.batch, a.q_len, a.kv_len, a.heads, a.kv_heads, a.head_dim, a.scale, a.lse = 1, 300, 300, 2, 1, 128, SCALE, lse.data_ptr()
+    a.q, a.k, a.v, a.out, a.out_grad, a.dq, a.dk, a.dv = (
+        view(x) for x in (q, k, v, out, do, torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)))
     L = _lib.load()
     assert L.h3c_cross_workspace_size(C.byref(a), _lib.H3C_OP_CROSS_BWD, C.byref(n), None, 0) == _lib.H3C_OK and n.value
     ws = torch.empty(n.value, dtype=torch.uint8, device="cuda")
