@@ -30,13 +30,39 @@ struct CrossLaunch {
   uint64_t wait_limit_ns;
 };
 
+// n / d for n < 2^31, d >= 1: m = ceil(2^(31 + s) / d) with 2^s >= d.
+struct Div {
+  uint32_t m, s;
+  __device__ uint32_t operator()(uint32_t n) const { return (uint32_t)(((uint64_t)n * m) >> (31 + s)); }
+};
+
+inline Div make_div(uint32_t d) {
+  uint32_t s = 0;
+  while ((1ull << s) < d) ++s;
+  return {(uint32_t)(((1ull << (31 + s)) + d - 1) / d), s};
+}
+
+// Members whose lengths a kernel keeps in shared memory: with all of it taken
+// by tiles, the lengths do not stay in L1, and a role that starts a unit would
+// wait for L2 (1,000 cycles under load).
+constexpr int kLens = 64;
+
+// The 128-byte swizzle needs tiles on 1024-byte boundaries: so dynamic shared
+// memory starts (the declaration's alignment), which this checks.
+__device__ __forceinline__ bool tiles_aligned(const uint8_t* smem, int32_t* status) {
+  if (!(smem_u32(smem) & 1023)) return true;
+  if (threadIdx.x == 0) atomicExch(status, (int32_t)H3C_ERR_UNSUPPORTED);
+  return false;
+}
+
 __device__ __forceinline__ int kv_len_of(const int32_t* kv_lens, int kv_len, int b) {
   return kv_lens ? max(0, min(kv_len, kv_lens[b])) : kv_len;
 }
 
-// (d, token, head, batch) map of an operand, boxes of 64 x 128; a broadcast
-// axis has one element.
-inline bool make_map4(CUtensorMap* m, const Rows& r, int tokens, int heads, int batch, std::string* err) {
+// (d, token, head, batch) map of an operand, boxes of 64 x box_tokens; a
+// broadcast axis has one element.
+inline bool make_map4(CUtensorMap* m, const Rows& r, int tokens, int heads, int batch, std::string* err,
+                      int box_tokens = 128) {
   EncodeTiledFn enc = get_encode();
   if (!enc) {
     *err += "cuTensorMapEncodeTiled unavailable; ";
@@ -45,7 +71,7 @@ inline bool make_map4(CUtensorMap* m, const Rows& r, int tokens, int heads, int 
   cuuint64_t dims[4] = {128, (cuuint64_t)tokens, r.h ? (cuuint64_t)heads : 1, r.b ? (cuuint64_t)batch : 1};
   cuuint64_t strides[3] = {r.t ? (cuuint64_t)r.t * 2 : 256, r.h ? (cuuint64_t)r.h * 2 : 256,
                            r.b ? (cuuint64_t)r.b * 2 : 256};
-  cuuint32_t box[4] = {64, 128, 1, 1};
+  cuuint32_t box[4] = {64, (cuuint32_t)box_tokens, 1, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   CUresult res = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, r.p, dims, strides, box, estr,
                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,

@@ -13,8 +13,8 @@
 // writes delta and -lse2 for dkv_kernel, padded to whole blocks of queries
 // (-inf there, so that P is 0).
 //
-// Roles of a CTA's 12 warps: 0 TMA producer, 1 MMA issuer, 2 TMEM owner,
-// 4-7 and 8-11 elementwise: each warpgroup takes 64 of a tile's 128 columns of
+// Roles of a CTA's 12 warps: 0 TMA producer, 1 MMA issuer, 2 TMEM owner (and
+// a second issuer in dq_kernel), 4-7 and 8-11 elementwise: each warpgroup takes 64 of a tile's 128 columns of
 // every row (thread = row = TMEM lane).  Every wait is bounded (attn_tc.cu).
 //
 // dkv_kernel's work, all (key tile, query block) pairs in a row, is cut into
@@ -46,6 +46,7 @@ struct BwdArgs {
   int32_t* status;
   uint64_t wait_limit_ns;
   int32_t q_b, q_h, k_b, k_h, v_b, v_h, g_b, g_h;
+  Div by_blocks, by_heads, by_group;
 };
 
 __device__ __forceinline__ uint64_t pair2(uint32_t lo, uint32_t hi) {
@@ -86,25 +87,6 @@ __device__ __forceinline__ void bulk_512(uint32_t dst, const float* src, uint32_
       : "memory");
 }
 
-// D (+)= A B^T over 128 channels, A and B K-major tiles in shared memory
-__device__ __forceinline__ void mma_tile_ss(uint32_t d, uint32_t a, uint32_t b) {
-  const uint64_t da = smem_desc(a, 16, 1024), db = smem_desc(b, 16, 1024);
-#pragma unroll
-  for (int kk = 0; kk < 8; ++kk) {
-    const uint32_t off = (kk >> 2) * kHalfBytes + (kk & 3) * 32;
-    mma_ss_w(d, da + (uint64_t)(off >> 4), db + (uint64_t)(off >> 4), kIdKK, kk > 0 ? 1u : 0u);
-  }
-}
-
-// D (+)= A B, A packed bf16 in TMEM (steps 0-3 at a0, 4-7 at a1), B a tile
-// with the summed axis along its rows
-__device__ __forceinline__ void mma_tile_ts(uint32_t d, uint32_t a0, uint32_t a1, uint32_t b, bool acc) {
-  const uint64_t db = smem_desc(b, kHalfBytes, 1024);
-#pragma unroll
-  for (int kk = 0; kk < 8; ++kk)
-    mma_ts_w(d, (kk < 4 ? a0 : a1) + (kk & 3) * 8, db + (uint64_t)((kk * 2048) >> 4), kIdKM, acc || kk > 0 ? 1u : 0u);
-}
-
 __device__ __forceinline__ void load64(uint32_t addr, uint32_t* v) {
 #pragma unroll
   for (int c = 0; c < 4; ++c) H3_TMEM_LD16(addr + 16 * c, (&v[16 * c]));
@@ -140,12 +122,18 @@ __device__ __forceinline__ void release_tmem(int warp, uint32_t tmem, volatile i
 }
 
 // --------------------------------------------------------------------- dq
-// Shared memory: q and do of two units (128 KB), two K tiles, one V tile.
+// Shared memory: q and do of the unit, three K and two V tiles (224 KB).
 // TMEM columns: dq 0, S 128, dP 256, dS (two buffers) 384 and 448.  Of block
-// e+1, S and dP run while block e is in the elementwise warps; dq of e follows.
-struct __align__(8) DqBarriers {
-  uint64_t qd_full[2], qd_empty[2];  // unit u on [u & 1]
-  uint64_t k_full[2], k_empty[2], v_full, v_empty;
+// e+1, S and dP run while block e is in the elementwise warps; dq of e
+// follows, so a K tile is held for two blocks and needs the third buffer to
+// be loaded ahead.  delta comes from do in shared memory and out rows that the
+// elementwise warps fetch into registers a unit ahead.  Global rows are read
+// and written eight lanes a row (128 bytes of it): a thread a row, 32 lines an
+// instruction, kept the load/store unit busy for 4,000 cycles a unit each way.
+struct __align__(16) DqBarriers {
+  float red[2][128];                 // halves of delta
+  uint64_t q_full, q_empty, g_full, g_empty;
+  uint64_t k_full[3], k_empty[3], v_full[2], v_empty[2];
   uint64_t s_full, s_empty, dp_full, dp_empty, dq_full, dq_empty, red_full, done;
   // block e on [e & 1]: S and dP of e + 1 are issued before the issuer waits
   // for dS of e, so one barrier could complete twice before that wait
@@ -153,55 +141,93 @@ struct __align__(8) DqBarriers {
   uint32_t tmem_base;
   int32_t abort;
   int32_t info[8];
-  float red[2][128];                 // halves of delta
+  int32_t lens[kLens];
 };
 constexpr int kDqTiles = 7 * kTileBytes;
-constexpr int kDqSmem = kDqTiles + 1024 + (int)sizeof(DqBarriers);
+constexpr int kDqSmem = kDqTiles + (int)sizeof(DqBarriers);
 static_assert(kDqSmem <= 227 * 1024, "shared memory");
 
 struct DqUnit {
   int b, h, t0, len, n;
-  __device__ DqUnit(const BwdArgs& a, int u) {
-    const int x = u / a.q_blocks;
+  __device__ DqUnit(const BwdArgs& a, const int32_t* lens, int u) {
+    const int x = a.by_blocks(u);
     t0 = (u - x * a.q_blocks) * 128;
-    b = x / a.n.heads;
+    b = a.by_heads(x);
     h = x - b * a.n.heads;
-    len = kv_len_of(a.kv_lens, a.n.kv_len, b);
+    len = b < kLens ? lens[b] : kv_len_of(a.kv_lens, a.n.kv_len, b);
     n = (len + 127) >> 7;
   }
 };
+
+// 8x8 transpose over groups of eight lanes: v[i] of lane j and v[j] of lane i
+// change places, so that a thread's row becomes 16 bytes of each of eight rows.
+__device__ __forceinline__ void transpose8(uint4 (&v)[8]) {
+  const int p = threadIdx.x & 7;
+#pragma unroll
+  for (int s = 1; s < 8; s <<= 1) {
+    const bool up = p & s;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (i & s) continue;
+      uint4 m = up ? v[i] : v[i | s];
+      m.x = __shfl_xor_sync(0xffffffffu, m.x, s);
+      m.y = __shfl_xor_sync(0xffffffffu, m.y, s);
+      m.z = __shfl_xor_sync(0xffffffffu, m.z, s);
+      m.w = __shfl_xor_sync(0xffffffffu, m.w, s);
+      if (up) v[i] = m;
+      else v[i | s] = m;
+    }
+  }
+}
+
+__device__ __forceinline__ float dot8(const uint4& x, const uint4& y) {
+  const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    s = fmaf(__uint_as_float(xw[i] << 16), __uint_as_float(yw[i] << 16), s);
+    s = fmaf(__uint_as_float(xw[i] & 0xffff0000u), __uint_as_float(yw[i] & 0xffff0000u), s);
+  }
+  return s;
+}
 
 __global__ void __launch_bounds__(kThreads, 1)
     dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
               const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_g,
               const __grid_constant__ BwdArgs a, int units) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  uint8_t *sQ = smem, *sG = smem + 2 * kTileBytes, *sK = smem + 4 * kTileBytes, *sV = smem + 6 * kTileBytes;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if (!tiles_aligned(smem, a.status)) return;
+  uint8_t *sQ = smem, *sG = smem + kTileBytes, *sK = smem + 2 * kTileBytes, *sV = smem + 5 * kTileBytes;
   DqBarriers* bars = (DqBarriers*)(smem + kDqTiles);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int32_t* abort_flag = &bars->abort;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(smem_u32(&bars->qd_full[i]), 1);
-      mbar_init(smem_u32(&bars->qd_empty[i]), 257);  // the unit's last product and 256 readers of do
+    for (int i = 0; i < 3; ++i) {
       mbar_init(smem_u32(&bars->k_full[i]), 1);
       mbar_init(smem_u32(&bars->k_empty[i]), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&bars->v_full[i]), 1);
+      mbar_init(smem_u32(&bars->v_empty[i]), 1);
       mbar_init(smem_u32(&bars->ds_full[i]), 256);
     }
-    mbar_init(smem_u32(&bars->v_full), 1);
-    mbar_init(smem_u32(&bars->v_empty), 1);
+    mbar_init(smem_u32(&bars->q_full), 1);
+    mbar_init(smem_u32(&bars->q_empty), 1);
+    mbar_init(smem_u32(&bars->g_full), 1);
+    mbar_init(smem_u32(&bars->g_empty), 257);  // the unit's last product and 256 readers of do
+    mbar_init(smem_u32(&bars->red_full), 256);
     mbar_init(smem_u32(&bars->s_full), 1);
     mbar_init(smem_u32(&bars->s_empty), 256);
     mbar_init(smem_u32(&bars->dp_full), 1);
     mbar_init(smem_u32(&bars->dp_empty), 256);
     mbar_init(smem_u32(&bars->dq_full), 1);
     mbar_init(smem_u32(&bars->dq_empty), 256);
-    mbar_init(smem_u32(&bars->red_full), 256);
-    mbar_init(smem_u32(&bars->done), 1);
+    mbar_init(smem_u32(&bars->done), 2);
     bars->abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (threadIdx.x >= 128 && threadIdx.x < 128 + kLens && threadIdx.x - 128 < a.n.batch)
+    bars->lens[threadIdx.x - 128] = kv_len_of(a.kv_lens, a.n.kv_len, threadIdx.x - 128);
   const uint32_t tmem = alloc_tmem(warp, &bars->tmem_base);
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     return mbar_wait(smem_u32(bar), parity, abort_flag, a.status, a.wait_limit_ns);
@@ -210,127 +236,139 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 0 && lane == 0) {
-      int e = 0, qn = 0;           // key tiles and units loaded
+      // a K tile, then what is needed next, so that no load waits behind one
+      // whose buffer frees later
+      int e = 0, qn = 0, nv = 0, ng = 0;  // K tiles, q tiles, V tiles, do tiles loaded
+      int kr = 0;
+      uint32_t kp = 0;
       bool ok = true;
-      auto next_unit = [&](int u) {  // the next unit with keys
-        while (u < units && DqUnit(a, u).n == 0) u += gridDim.x;
-        return u;
-      };
-      auto load_q = [&](int u) {
-        const DqUnit x(a, u);
-        const int i = qn & 1;
-        if (!wait(&bars->qd_empty[i], ((qn >> 1) & 1) ^ 1)) return false;
-        const uint32_t bar = smem_u32(&bars->qd_full[i]);
-        mbar_expect_tx(bar, 2 * kTileBytes);
-        tma_tile(smem_u32(sQ + i * kTileBytes), &tm_q, bar, x.t0, x.h * a.q_h, x.b * a.q_b);
-        tma_tile(smem_u32(sG + i * kTileBytes), &tm_g, bar, x.t0, x.h * a.g_h, x.b * a.g_b);
-        ++qn;
-        return true;
-      };
-      int u = next_unit(blockIdx.x);
-      if (u < units) ok = load_q(u);
-      while (ok && u < units) {
-        const DqUnit x(a, u);
-        const int hk = x.h / a.n.group;
-        const int following = next_unit(u + gridDim.x);
-        for (int j = 0; ok && j < x.n; ++j, ++e) {
-          const int i = e & 1;
-          if (!wait(&bars->k_empty[i], ((e >> 1) & 1) ^ 1)) {
-            ok = false;
-            break;
-          }
+      for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
+        const DqUnit x(a, bars->lens, u);
+        const int hk = a.by_group(x.h);
+        for (int j = 0; j < x.n; ++j) {
+          if (!(ok = wait(&bars->k_empty[kr], kp ^ 1))) break;
           const int valid = x.len - 128 * j;
           // key rows past the member's length hold whatever the caller left
           // there: the issuer clears them (0 x NaN would reach dq)
           bars->info[e & 7] = (j == 0 ? kFirst : 0) | (j == x.n - 1 ? kLast : 0) |
                               (valid < 128 && x.len < a.n.kv_len ? valid << kZeroShift : 0);
-          uint32_t bar = smem_u32(&bars->k_full[i]);
+          uint32_t bar = smem_u32(&bars->k_full[kr]);
           mbar_expect_tx(bar, kTileBytes);
-          tma_tile(smem_u32(sK + i * kTileBytes), &tm_k, bar, 128 * j, hk * a.k_h, x.b * a.k_b);
-          if (!wait(&bars->v_empty, (e & 1) ^ 1)) {
-            ++e;
-            ok = false;
-            break;
+          tma_tile(smem_u32(sK + kr * kTileBytes), &tm_k, bar, 128 * j, hk * a.k_h, x.b * a.k_b);
+          ++e;
+          if (++kr == 3) {
+            kr = 0;
+            kp ^= 1;
           }
-          bar = smem_u32(&bars->v_full);
+          if (j == 0) {
+            if (!(ok = wait(&bars->q_empty, (qn & 1) ^ 1))) break;
+            bar = smem_u32(&bars->q_full);
+            mbar_expect_tx(bar, kTileBytes);
+            tma_tile(smem_u32(sQ), &tm_q, bar, x.t0, x.h * a.q_h, x.b * a.q_b);
+            ++qn;
+          }
+          if (!(ok = wait(&bars->v_empty[nv & 1], ((nv >> 1) & 1) ^ 1))) break;
+          bar = smem_u32(&bars->v_full[nv & 1]);
           mbar_expect_tx(bar, kTileBytes);
-          tma_tile(smem_u32(sV), &tm_v, bar, 128 * j, hk * a.v_h, x.b * a.v_b);
-          if (j == 0 && following < units) ok = load_q(following);
+          tma_tile(smem_u32(sV + (nv & 1) * kTileBytes), &tm_v, bar, 128 * j, hk * a.v_h, x.b * a.v_b);
+          ++nv;
+          if (j == 0) {
+            if (!(ok = wait(&bars->g_empty, (ng & 1) ^ 1))) break;
+            bar = smem_u32(&bars->g_full);
+            mbar_expect_tx(bar, kTileBytes);
+            tma_tile(smem_u32(sG), &tm_g, bar, x.t0, x.h * a.g_h, x.b * a.g_b);
+            ++ng;
+          }
         }
-        u = following;
       }
-      if (ok && wait(&bars->k_empty[e & 1], ((e >> 1) & 1) ^ 1)) {
+      if (ok && wait(&bars->k_empty[kr], kp ^ 1) && wait(&bars->v_empty[nv & 1], ((nv >> 1) & 1) ^ 1)) {
         bars->info[e & 7] = kEnd;
-        mbar_arrive(smem_u32(&bars->k_full[e & 1]));
+        mbar_arrive(smem_u32(&bars->k_full[kr]));
+        mbar_arrive(smem_u32(&bars->v_full[nv & 1]));
       } else {  // abort: every load in flight lands before anyone may exit
         volatile int32_t zero = 0;
-        for (int i = 0; i < 2; ++i) {
-          const int ke = e - 1 - ((e - 1 - i) & 1), qe = qn - 1 - ((qn - 1 - i) & 1);
-          if (ke >= 0) mbar_wait(smem_u32(&bars->k_full[i]), (ke >> 1) & 1, &zero, nullptr);
-          if (qe >= 0) mbar_wait(smem_u32(&bars->qd_full[i]), (qe >> 1) & 1, &zero, nullptr);
-        }
-        // of the last two V loads at least the older one was issued
-        if (e >= 2) mbar_wait(smem_u32(&bars->v_full), e & 1, &zero, nullptr, 1000000);
-        if (e >= 1) mbar_wait(smem_u32(&bars->v_full), (e - 1) & 1, &zero, nullptr, 1000000);
+        for (int x = max(0, e - 3); x < e; ++x)
+          mbar_wait(smem_u32(&bars->k_full[x % 3]), (x / 3) & 1, &zero, nullptr);
+        for (int x = max(0, nv - 2); x < nv; ++x)
+          mbar_wait(smem_u32(&bars->v_full[x & 1]), (x >> 1) & 1, &zero, nullptr);
+        if (qn) mbar_wait(smem_u32(&bars->q_full), (qn - 1) & 1, &zero, nullptr);
+        if (ng) mbar_wait(smem_u32(&bars->g_full), (ng - 1) & 1, &zero, nullptr);
       }
-    } else if (warp == 1) {
+    } else if (warp == 1 || warp == 2) {
+      // Two issuers, one of S and one of dP and dq, so that the waits of one
+      // (100-200 cycles each) pass while the products of the other run.
       auto iwait = [&](uint64_t* bar, uint32_t par) -> bool {
         int got = 0;
         if (lane == 0) got = wait(bar, par) ? 1 : 0;
         return __shfl_sync(0xffffffff, got, 0) != 0;
       };
-      int e = 0, pinfo = 0, units_s = 0, units_q = 0;
-      bool ok = true;
-      auto issue_dq = [&](int p, int info) -> bool {  // dq += dS_p K_p
-        if (info & kFirst) {
-          if (units_q > 0 && !iwait(&bars->dq_empty, (units_q - 1) & 1)) return false;
-          ++units_q;
+      int e = 0, un = 0, kr = 0;
+      if (warp == 1) {
+        uint32_t kp = 0;
+        while (iwait(&bars->k_full[kr], kp)) {
+          tc_fence_after();
+          const int info = ((volatile int32_t*)bars->info)[e & 7];
+          if (info & kEnd) break;
+          if (info >> kZeroShift) {
+            uint4* k = reinterpret_cast<uint4*>(sK + kr * kTileBytes);
+            for (int x = (info >> kZeroShift) * 8 + lane; x < 1024; x += 32) k[x] = k[1024 + x] = make_uint4(0, 0, 0, 0);
+            fence_async_shared();
+            __syncwarp();
+          }
+          if (info & kFirst) {
+            if (!iwait(&bars->q_full, un & 1)) break;
+            ++un;
+          }
+          if (e > 0 && !iwait(&bars->s_empty, (e - 1) & 1)) break;
+          tc_fence_after();
+          mma_tile_ss(tmem + 128, desc_lo(smem_u32(sQ), 16), desc_lo(smem_u32(sK + kr * kTileBytes), 16), kIdKK, 0);
+          tc_commit_w(smem_u32(&bars->s_full));
+          if (info & kLast) tc_commit_w(smem_u32(&bars->q_empty));
+          ++e;
+          if (++kr == 3) {
+            kr = 0;
+            kp ^= 1;
+          }
         }
-        if (!iwait(&bars->ds_full[p & 1], (p >> 1) & 1)) return false;
-        tc_fence_after();
-        const uint32_t ds = tmem + 384 + 64 * (p & 1);
-        mma_tile_ts(tmem, ds, ds + 32, smem_u32(sK + (p & 1) * kTileBytes), !(info & kFirst));
-        tc_commit_w(smem_u32(&bars->k_empty[p & 1]));
-        if (info & kLast) tc_commit_w(smem_u32(&bars->dq_full));
-        return true;
-      };
-      while (true) {
-        const int i = e & 1;
-        ok = iwait(&bars->k_full[i], (e >> 1) & 1);
-        if (!ok) break;
-        tc_fence_after();
-        const int info = ((volatile int32_t*)bars->info)[e & 7];
-        if (info & kEnd) break;
-        if (info >> kZeroShift) {
-          uint4* k = reinterpret_cast<uint4*>(sK + i * kTileBytes);
-          for (int x = (info >> kZeroShift) * 8 + lane; x < 1024; x += 32) k[x] = k[1024 + x] = make_uint4(0, 0, 0, 0);
-          fence_async_shared();
-          __syncwarp();
+      } else {
+        int dn = 0, pk = 0;
+        auto issue_dq = [&](int p, int info, int k) -> bool {  // dq += dS_p K_p
+          if (info & kFirst) {
+            if (dn > 0 && !iwait(&bars->dq_empty, (dn - 1) & 1)) return false;
+            ++dn;
+          }
+          if (!iwait(&bars->ds_full[p & 1], (p >> 1) & 1)) return false;
+          tc_fence_after();
+          const uint32_t ds = tmem + 384 + 64 * (p & 1);
+          mma_tile_ts(tmem, ds, desc_lo(smem_u32(sK + k * kTileBytes), kHalfBytes), kIdKM, !(info & kFirst));
+          tc_commit_w(smem_u32(&bars->k_empty[k]));
+          if (info & kLast) tc_commit_w(smem_u32(&bars->dq_full));
+          return true;
+        };
+        int pinfo = kLast;  // no product of the block before is due
+        while (iwait(&bars->v_full[e & 1], (e >> 1) & 1)) {
+          const int info = ((volatile int32_t*)bars->info)[e & 7];
+          if (info & kEnd) break;
+          if (info & kFirst) {
+            if (!iwait(&bars->g_full, un & 1)) break;
+            ++un;
+          }
+          if (e > 0 && !iwait(&bars->dp_empty, (e - 1) & 1)) break;
+          tc_fence_after();
+          mma_tile_ss(tmem + 256, desc_lo(smem_u32(sG), 16), desc_lo(smem_u32(sV + (e & 1) * kTileBytes), 16), kIdKK, 0);
+          tc_commit_w(smem_u32(&bars->dp_full));
+          tc_commit_w(smem_u32(&bars->v_empty[e & 1]));
+          if (info & kLast) tc_commit_w(smem_u32(&bars->g_empty));
+          // dq of the block before; of a unit's last block at once, as the next
+          // dP waits for the next unit's do
+          if (!(pinfo & kLast) && !issue_dq(e - 1, pinfo, pk)) break;
+          if ((info & kLast) && !issue_dq(e, info, kr)) break;
+          pinfo = info;
+          pk = kr;
+          ++e;
+          if (++kr == 3) kr = 0;
         }
-        if (info & kFirst) {
-          ok = iwait(&bars->qd_full[units_s & 1], (units_s >> 1) & 1);
-          if (!ok) break;
-          ++units_s;
-        }
-        const int qi = (units_s - 1) & 1;
-        ok = e == 0 || iwait(&bars->s_empty, (e - 1) & 1);
-        if (!ok) break;
-        tc_fence_after();
-        mma_tile_ss(tmem + 128, smem_u32(sQ + qi * kTileBytes), smem_u32(sK + i * kTileBytes));
-        tc_commit_w(smem_u32(&bars->s_full));
-        ok = iwait(&bars->v_full, e & 1) && (e == 0 || iwait(&bars->dp_empty, (e - 1) & 1));
-        if (!ok) break;
-        tc_fence_after();
-        mma_tile_ss(tmem + 256, smem_u32(sG + qi * kTileBytes), smem_u32(sV));
-        tc_commit_w(smem_u32(&bars->dp_full));
-        tc_commit_w(smem_u32(&bars->v_empty));
-        if (info & kLast) tc_commit_w(smem_u32(&bars->qd_empty[qi]));
-        ok = e == 0 || issue_dq(e - 1, pinfo);
-        if (!ok) break;
-        pinfo = info;
-        ++e;
       }
-      if (ok && e > 0) issue_dq(e - 1, pinfo);
       tc_commit_w(smem_u32(&bars->done));
     }
   } else {
@@ -340,60 +378,48 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int w = (warp - 4) >> 2, q = warp & 3, r = 32 * q + lane;
     const uint32_t lane_base = tmem + ((uint32_t)(32 * q) << 16);
     const uint64_t sl2 = dup2(a.scale * kLog2e);
+    // the next unit with keys: 16 bytes of rows 4i + lane / 8 of this warp's
+    // half rows of out, and this thread's row's lse
+    uint4 o[8];
+    float lse = INFINITY;  // rows past the end: P = 0
+    auto fetch = [&](int u) {
+      while (u < units) {
+        const DqUnit x(a, bars->lens, u);
+        if (x.n) {
+          const int tok = x.t0 + r, t1 = x.t0 + 32 * q + (lane >> 3);
+          lse = INFINITY;
+          if (tok < a.n.q_len) lse = a.lse[((int64_t)x.b * a.n.heads + x.h) * a.n.q_len + tok];
+          const uint16_t* po = a.out.at(x.b, t1, x.h) + 64 * w + 8 * (lane & 7);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            o[i] = make_uint4(0, 0, 0, 0);
+            if (t1 + 4 * i < a.n.q_len) o[i] = *reinterpret_cast<const uint4*>(po + (int64_t)4 * i * a.out.t);
+          }
+          return;
+        }
+        u += gridDim.x;
+      }
+    };
+    fetch(blockIdx.x);
     int e = 0, un = 0;
     bool ok = true;
     for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
-      const DqUnit x(a, u);
+      const DqUnit x(a, bars->lens, u);
       const int tok = x.t0 + r;
-      const bool live = tok < a.n.q_len;
-      uint4* go = reinterpret_cast<uint4*>(live ? a.dq.at(x.b, tok, x.h) + 64 * w : nullptr);
+      // rows 8 (lane / 8) + i of this warp's 32, 16 bytes a lane
+      const int t1 = x.t0 + 32 * q + 8 * (lane >> 3);
+      uint16_t* go = a.dq.at(x.b, t1, x.h) + 64 * w + 8 * (lane & 7);
       if (x.n == 0) {
-        if (live)
 #pragma unroll
-          for (int c = 0; c < 8; ++c) go[c] = make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < 8; ++i)
+          if (t1 + i < a.n.q_len) *reinterpret_cast<uint4*>(go + i * a.dq.t) = make_uint4(0, 0, 0, 0);
         continue;
       }
-      // delta: this warpgroup's 64 channels, then both halves
-      const int64_t pad = ((int64_t)x.b * a.n.heads + x.h) * a.q_blocks * 128 + tok;
-      float nl2 = -INFINITY, half = 0.f;
-      uint4 o[8];
-      if (live) {
-        nl2 = a.lse[((int64_t)x.b * a.n.heads + x.h) * a.n.q_len + tok] * -kLog2e;
-        const uint4* po = reinterpret_cast<const uint4*>(a.out.at(x.b, tok, x.h) + 64 * w);
-#pragma unroll
-        for (int c = 0; c < 8; ++c) o[c] = po[c];
-      }
-      if (!wait_w(&bars->qd_full[un & 1], (un >> 1) & 1)) break;
-      if (live) {
-        const uint8_t* pg = sG + (un & 1) * kTileBytes + w * kHalfBytes + r * 128;
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          const uint4 g = *reinterpret_cast<const uint4*>(pg + ((c ^ (r & 7)) << 4));
-          const uint32_t gw[4] = {g.x, g.y, g.z, g.w}, ow[4] = {o[c].x, o[c].y, o[c].z, o[c].w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            half = fmaf(__uint_as_float(gw[i] << 16), __uint_as_float(ow[i] << 16), half);
-            half = fmaf(__uint_as_float(gw[i] & 0xffff0000u), __uint_as_float(ow[i] & 0xffff0000u), half);
-          }
-        }
-      }
-      mbar_arrive(smem_u32(&bars->qd_empty[un & 1]));
-      // every reader of the last unit's halves arrived on ds_full before this
-      // thread saw that unit's dq_full
-      bars->red[w][r] = half;
-      mbar_arrive(smem_u32(&bars->red_full));
-      if (!wait_w(&bars->red_full, un & 1)) break;
-      const float delta = bars->red[0][r] + bars->red[1][r];
-      if (w == 0) {
-        a.nl2[pad] = nl2;
-        a.delta[pad] = delta;
-      }
-      const uint64_t nl2x2 = dup2(nl2), ndelta = dup2(-delta);
+      const float nl2 = lse * -kLog2e;  // here, not in fetch, which must not wait for its loads
+      const uint64_t nl2x2 = dup2(nl2);
+      uint64_t ndelta = 0;
       for (int j = 0; j < x.n; ++j, ++e) {
-        if (!wait_w(&bars->s_full, e & 1)) {
-          ok = false;
-          break;
-        }
+        if (!(ok = wait_w(&bars->s_full, e & 1))) break;
         tc_fence_after();
         uint32_t s[64];
         load64(lane_base + 128 + 64 * w, s);
@@ -406,10 +432,34 @@ __global__ void __launch_bounds__(kThreads, 1)
           p[2 * c] = ex2(lo2(v));
           p[2 * c + 1] = ex2(hi2(v));
         }
-        if (!wait_w(&bars->dp_full, e & 1)) {
-          ok = false;
-          break;
+        if (j == 0) {
+          // delta: this warpgroup's 64 channels, then both halves
+          if (!(ok = wait_w(&bars->g_full, un & 1))) break;
+          // (every reader of the last unit's halves arrived on ds_full before
+          // this thread saw that unit's dq_full)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int row = 32 * q + 4 * i + (lane >> 3);
+            float v = dot8(*reinterpret_cast<const uint4*>(sG + w * kHalfBytes + row * 128 +
+                                                           (((lane & 7) ^ (row & 7)) << 4)), o[i]);
+            v += __shfl_xor_sync(0xffffffffu, v, 4);
+            v += __shfl_xor_sync(0xffffffffu, v, 2);
+            v += __shfl_xor_sync(0xffffffffu, v, 1);
+            if ((lane & 7) == 0) bars->red[w][row] = v;
+          }
+          mbar_arrive(smem_u32(&bars->g_empty));
+          mbar_arrive(smem_u32(&bars->red_full));
+          if (!(ok = wait_w(&bars->red_full, un & 1))) break;
+          const float delta = bars->red[0][r] + bars->red[1][r];
+          ndelta = dup2(-delta);
+          if (w == 0) {
+            const int64_t pad = ((int64_t)x.b * a.n.heads + x.h) * a.q_blocks * 128 + tok;
+            a.nl2[pad] = nl2;
+            a.delta[pad] = delta;
+          }
+          fetch(u + gridDim.x);
         }
+        if (!(ok = wait_w(&bars->dp_full, e & 1))) break;
         tc_fence_after();
         uint32_t d[64];
         load64(lane_base + 256 + 64 * w, d);
@@ -441,37 +491,41 @@ __global__ void __launch_bounds__(kThreads, 1)
       load64(lane_base + 64 * w, v);
       tc_fence_before();
       mbar_arrive(smem_u32(&bars->dq_empty));
-      if (live) {
+      uint4 k[8];
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          uint32_t k[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            k[i] = pack_bf16(__uint_as_float(v[8 * c + 2 * i]) * a.scale, __uint_as_float(v[8 * c + 2 * i + 1]) * a.scale);
-          go[c] = make_uint4(k[0], k[1], k[2], k[3]);
-        }
+      for (int c = 0; c < 8; ++c) {
+        const auto two = [&](int i) {
+          return pack_bf16(__uint_as_float(v[8 * c + i]) * a.scale, __uint_as_float(v[8 * c + i + 1]) * a.scale);
+        };
+        k[c] = make_uint4(two(0), two(2), two(4), two(6));
       }
+      transpose8(k);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (t1 + i < a.n.q_len) *reinterpret_cast<uint4*>(go + i * a.dq.t) = k[i];
     }
   }
   release_tmem(warp, tmem, abort_flag, &bars->done);
 }
 
 // ------------------------------------------------------------------ dk, dv
-// Shared memory: K and V of the unit (64 KB), q and do of two query blocks
-// (128 KB) with their -lse2 and delta.  TMEM columns: dk 0, dv 128, S^T 256,
-// dP^T 384; a warpgroup writes its half of P^T (dS^T) over its own half of
-// S^T (dP^T), so neither waits for the other's loads.
+// Shared memory: K and V of the unit, three q and two do tiles (224 KB), -lse2
+// and delta of two query blocks.  TMEM columns: dk 0, dv 128, S^T 256, dP^T
+// 384; a warpgroup writes its half of P^T (dS^T) over its own half of S^T
+// (dP^T), so neither waits for the other's loads.  A q tile is held from S(e) to dk(e), over one block's time
+// and a half, so it needs the third buffer to be loaded ahead.
 struct __align__(16) DkvBarriers {
   float nl2[2][128], delta[2][128];
   uint64_t kv_full, kv_empty;
-  uint64_t q_full[2], q_empty[2], g_empty[2];
+  uint64_t q_full[3], q_empty[3], g_full[2], g_empty[2];
   uint64_t s_full, dp_full, p_full, ds_full, acc_full, acc_empty, done;
   uint32_t tmem_base;
   int32_t abort;
   int32_t info[8];
 };
-constexpr int kDkvTiles = 6 * kTileBytes;
-constexpr int kDkvSmem = kDkvTiles + 1024 + (int)sizeof(DkvBarriers);
+constexpr int kDkvTiles = 7 * kTileBytes;
+constexpr int kDkvSmem = kDkvTiles + (int)sizeof(DkvBarriers);
+static_assert(kDkvSmem <= 227 * 1024, "shared memory");
 
 // The run of (key tile, query block) pairs of one CTA, over key tiles that
 // hold valid keys: tile order member, key head, tile.
@@ -517,16 +571,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_g,
                const __grid_constant__ BwdArgs a) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  uint8_t *sK = smem, *sV = smem + kTileBytes, *sQ = smem + 2 * kTileBytes, *sG = smem + 4 * kTileBytes;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if (!tiles_aligned(smem, a.status)) return;
+  uint8_t *sK = smem, *sV = smem + kTileBytes, *sQ = smem + 2 * kTileBytes, *sG = smem + 5 * kTileBytes;
   DkvBarriers* bars = (DkvBarriers*)(smem + kDkvTiles);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int32_t* abort_flag = &bars->abort;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 3; ++i) {
       mbar_init(smem_u32(&bars->q_full[i]), 1);
       mbar_init(smem_u32(&bars->q_empty[i]), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&bars->g_full[i]), 1);
       mbar_init(smem_u32(&bars->g_empty[i]), 1);
     }
     mbar_init(smem_u32(&bars->kv_full), 1);
@@ -549,98 +606,118 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 0 && lane == 0) {
       DkvWalk seg(a, blockIdx.x, gridDim.x);
-      int e = 0, sn = 0;           // query blocks and segments loaded
+      int e = 0, ng = 0, sn = 0, qr = 0;  // q tiles, do tiles and segments loaded
+      uint32_t qp = 0;
       bool ok = true;
       while (ok && seg.next(a)) {
-        if (!wait(&bars->kv_empty, (sn & 1) ^ 1)) {
-          ok = false;
-          break;
-        }
+        if (!(ok = wait(&bars->kv_empty, (sn & 1) ^ 1))) break;
         uint32_t bar = smem_u32(&bars->kv_full);
         mbar_expect_tx(bar, 2 * kTileBytes);
         tma_tile(smem_u32(sK), &tm_k, bar, 128 * seg.tile, seg.hk * a.k_h, seg.b * a.k_b);
         tma_tile(smem_u32(sV), &tm_v, bar, 128 * seg.tile, seg.hk * a.v_h, seg.b * a.v_b);
         ++sn;
         int g = seg.it0 / a.q_blocks, qb = seg.it0 - g * a.q_blocks;
-        for (int it = seg.it0; it < seg.it1; ++it, ++e) {
-          const int i = e & 1, h = seg.hk * a.n.group + g;
-          if (!wait(&bars->g_empty[i], ((e >> 1) & 1) ^ 1) || !wait(&bars->q_empty[i], ((e >> 1) & 1) ^ 1)) {
-            ok = false;
-            break;
-          }
+        for (int it = seg.it0; it < seg.it1; ++it) {
+          const int h = seg.hk * a.n.group + g;
+          if (!(ok = wait(&bars->q_empty[qr], qp ^ 1))) break;
           bars->info[e & 7] = (it == seg.it0 ? kFirst : 0) | (it == seg.it1 - 1 ? kLast : 0);
-          bar = smem_u32(&bars->q_full[i]);
-          mbar_expect_tx(bar, 2 * kTileBytes + 1024);
-          tma_tile(smem_u32(sQ + i * kTileBytes), &tm_q, bar, 128 * qb, h * a.q_h, seg.b * a.q_b);
+          bar = smem_u32(&bars->q_full[qr]);
+          mbar_expect_tx(bar, kTileBytes);
+          tma_tile(smem_u32(sQ + qr * kTileBytes), &tm_q, bar, 128 * qb, h * a.q_h, seg.b * a.q_b);
+          ++e;
+          if (++qr == 3) {
+            qr = 0;
+            qp ^= 1;
+          }
+          const int i = ng & 1;
+          if (!(ok = wait(&bars->g_empty[i], ((ng >> 1) & 1) ^ 1))) break;
+          bar = smem_u32(&bars->g_full[i]);
+          mbar_expect_tx(bar, kTileBytes + 1024);
           tma_tile(smem_u32(sG + i * kTileBytes), &tm_g, bar, 128 * qb, h * a.g_h, seg.b * a.g_b);
           const int64_t pad = (((int64_t)seg.b * a.n.heads + h) * a.q_blocks + qb) * 128;
           bulk_512(smem_u32(bars->nl2[i]), a.nl2 + pad, bar);
           bulk_512(smem_u32(bars->delta[i]), a.delta + pad, bar);
+          ++ng;
           if (++qb == a.q_blocks) {
             qb = 0;
             ++g;
           }
         }
       }
-      if (ok && wait(&bars->g_empty[e & 1], ((e >> 1) & 1) ^ 1) && wait(&bars->q_empty[e & 1], ((e >> 1) & 1) ^ 1)) {
+      if (ok && wait(&bars->q_empty[qr], qp ^ 1)) {
         bars->info[e & 7] = kEnd;
-        mbar_arrive(smem_u32(&bars->q_full[e & 1]));
-      } else {
+        mbar_arrive(smem_u32(&bars->q_full[qr]));
+      } else {  // abort: every load in flight lands before anyone may exit
         volatile int32_t zero = 0;
-        for (int x = max(0, e - 2); x < e; ++x) mbar_wait(smem_u32(&bars->q_full[x & 1]), (x >> 1) & 1, &zero, nullptr);
+        for (int x = max(0, e - 3); x < e; ++x)
+          mbar_wait(smem_u32(&bars->q_full[x % 3]), (x / 3) & 1, &zero, nullptr);
+        for (int x = max(0, ng - 2); x < ng; ++x)
+          mbar_wait(smem_u32(&bars->g_full[x & 1]), (x >> 1) & 1, &zero, nullptr);
         if (sn) mbar_wait(smem_u32(&bars->kv_full), (sn - 1) & 1, &zero, nullptr);
       }
     } else if (warp == 1) {
+      // dv(e-1) S(e) dk(e-1) dP(e): the order keeps P^T (dS^T) in place until
+      // its product has read it.  (A second issuer for dk and dP: 7% slower.)
       auto iwait = [&](uint64_t* bar, uint32_t par) -> bool {
         int got = 0;
         if (lane == 0) got = wait(bar, par) ? 1 : 0;
         return __shfl_sync(0xffffffff, got, 0) != 0;
       };
-      int e = 0, pinfo = 0, segs = 0, accs = 0;
+      int e = 0, pinfo = 0, segs = 0, accs = 0, qr = 0, pq = 0;
+      uint32_t qp = 0;
       bool ok = true;
-      auto issue_dv = [&](int p, int info) -> bool {  // dv += P^T do
-        if (info & kFirst) {
+      auto issue_dv = [&](int p) -> bool {  // dv += P^T do
+        if (pinfo & kFirst) {  // the epilogue of the last segment has read dk and dv
           if (accs > 0 && !iwait(&bars->acc_empty, (accs - 1) & 1)) return false;
           ++accs;
         }
         if (!iwait(&bars->p_full, p & 1)) return false;
         tc_fence_after();
-        mma_tile_ts(tmem + 128, tmem + 256, tmem + 320, smem_u32(sG + (p & 1) * kTileBytes), !(info & kFirst));
-        tc_commit_w(smem_u32(&bars->g_empty[p & 1]));
+        const uint32_t g = desc_lo(smem_u32(sG + (p & 1) * kTileBytes), kHalfBytes);
+        mma_tile_ts_0_4(tmem + 128, tmem + 256, g, kIdKM, !(pinfo & kFirst));
+        mma_tile_ts_4_8(tmem + 128, tmem + 320, g, kIdKM, 1);
         return true;
       };
-      auto issue_dk = [&](int p, int info) -> bool {  // dk += dS^T q
+      auto issue_dk = [&](int p) -> bool {  // dk += dS^T q
         if (!iwait(&bars->ds_full, p & 1)) return false;
         tc_fence_after();
-        mma_tile_ts(tmem, tmem + 384, tmem + 448, smem_u32(sQ + (p & 1) * kTileBytes), !(info & kFirst));
-        tc_commit_w(smem_u32(&bars->q_empty[p & 1]));
-        if (info & kLast) tc_commit_w(smem_u32(&bars->acc_full));
+        const uint32_t x = desc_lo(smem_u32(sQ + pq * kTileBytes), kHalfBytes);
+        mma_tile_ts_0_4(tmem, tmem + 384, x, kIdKM, !(pinfo & kFirst));
+        mma_tile_ts_4_8(tmem, tmem + 448, x, kIdKM, 1);
+        tc_commit_w(smem_u32(&bars->q_empty[pq]));
+        // do, and -lse2 and delta, which the elementwise warps have read
+        // before they handed dS over
+        tc_commit_w(smem_u32(&bars->g_empty[p & 1]));
+        if (pinfo & kLast) tc_commit_w(smem_u32(&bars->acc_full));
         return true;
       };
       while (true) {
-        const int i = e & 1;
-        ok = iwait(&bars->q_full[i], (e >> 1) & 1);
+        ok = (e == 0 || issue_dv(e - 1)) && iwait(&bars->q_full[qr], qp);
         if (!ok) break;
         const int info = ((volatile int32_t*)bars->info)[e & 7];
         if (info & kEnd) break;
-        ok = e == 0 || issue_dv(e - 1, pinfo);
-        if (ok && (info & kFirst)) {
-          ok = iwait(&bars->kv_full, segs & 1);
+        if (info & kFirst) {
+          if (!(ok = iwait(&bars->kv_full, segs & 1))) break;
           ++segs;
         }
+        tc_fence_after();
+        mma_tile_ss(tmem + 256, desc_lo(smem_u32(sK), 16), desc_lo(smem_u32(sQ + qr * kTileBytes), 16), kIdKK, 0);
+        tc_commit_w(smem_u32(&bars->s_full));
+        ok = (e == 0 || issue_dk(e - 1)) && iwait(&bars->g_full[e & 1], (e >> 1) & 1);
         if (!ok) break;
         tc_fence_after();
-        mma_tile_ss(tmem + 256, smem_u32(sK), smem_u32(sQ + i * kTileBytes));
-        tc_commit_w(smem_u32(&bars->s_full));
-        ok = e == 0 || issue_dk(e - 1, pinfo);
-        if (!ok) break;
-        mma_tile_ss(tmem + 384, smem_u32(sV), smem_u32(sG + i * kTileBytes));
+        mma_tile_ss(tmem + 384, desc_lo(smem_u32(sV), 16), desc_lo(smem_u32(sG + (e & 1) * kTileBytes), 16), kIdKK, 0);
         tc_commit_w(smem_u32(&bars->dp_full));
         if (info & kLast) tc_commit_w(smem_u32(&bars->kv_empty));
         pinfo = info;
+        pq = qr;
         ++e;
+        if (++qr == 3) {
+          qr = 0;
+          qp ^= 1;
+        }
       }
-      if (ok && e > 0) ok = issue_dv(e - 1, pinfo) && issue_dk(e - 1, pinfo);
+      if (ok && e > 0) issue_dk(e - 1);
       tc_commit_w(smem_u32(&bars->done));
     } else if (warp >= 2) {
       // gradients of key tiles without a valid key: 0
@@ -666,7 +743,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     while (ok && seg.next(a)) {
       for (int it = seg.it0; it < seg.it1; ++it, ++e) {
-        if (!wait_w(&bars->q_full[e & 1], (e >> 1) & 1) || !wait_w(&bars->s_full, e & 1)) {
+        if (!wait_w(&bars->g_full[e & 1], (e >> 1) & 1) || !wait_w(&bars->s_full, e & 1)) {
           ok = false;
           break;
         }
@@ -734,8 +811,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int i = 0; i < 8; ++i)
             k[i] = valid ? pack_bf16(__uint_as_float(v[2 * i]) * f, __uint_as_float(v[2 * i + 1]) * f) : 0u;
-          reinterpret_cast<uint4*>(go + 16 * c)[0] = make_uint4(k[0], k[1], k[2], k[3]);
-          reinterpret_cast<uint4*>(go + 16 * c)[1] = make_uint4(k[4], k[5], k[6], k[7]);
+          store32(go + 16 * c, k);
         }
       }
       tc_fence_before();
@@ -837,6 +913,7 @@ cudaError_t launch_cross_bwd(const CrossLaunch& L, cudaStream_t s, std::string* 
   a.lse = L.lse;
   a.scale = L.scale;
   a.q_blocks = (n.q_len + 127) / 128;
+  a.by_blocks = make_div(a.q_blocks), a.by_heads = make_div(n.heads), a.by_group = make_div(n.group);
   const int64_t rows = (int64_t)n.batch * n.heads * a.q_blocks * 128;
   a.nl2 = (float*)L.ws;
   a.delta = a.nl2 + rows;

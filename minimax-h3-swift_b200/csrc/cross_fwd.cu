@@ -11,7 +11,7 @@
 // source.  A CTA takes whole units in turn, or, where there are too few units
 // for the SMs, an equal share of all (unit, key tile) pairs in a row; a unit
 // that is cut, or whose rows have two sources, leaves fp32 partial results
-// (o, m, l) that combine_kernel joins in a fixed order.  Row blocks:
+// (o, m, l) that a second kernel joins in a fixed order.  Row blocks:
 //   dense   q_len >= 128: 2 x 128 tokens of one head, Q tiles by TMA; keys are
 //           the prefix's and then the member's own
 //   folded  q_len < 128: a row is (member, token, head of the group), so one
@@ -21,16 +21,18 @@
 //           More than 128 rows: two row tiles share each K/V tile (dual).
 //           Up to 128: the two halves of the CTA take alternate K/V tiles of
 //           the same rows (single) and their results are joined through TMEM;
-//           one half alone reaches 5.3 of the 6.5 TB/s that HBM gives.
+//           one half alone would reach 5.3 of the 6.5 TB/s that HBM gives.
 //
-// Roles of a CTA's 12 warps: 0 TMA producer; 1 MMA issuer; 2-3 gather folded
-// query rows (2 also owns TMEM); 4-7 and 8-11 softmax and epilogue of half 0
-// and 1, thread = row = TMEM lane.  TMEM: half t has S (then P, packed bf16,
-// over its first 64 columns) at 256t and O at 256t + 128.  K/V entries run
-// through a ring of 2 (3 in single mode, where each entry is needed for two
-// steps); the producer hands each entry's flags to the issuer through shared
-// memory.  The next unit's Q and K/V loads and its first S overlap the
-// epilogue of this one.  Every wait is bounded (see attn_tc.cu).
+// Roles of a CTA's 16 warps: 0 K/V producer (TMA); 1 MMA issuer; 2-3 query
+// rows (folded: gather; dense: one thread of 3 by TMA), 2 also owns TMEM; 4-7
+// and 8-11 softmax of half 0 and 1, thread = row = TMEM lane; 12-15 epilogue
+// of both halves.  TMEM: half t has S (then P, packed bf16, over its first 64
+// columns) at 256t and O at 256t + 128.  K/V entries run through a ring of 2
+// (3 in single mode, where each entry is needed for two steps); the producer
+// hands each entry's flags to the issuer through shared memory.  The next
+// unit's Q and K/V loads, its first S and softmax overlap the epilogue of
+// this one, which with 3-4 key tiles a unit is a third of a unit's time.
+// Every wait is bounded (see attn_tc.cu).
 #include <climits>
 #include <mutex>
 #include <type_traits>
@@ -40,7 +42,7 @@
 namespace h3 {
 namespace {
 
-constexpr int kThreads = 384;
+constexpr int kThreads = 512;
 constexpr int kSms = 148;
 
 enum { kDense = 0, kSingle = 1, kDual = 2 };
@@ -58,6 +60,7 @@ struct FwdPlan {
   int32_t slots_p, slots;     // partial results a row, at most: from the prefix's units, in all
   int32_t combine;
   int64_t part_rows;
+  Div by_per_p, by_per_o, by_tiles_p, by_tiles_o, by_heads, by_kv_heads, by_group, by_q_len, by_rows, by_tpc;
 };
 
 struct FwdArgs {
@@ -86,35 +89,35 @@ struct Seg {
 };
 
 struct SegIter {
-  int64_t pos, end;
+  uint32_t pos, end;          // key tiles of the linear split, or units
   __device__ explicit SegIter(const FwdPlan& p) {
     if (p.tpc) {
-      const int64_t total = (int64_t)p.units_p * p.tiles_p + (int64_t)p.units_o * p.tiles_o;
-      pos = (int64_t)blockIdx.x * p.tpc;
+      const uint32_t total = (uint32_t)(p.units_p * p.tiles_p + p.units_o * p.tiles_o);
+      pos = blockIdx.x * p.tpc;
       end = min(total, pos + p.tpc);
     } else {
       pos = blockIdx.x;
       end = p.units_p + p.units_o;
     }
   }
-  __device__ bool next(const FwdArgs& a, Seg& s) {
+  __device__ bool next(const FwdArgs& a, const int32_t* lens, Seg& s) {
     if (pos >= end) return false;
     const FwdPlan& p = a.p;
     int u, j1, tiles;
     s.slot = 0;
     if (p.tpc) {
-      const int64_t pre = (int64_t)p.units_p * p.tiles_p;
+      const uint32_t pre = p.units_p * p.tiles_p;
       const bool own = pos >= pre;
-      const int64_t off = own ? pos - pre : pos;
+      const uint32_t off = own ? pos - pre : pos;
       tiles = own ? p.tiles_o : p.tiles_p;
-      const int v = (int)(off / tiles);
+      const int v = own ? p.by_tiles_o(off) : p.by_tiles_p(off);
       u = own ? p.units_p + v : v;
-      s.j0 = (int)(off - (int64_t)v * tiles);
-      j1 = (int)min((int64_t)tiles, s.j0 + (end - pos));
-      s.slot = (int)(blockIdx.x - (pos - s.j0) / p.tpc);
+      s.j0 = (int)off - v * tiles;
+      j1 = min(tiles, s.j0 + (int)(end - pos));
+      s.slot = blockIdx.x - p.by_tpc(pos - s.j0);
       pos += j1 - s.j0;
     } else {
-      u = (int)pos;
+      u = pos;
       tiles = u < p.units_p ? p.tiles_p : p.tiles_o;
       s.j0 = 0;
       j1 = tiles;
@@ -122,23 +125,23 @@ struct SegIter {
     }
     int limit;
     if (u < p.units_p) {
-      s.hk = u / p.per_p;
+      s.hk = p.by_per_p(u);
       s.row0 = (u - s.hk * p.per_p) * p.unit_rows;
       s.row_end = min(p.fold_rows, s.row0 + p.unit_rows);
       s.b = 0;
       s.len = 0;
       s.npre = limit = p.np;
     } else {
-      const int v = u - p.units_p, x = v / p.per_o, rt = v - x * p.per_o;
+      const int v = u - p.units_p, x = p.by_per_o(v), rt = v - x * p.per_o;
       if (p.mode == kDense) {
-        s.b = x / a.n.heads;
+        s.b = p.by_heads(x);
         s.h = x - s.b * a.n.heads;
-        s.hk = s.h / a.n.group;
+        s.hk = p.by_group(s.h);
         s.row0 = rt * p.unit_rows;
         s.row_end = min(a.n.q_len, s.row0 + p.unit_rows);
         s.npre = p.np;
       } else {
-        s.b = x / a.n.kv_heads;
+        s.b = p.by_kv_heads(x);
         s.hk = x - s.b * a.n.kv_heads;
         const int rows = a.n.q_len * a.n.group;
         s.row0 = s.b * rows + rt * p.unit_rows;
@@ -146,7 +149,7 @@ struct SegIter {
         s.npre = 0;
         s.slot += p.slots_p;
       }
-      s.len = kv_len_of(a.kv_lens, a.n.kv_len, s.b);
+      s.len = s.b < kLens ? lens[s.b] : kv_len_of(a.kv_lens, a.n.kv_len, s.b);
       limit = s.npre + ((s.len + 127) >> 7);
     }
     s.n = max(0, min(j1, limit) - s.j0);
@@ -163,19 +166,20 @@ template <bool SINGLE>
 struct Layout {
   static constexpr int kRing = SINGLE ? 3 : 2;      // K/V entries
   static constexpr int kQTiles = SINGLE ? 1 : 2;
-  static constexpr int kTiles = (kQTiles + 2 * kRing) * kTileBytes;
+  // the rest of 224 KB in dense mode: two 4 KB output buffers an epilogue warp
+  static constexpr int kTiles = 7 * kTileBytes;
 };
 
 struct __align__(8) Barriers {
   uint64_t q_full[2], q_empty[2];
   uint64_t kv_full[3], k_empty[3], v_empty[3];
-  uint64_t s_full[2], p_half[2], p_full[2], o_full[2], o_empty[2];
-  uint64_t ml_full;
+  uint64_t s_full[2], p_half[2], p_full[2], o_full[2], o_empty[2], ml_full[2];
   uint64_t done;              // every MMA has retired
   uint32_t tmem_base;
   int32_t abort;
   int32_t info[16];           // flags of entry e at [e & 15]
-  float2 ml[128];             // single mode: maximum and sum of half 1
+  int32_t lens[kLens];
+  float2 ml[2][128];          // maximum and sum of a half's rows
 };
 
 // flags of an entry: bit t: half t takes it; 2 + t / 4 + t: first / last of the segment for half t
@@ -183,29 +187,22 @@ enum { kFirst = 2, kLast = 4, kSegFirst = 1 << 6, kSegLast = 1 << 7, kEnd = 1 <<
 
 template <bool SINGLE>
 constexpr int smem_bytes() {
-  return Layout<SINGLE>::kTiles + 1024 + (int)sizeof(Barriers);
+  return Layout<SINGLE>::kTiles + (int)sizeof(Barriers);
 }
 static_assert(smem_bytes<true>() <= 227 * 1024 && smem_bytes<false>() <= 227 * 1024, "shared memory");
 
 // Instruction descriptor, kind::f16: bf16 x bf16 -> f32, M = N = 128.
 constexpr uint32_t kIdS = idesc_bf16(false), kIdPV = idesc_bf16(true);
 
-__device__ __forceinline__ void store_row32(uint16_t* p, const float* v, float f) {
-  uint32_t w[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) w[i] = pack_bf16(v[2 * i] * f, v[2 * i + 1] * f);
-  reinterpret_cast<uint4*>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-  reinterpret_cast<uint4*>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
-}
-
 template <bool SINGLE>
 __global__ void __launch_bounds__(kThreads, 1)
     cross_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                      const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_pk,
-                     const __grid_constant__ CUtensorMap tm_pv, const __grid_constant__ FwdArgs a) {
+                     const __grid_constant__ CUtensorMap tm_pv, const __grid_constant__ CUtensorMap tm_o,
+                     const __grid_constant__ FwdArgs a) {
   using L = Layout<SINGLE>;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if (!tiles_aligned(smem, a.status)) return;
   uint8_t* sQ = smem;
   uint8_t* sKV = smem + L::kQTiles * kTileBytes;  // entry r: K at 2r, V at 2r + 1
   Barriers* bars = (Barriers*)(smem + L::kTiles);
@@ -222,17 +219,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(smem_u32(&bars->p_full[t]), 128);
       mbar_init(smem_u32(&bars->o_full[t]), 1);
       mbar_init(smem_u32(&bars->o_empty[t]), 128);
+      mbar_init(smem_u32(&bars->ml_full[t]), 128);
     }
     for (int r = 0; r < 3; ++r) {
       mbar_init(smem_u32(&bars->kv_full[r]), 1);
       mbar_init(smem_u32(&bars->k_empty[r]), 1);
       mbar_init(smem_u32(&bars->v_empty[r]), 1);
     }
-    mbar_init(smem_u32(&bars->ml_full), 128);
     mbar_init(smem_u32(&bars->done), 1);
     bars->abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (threadIdx.x >= 128 && threadIdx.x < 128 + kLens && threadIdx.x - 128 < a.n.batch)
+    bars->lens[threadIdx.x - 128] = kv_len_of(a.kv_lens, a.n.kv_len, threadIdx.x - 128);
   if (warp == 2) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(
                      smem_u32(&bars->tmem_base)));
@@ -247,36 +246,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     return mbar_wait(smem_u32(bar), parity, abort_flag, a.status, a.wait_limit_ns);
   };
 
-  // Register split of the launch's 384 x 168: 128 x 72 + 256 x 216.
+  // Register split of the launch's 512 x 128: 128 x 48 + 256 x 192 + 128 x 80.
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
     if (warp == 0) {
       // ------------------------------------------------------- TMA producer
       if (lane == 0) {
         SegIter it(a.p);
-        Seg s;
+        Seg s{};
         int ec = 0, r = 0, issued = 0;
         uint32_t ph = 0;
-        int qn[2] = {0, 0};
         bool ok = true;
-        while (ok && it.next(a, s)) {
+        while (ok && it.next(a, bars->lens, s)) {
           if (s.n == 0) continue;
           const bool act1 = !SINGLE && s.row0 + 128 < s.row_end;
-          if (!SINGLE && dense) {
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-              if (!ok || (t && !act1)) continue;
-              if (!wait(&bars->q_empty[t], (qn[t] & 1) ^ 1)) {
-                ok = false;
-                continue;
-              }
-              const uint32_t bar = smem_u32(&bars->q_full[t]), dst = smem_u32(sQ + t * kTileBytes);
-              mbar_expect_tx(bar, kTileBytes);
-              tma_load_4d(dst, &tm_q, bar, 0, s.row0 + 128 * t, s.h * a.q_h, s.b * a.q_b);
-              tma_load_4d(dst + kHalfBytes, &tm_q, bar, 64, s.row0 + 128 * t, s.h * a.q_h, s.b * a.q_b);
-              ++qn[t];
-            }
-          }
           for (int i = 0; ok && i < s.n; ++i) {
             const int j = s.j0 + i;
             int info;
@@ -330,9 +313,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           volatile int32_t zero = 0;
           for (int e = max(0, issued - L::kRing); e < issued; ++e)
             mbar_wait(smem_u32(&bars->kv_full[e % L::kRing]), (e / L::kRing) & 1, &zero, nullptr);
-          if (dense)
-            for (int t = 0; t < 2; ++t)
-              if (qn[t]) mbar_wait(smem_u32(&bars->q_full[t]), (qn[t] - 1) & 1, &zero, nullptr);
         }
       }
     } else if (warp == 1) {
@@ -342,70 +322,54 @@ __global__ void __launch_bounds__(kThreads, 1)
       // the halves alternate between tensor pipe and softmax.
       auto iwait = [&](uint64_t* bar, uint32_t par) -> bool {
         int got = 0;
-        if (lane == 0) got = wait(bar, par) ? 1 : 0;
+        if (lane == 0) got = wait(bar, par & 1) ? 1 : 0;
         return __shfl_sync(0xffffffff, got, 0) != 0;
       };
-      int pend0 = -1, pend1 = -1;    // entry whose PV is due
-      int pr0 = 0, pr1 = 0;          // its ring slot
-      int pf0 = 0, pf1 = 0;          // bit 0 first, bit 1 last of its segment
-      int ns0 = 0, ns1 = 0;          // S issued
-      int no0 = 0, no1 = 0;          // segments begun (O in use)
-      int nq0 = 0, nq1 = 0;          // Q tiles taken
+      // phase bits: 0 K/V ring, 1 + t Q, 3 + t P, 5 + t O
+      uint32_t ph = 0x60;
+      // entry whose PV is due: ring slot, its first / last flags as bits 4, 5; or -1
+      int pend0 = -1, pend1 = -1;
+      const uint32_t q_lo = desc_lo(smem_u32(sQ), 16), k_lo = desc_lo(smem_u32(sKV), 16);
+      const uint32_t v_lo = desc_lo(smem_u32(sKV) + kTileBytes, kHalfBytes);
+      constexpr uint32_t kTileLo = kTileBytes >> 4;
       int ec = 0, r = 0;
-      uint32_t ph = 0;
-      bool ok = true;
       using T0 = std::integral_constant<int, 0>;
       using T1 = std::integral_constant<int, 1>;
       auto issue_pv = [&](auto tile) -> bool {
         constexpr int t = decltype(tile)::value;
         int& pend = t == 0 ? pend0 : pend1;
-        int& no = t == 0 ? no0 : no1;
-        const int pr = t == 0 ? pr0 : pr1, pf = t == 0 ? pf0 : pf1, ns = t == 0 ? ns0 : ns1;
-        const int other = t == 0 ? pend1 : pend0;
-        if (pf & 1) {  // the epilogue of the half's last segment has read O
-          if (no > 0 && !iwait(&bars->o_empty[t], (no - 1) & 1)) return false;
-          ++no;
+        const int slot = pend & 15, other = t == 0 ? pend1 : pend0;
+        if (pend & 16) {  // the epilogue of the half's last segment has read O
+          if (!iwait(&bars->o_empty[t], ph >> (5 + t))) return false;
+          ph ^= 1u << (5 + t);
         }
-        if (!iwait(&bars->p_half[t], (ns - 1) & 1)) return false;
+        if (!iwait(&bars->p_half[t], ph >> (3 + t))) return false;
         tc_fence_after();
-        const uint64_t vdesc = smem_desc(smem_u32(sKV + (2 * pr + 1) * kTileBytes), kHalfBytes, 1024);
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk) {
-          if (kk == 6) {
-            if (!iwait(&bars->p_full[t], (ns - 1) & 1)) return false;
-            tc_fence_after();
-          }
-          mma_ts_w(tmem + 256 * t + 128, tmem + 256 * t + kk * 8, vdesc + (uint64_t)((kk * 2048) >> 4), kIdPV,
-                   (!(pf & 1) || kk > 0) ? 1u : 0u);
-        }
-        if (pf & 2) tc_commit_w(smem_u32(&bars->o_full[t]));
-        if (other != pend) tc_commit_w(smem_u32(&bars->v_empty[pr]));
+        const uint32_t b = v_lo + 2 * slot * kTileLo;
+        mma_tile_ts_0_6(tmem + 256 * t + 128, tmem + 256 * t, b, kIdPV, !(pend & 16));
+        if (!iwait(&bars->p_full[t], ph >> (3 + t))) return false;
+        tc_fence_after();
+        ph ^= 1u << (3 + t);
+        mma_tile_ts_6_8(tmem + 256 * t + 128, tmem + 256 * t, b, kIdPV, 1);
+        if (pend & 32) tc_commit_w(smem_u32(&bars->o_full[t]));
+        if (other < 0 || (other & 15) != slot) tc_commit_w(smem_u32(&bars->v_empty[slot]));
         pend = -1;
         return true;
       };
       auto issue_s = [&](auto tile, int info) -> bool {
         constexpr int t = decltype(tile)::value;
         if (!SINGLE && (info & (1 << (kFirst + t)))) {
-          int& nq = t == 0 ? nq0 : nq1;
-          if (!iwait(&bars->q_full[t], nq & 1)) return false;
+          if (!iwait(&bars->q_full[t], ph >> (1 + t))) return false;
           tc_fence_after();
-          ++nq;
+          ph ^= 1u << (1 + t);
         }
-        const uint64_t qdesc = smem_desc(smem_u32(sQ + (SINGLE ? 0 : t) * kTileBytes), 16, 1024);
-        const uint64_t kdesc = smem_desc(smem_u32(sKV + 2 * r * kTileBytes), 16, 1024);
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk) {
-          const uint32_t off = (kk >> 2) * kHalfBytes + (kk & 3) * 32;
-          mma_ss_w(tmem + 256 * t, qdesc + (uint64_t)(off >> 4), kdesc + (uint64_t)(off >> 4), kIdS, kk > 0 ? 1u : 0u);
-        }
+        mma_tile_ss(tmem + 256 * t, q_lo + (SINGLE ? 0 : t) * kTileLo, k_lo + 2 * r * kTileLo, kIdS, 0);
         tc_commit_w(smem_u32(&bars->s_full[t]));
         if (!SINGLE && (info & (1 << (kLast + t)))) tc_commit_w(smem_u32(&bars->q_empty[t]));
-        (t == 0 ? pend0 : pend1) = ec;
-        (t == 0 ? pr0 : pr1) = r;
-        (t == 0 ? pf0 : pf1) = ((info >> (kFirst + t)) & 1) | (((info >> (kLast + t)) & 1) << 1);
-        ++(t == 0 ? ns0 : ns1);
+        (t == 0 ? pend0 : pend1) = r | (((info >> (kFirst + t)) & 1) << 4) | (((info >> (kLast + t)) & 1) << 5);
         return true;
       };
+      bool ok;
       while (true) {
         if (SINGLE) {
           if (ec & 1) ok = pend1 < 0 || issue_pv(T1{});
@@ -423,18 +387,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (info >> kZeroShift) {
           // rows [valid, 128) of V; a row is 128 bytes of either half tile
           uint4* v = reinterpret_cast<uint4*>(sKV + (2 * r + 1) * kTileBytes);
-          const int lo = (info >> kZeroShift) * 8;
-          for (int x = lo + lane; x < 1024; x += 32) v[x] = v[1024 + x] = make_uint4(0, 0, 0, 0);
+          for (int x = (info >> kZeroShift) * 8 + lane; x < 1024; x += 32) v[x] = v[1024 + x] = make_uint4(0, 0, 0, 0);
           fence_async_shared();
           __syncwarp();
         }
         if (SINGLE && (info & kSegFirst)) {
-          if (!iwait(&bars->q_full[0], nq0 & 1)) {
+          if (!iwait(&bars->q_full[0], ph >> 1)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          ++nq0;
+          ph ^= 2;
         }
         if (info & 1) ok = issue_s(T0{}, info);
         if (!SINGLE && ok && pend1 >= 0) ok = issue_pv(T1{});
@@ -449,57 +412,80 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (ok && pend0 >= 0) ok = issue_pv(T0{});
-      if (ok && pend1 >= 0) ok = issue_pv(T1{});
+      if (ok && pend1 >= 0) issue_pv(T1{});
       // aborted or not: MMAs retire in order, so this covers all of them
       tc_commit_w(smem_u32(&bars->done));
-    } else if (!dense) {
+    } else if (dense) {
+      // -------------------------------------------------- Q tiles (TMA)
+      if (warp == 3 && lane == 0) {
+        SegIter it(a.p);
+        Seg s{};
+        int qn0 = 0, qn1 = 0;
+        bool ok = true;
+        auto load = [&](int t, int& qn) {
+          if (!wait(&bars->q_empty[t], (qn & 1) ^ 1)) return false;
+          const uint32_t bar = smem_u32(&bars->q_full[t]), dst = smem_u32(sQ + t * kTileBytes);
+          mbar_expect_tx(bar, kTileBytes);
+          tma_load_4d(dst, &tm_q, bar, 0, s.row0 + 128 * t, s.h * a.q_h, s.b * a.q_b);
+          tma_load_4d(dst + kHalfBytes, &tm_q, bar, 64, s.row0 + 128 * t, s.h * a.q_h, s.b * a.q_b);
+          ++qn;
+          return true;
+        };
+        while (ok && it.next(a, bars->lens, s)) {
+          if (s.n == 0) continue;
+          ok = load(0, qn0) && (s.row0 + 128 >= s.row_end || load(1, qn1));
+        }
+        if (!ok) {
+          volatile int32_t zero = 0;
+          if (qn0) mbar_wait(smem_u32(&bars->q_full[0]), (qn0 - 1) & 1, &zero, nullptr);
+          if (qn1) mbar_wait(smem_u32(&bars->q_full[1]), (qn1 - 1) & 1, &zero, nullptr);
+        }
+      }
+    } else {
       // -------------------------------------------- gather of folded Q rows
       // 16 lanes take a row, 4 rows a pass of the 64 threads; rows past the
       // block are zero.  Swizzle: 16-byte chunk c of row r sits at c ^ (r & 7).
       const int g = threadIdx.x - 64, c = g & 15;
       SegIter it(a.p);
-      Seg s;
-      int qn[2] = {0, 0};
-      bool ok = true;
-      while (ok && it.next(a, s)) {
-        if (s.n == 0) continue;
+      Seg s{};
+      int qn0 = 0, qn1 = 0;
+      auto gather = [&](int t, int& qn) {
+        if (!wait(&bars->q_empty[t], (qn & 1) ^ 1)) return false;
+        ++qn;
+        uint8_t* dst = sQ + t * kTileBytes + (c >> 3) * kHalfBytes;
+        for (int r0 = g >> 4; r0 < 128; r0 += 16) {
+          uint4 v[4];
 #pragma unroll
-        for (int t = 0; t < L::kQTiles; ++t) {
-          if (!ok || (t && s.row0 + 128 >= s.row_end)) continue;
-          if (!wait(&bars->q_empty[t], (qn[t] & 1) ^ 1)) {
-            ok = false;
-            continue;
-          }
-          ++qn[t];
-          uint8_t* dst = sQ + t * kTileBytes + (c >> 3) * kHalfBytes;
-          for (int r0 = g >> 4; r0 < 128; r0 += 32) {
-            uint4 v[8];
-#pragma unroll
-            for (int x = 0; x < 8; ++x) {
-              const int row = s.row0 + 128 * t + r0 + 4 * x;
-              v[x] = make_uint4(0, 0, 0, 0);
-              if (row < s.row_end) {
-                const int tok = row / a.n.group, b = tok / a.n.q_len;
-                v[x] = *reinterpret_cast<const uint4*>(
-                    a.q.at(b, tok - b * a.n.q_len, s.hk * a.n.group + (row - tok * a.n.group)) + 8 * c);
-              }
-            }
-#pragma unroll
-            for (int x = 0; x < 8; ++x) {
-              const int r = r0 + 4 * x;
-              *reinterpret_cast<uint4*>(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[x];
+          for (int x = 0; x < 4; ++x) {
+            const int row = s.row0 + 128 * t + r0 + 4 * x;
+            v[x] = make_uint4(0, 0, 0, 0);
+            if (row < s.row_end) {
+              const int tok = a.p.by_group(row), b = a.p.by_q_len(tok);
+              v[x] = *reinterpret_cast<const uint4*>(
+                  a.q.at(b, tok - b * a.n.q_len, s.hk * a.n.group + (row - tok * a.n.group)) + 8 * c);
             }
           }
-          fence_async_shared();
-          mbar_arrive(smem_u32(&bars->q_full[t]));
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int r = r0 + 4 * x;
+            *reinterpret_cast<uint4*>(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[x];
+          }
         }
+        fence_async_shared();
+        mbar_arrive(smem_u32(&bars->q_full[t]));
+        return true;
+      };
+      while (it.next(a, bars->lens, s)) {
+        if (s.n == 0) continue;
+        if (!gather(0, qn0)) break;
+        if (!SINGLE && s.row0 + 128 < s.row_end && !gather(1, qn1)) break;
       }
     }
-  } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+  } else if (warp < 12) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     // one outcome a warp: the TMEM accesses need its lanes together
     auto wait_w = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
-    // ----------------------------------------------------- softmax + epilogue
+    // ---------------------------------------------------------------- softmax
     const int t = (warp - 4) >> 2, q = warp & 3;
     const int r = 32 * q + lane;  // row of the tile = TMEM lane
     const uint32_t lane_base = tmem + ((uint32_t)(32 * q) << 16);
@@ -507,15 +493,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float sl2 = a.scale_log2;
     const uint64_t sl2x2 = dup2(sl2);
     SegIter it(a.p);
-    Seg s;
-    int ec = 0, ns = 0, no = 0, no1 = 0, nml = 0;
+    Seg s{};
+    int ec = 0, ns = 0, nseg = 0;
     bool ok = true;
-    while (ok && it.next(a, s)) {
-      const int row = s.row0 + (SINGLE ? 0 : 128 * t) + r;
+    while (ok && it.next(a, bars->lens, s)) {
       const int i0 = SINGLE ? ((ec ^ t) & 1) : 0;
       const int step = SINGLE ? 2 : 1;
       const int nt = SINGLE ? (s.n - i0 + 1) / 2 : (s.row0 + 128 * t < s.row_end ? s.n : 0);
       ec += s.n;
+      if (nt == 0) continue;
       float m = -1e30f, l = 0.f;
       for (int x = 0; x < nt; ++x) {
         const int valid = SegIter::valid(a, s, s.j0 + i0 + x * step);
@@ -591,88 +577,149 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_before();
         mbar_arrive(smem_u32(&bars->p_full[t]));
       }
-      if (!ok) break;
-      // ---------------------------------------------------------- epilogue
-      bool has0 = nt > 0, has1 = false;  // this half's O; single mode: half 1's
-      float w0 = 1.f, w1 = 0.f;
-      if (SINGLE) {
-        if (t == 1) {
-          if (nt > 0) {
-            // half 0 has read the last segment's
-            if (nml > 0 && !wait_w(&bars->o_empty[1], (nml - 1) & 1)) break;
-            bars->ml[r] = make_float2(m, l);
-            ++nml;
-            mbar_arrive(smem_u32(&bars->ml_full));
-          }
-          continue;
-        }
-        has1 = s.n - nt > 0;
-        if (has1) {
-          if (!wait_w(&bars->ml_full, nml & 1)) break;
-          const float2 ml = bars->ml[r];
-          ++nml;
-          const float top = fmaxf(m, ml.x);
-          w0 = ex2(m - top);
-          w1 = ex2(ml.x - top);
-          m = top;
-          l = l * w0 + ml.y * w1;
-          if (!wait_w(&bars->o_full[1], no1 & 1)) break;
-          ++no1;
-        }
-      }
-      if (has0) {
-        if (!wait_w(&bars->o_full[t], no & 1)) break;
-        ++no;
-      }
+      // the epilogue has read the last segment's
+      if (!ok || (nseg > 0 && !wait_w(&bars->o_empty[t], (nseg - 1) & 1))) break;
+      bars->ml[t][r] = make_float2(m, l);
+      ++nseg;
+      mbar_arrive(smem_u32(&bars->ml_full[t]));
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    // --------------------------------------------------------------- epilogue
+    auto wait_w = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
+    const int q = warp & 3, r = 32 * q + lane;
+    const uint32_t tO = tmem + ((uint32_t)(32 * q) << 16) + 128;
+    uint8_t* stage = smem + 6 * kTileBytes + q * 8192;  // dense: two boxes of 32 rows x 64 columns
+    SegIter it(a.p);
+    Seg s{};
+    int ec = 0, n0 = 0, n1 = 0;  // segments of either half
+    // half t's (m, l) and O are there
+    auto arrived = [&](int t, int& n, float2& ml) {
+      if (!wait_w(&bars->ml_full[t], n & 1)) return false;
+      ml = bars->ml[t][r];
+      if (!wait_w(&bars->o_full[t], n & 1)) return false;
+      ++n;
+      return true;
+    };
+    // dense rows of tile t, whole: boxes of 32 rows x 64 columns by TMA
+    auto finish_box = [&](int t, bool has, float2 ml) {
       tc_fence_after();
+      const int row0 = s.row0 + 128 * t + 32 * q;
+      const float f = 1.0f / fmaxf(ml.y, 1e-30f);
+      if (a.lse && row0 + lane < s.row_end)
+        a.lse[((int64_t)s.b * a.n.heads + s.h) * a.n.q_len + row0 + lane] =
+            ml.y == 0.f ? -INFINITY : (ml.x + lg2(ml.y)) * 0.69314718055994531f;
+#pragma unroll 1
+      for (int p = 0; p < 2; ++p) {
+        uint8_t* box = stage + p * 4096;
+        if (lane == 0) tma_store_wait_read<1>();  // the box two stores ago has been read
+        __syncwarp();
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          // a load's latency is 200-400 cycles beside the other warps' TMEM
+          // traffic, so as many columns as the registers hold
+          uint32_t x[32];
+          if (has) {
+            H3_TMEM_LD16(tO + 256 * t + 64 * p + 32 * c, (&x[0]));
+            H3_TMEM_LD16(tO + 256 * t + 64 * p + 32 * c + 16, (&x[16]));
+            tmem_wait_ld();
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) x[e] = 0u;
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const auto two = [&](int k) {
+              return pack_bf16(__uint_as_float(x[8 * e + k]) * f, __uint_as_float(x[8 * e + k + 1]) * f);
+            };
+            *reinterpret_cast<uint4*>(box + lane * 128 + (((4 * c + e) ^ (lane & 7)) << 4)) =
+                make_uint4(two(0), two(2), two(4), two(6));
+          }
+        }
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0 && row0 < s.row_end)
+          tma_store_4d(&tm_o, smem_u32(box), 64 * p, row0, s.h * (a.out.h != 0), s.b * (a.out.b != 0));
+      }
+    };
+    // any other rows of tile t: O of half t (f0) and, where has1, of half 1
+    // (f1), to the output or to the partial results
+    auto finish_rows = [&](int t, bool has0, bool has1, float2 ml, float f0, float f1) {
+      tc_fence_after();
+      const int row = s.row0 + 128 * t + r;
       const bool live = row < s.row_end;
       int tok = row, b = s.b, h = s.h;
       if (!dense) {
-        const int bt = row / a.n.group;
-        b = bt / a.n.q_len;
+        const int bt = a.p.by_group(row);
+        b = a.p.by_q_len(bt);
         tok = bt - b * a.n.q_len;
         h = s.hk * a.n.group + (row - bt * a.n.group);
       }
-      const int64_t rid = dense ? ((int64_t)b * a.n.heads + h) * a.n.q_len + tok
-                                : (int64_t)s.hk * a.p.fold_rows + row;
-      const int64_t part = rid * a.p.slots + s.slot;
-      uint16_t* go = a.out.p + (live ? b * a.out.b + tok * a.out.t + h * a.out.h : 0);
+      const int64_t out_row = ((int64_t)b * a.n.heads + h) * a.n.q_len + tok;
+      const int64_t part = (dense ? out_row : (int64_t)s.hk * a.p.fold_rows + row) * a.p.slots + s.slot;
       if (s.direct) {
-        const float inv = 1.0f / fmaxf(l, 1e-30f);
-        w0 *= inv;
-        w1 *= inv;
-        if (live && a.lse)
-          a.lse[((int64_t)b * a.n.heads + h) * a.n.q_len + tok] =
-              l == 0.f ? -INFINITY : (m + lg2(l)) * 0.69314718055994531f;
+        const float inv = 1.0f / fmaxf(ml.y, 1e-30f);
+        f0 *= inv;
+        f1 *= inv;
+        if (live && a.lse) a.lse[out_row] = ml.y == 0.f ? -INFINITY : (ml.x + lg2(ml.y)) * 0.69314718055994531f;
       } else if (live) {
-        a.part_ml[part] = make_float2(m, l);
+        a.part_ml[part] = ml;
       }
-      if (has0 || has1 || s.direct) {
-#pragma unroll 2
-        for (int c = 0; c < 8; ++c) {
-          uint32_t o0[16], o1[16];
-          float o[16];
-          if (has0) H3_TMEM_LD16(tO + 16 * c, o0);
-          if (has1) H3_TMEM_LD16(tO + 256 + 16 * c, o1);
-          tmem_wait_ld();
+      if (!has0 && !has1 && !s.direct) return;
+      uint16_t* go = a.out.p + (live ? b * a.out.b + tok * a.out.t + h * a.out.h : 0);
+      float* po = a.part_o + part * 128;
+#pragma unroll 1
+      for (int c = 0; c < 128; c += 16) {
+        uint32_t x[16], y[16];
+        if (has0) H3_TMEM_LD16(tO + 256 * t + c, x);
+        if (has1) H3_TMEM_LD16(tO + 256 + c, y);
+        tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            o[e] = has0 ? __uint_as_float(o0[e]) * w0 : 0.f;
-            if (has1) o[e] += __uint_as_float(o1[e]) * w1;
-          }
-          if (live && s.direct) {
-            store_row32(go + 16 * c, o, 1.0f);
-          } else if (live) {
-            float4* po = reinterpret_cast<float4*>(a.part_o + part * 128 + 16 * c);
+        for (int e = 0; e < 16; ++e) {
+          float o = has0 ? __uint_as_float(x[e]) * f0 : 0.f;
+          if (has1) o = fmaf(__uint_as_float(y[e]), f1, o);
+          x[e] = __float_as_uint(o);
+        }
+        if (!live) continue;
+        if (s.direct) {
+          uint32_t k[8];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) po[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-          }
+          for (int e = 0; e < 8; ++e) k[e] = pack_bf16(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
+          store32(go + c, k);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            *reinterpret_cast<uint4*>(po + c + 4 * e) = make_uint4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
         }
       }
-      tc_fence_before();
-      if (has0) mbar_arrive(smem_u32(&bars->o_empty[t]));
-      if (has1) mbar_arrive(smem_u32(&bars->o_empty[1]));
+    };
+    while (it.next(a, bars->lens, s)) {
+      float2 ml0 = make_float2(-1e30f, 0.f);
+      if (SINGLE) {
+        float2 ml1 = ml0;
+        const bool has0 = s.n > (ec & 1), has1 = s.n > ((ec ^ 1) & 1);
+        ec += s.n;
+        if ((has0 && !arrived(0, n0, ml0)) || (has1 && !arrived(1, n1, ml1))) break;
+        const float top = fmaxf(ml0.x, ml1.x), f0 = ex2(ml0.x - top), f1 = ex2(ml1.x - top);
+        finish_rows(0, has0, has1, make_float2(top, ml0.y * f0 + ml1.y * f1), f0, f1);
+        tc_fence_before();
+        if (has0) mbar_arrive(smem_u32(&bars->o_empty[0]));
+        if (has1) mbar_arrive(smem_u32(&bars->o_empty[1]));
+      } else {
+#pragma unroll 1
+        for (int t = 0; t < 2; ++t) {
+          if (t && s.row0 + 128 >= s.row_end) continue;
+          if (s.n > 0 && !arrived(t, t ? n1 : n0, ml0)) goto out;
+          if (dense && s.direct) finish_box(t, s.n > 0, ml0);
+          else finish_rows(t, s.n > 0, false, ml0, 1.f, 0.f);
+          tc_fence_before();
+          if (s.n > 0) mbar_arrive(smem_u32(&bars->o_empty[t]));
+        }
+      }
     }
+  out:
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    __syncwarp();
   }
 
   // ------------------------------------------------------------------ exit
@@ -689,60 +736,79 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Joins the partial results of a row: o = sum 2^(m_s - M) o_s / sum 2^(m_s - M) l_s.
-// One warp a row, lane l holds channels 4l..4l+3.
-__global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ FwdArgs a) {
+// Joins n partial results of a row, the first n_p in slots 0.., the others in
+// slots slots_p..: o = sum 2^(m_s - M) o_s / sum 2^(m_s - M) l_s.  One warp a
+// row, lane l holds channels 4l..4l+3.
+__device__ __forceinline__ void join_row(const FwdArgs& a, int64_t rid, int n_p, int n, uint16_t* out, float* lse) {
+  const int lane = threadIdx.x & 31;
+  const float2* ml = a.part_ml + rid * a.p.slots;
+  float m = -1e30f;
+  for (int i = lane; i < n; i += 32) m = fmaxf(m, ml[i < n_p ? i : a.p.slots_p + i - n_p].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  float l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) {
+    const int slot = i < n_p ? i : a.p.slots_p + i - n_p;
+    const float2 e = ml[slot];
+    if (e.y == 0.f) continue;  // no keys: its o was not written
+    const float w = ex2(e.x - m);
+    const float4 v = *reinterpret_cast<const float4*>(a.part_o + (rid * a.p.slots + slot) * 128 + 4 * lane);
+    l += e.y * w;
+    acc.x = fmaf(v.x, w, acc.x);
+    acc.y = fmaf(v.y, w, acc.y);
+    acc.z = fmaf(v.z, w, acc.z);
+    acc.w = fmaf(v.w, w, acc.w);
+  }
+  const float inv = 1.0f / fmaxf(l, 1e-30f);
+  *reinterpret_cast<uint2*>(out + 4 * lane) =
+      make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+  if (lse && lane == 0) *lse = l == 0.f ? -INFINITY : (m + lg2(l)) * 0.69314718055994531f;
+}
+
+// Dense units: block (x, y) joins rows 32y..32y+31 of the unit that the start
+// of CTA x + 1's run cuts (if it is the first such start inside the unit).
+__global__ void __launch_bounds__(256) join_dense_kernel(const __grid_constant__ FwdArgs a) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const FwdPlan& p = a.p;
-  const int lane = threadIdx.x & 31;
-  const int64_t rows = (int64_t)a.n.batch * a.n.heads * a.n.q_len;
-  for (int64_t row = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5; row < rows;
-       row += ((int64_t)gridDim.x * blockDim.x) >> 5) {
-    const int tok = (int)(row % a.n.q_len);
-    const int64_t bh = row / a.n.q_len;
-    const int h = (int)(bh % a.n.heads), b = (int)(bh / a.n.heads), hk = h / a.n.group;
-    int64_t rid, start_o;      // partial row; first position of its own unit in the linear split
-    int np = 0, no = 0;        // partial results of either source
-    if (p.mode == kDense) {
-      rid = row;
-      start_o = (bh * p.per_o + tok / p.unit_rows) * p.tiles_o;
-    } else {
-      const int in_b = tok * a.n.group + (h - hk * a.n.group);
-      const int fr = b * a.n.q_len * a.n.group + in_b;
-      rid = (int64_t)hk * p.fold_rows + fr;
-      start_o = (int64_t)p.units_p * p.tiles_p +
-                (((int64_t)b * a.n.kv_heads + hk) * p.per_o + in_b / p.unit_rows) * p.tiles_o;
-      if (p.units_p) {
-        const int64_t start = ((int64_t)hk * p.per_p + fr / p.unit_rows) * p.tiles_p;
-        np = p.tpc ? (int)((start + p.tiles_p - 1) / p.tpc - start / p.tpc) + 1 : 1;
-      }
+  const uint32_t start = (blockIdx.x + 1) * p.tpc;
+  const int u = p.by_tiles_o(start), j0 = start - u * p.tiles_o;
+  if (u >= p.units_o || j0 == 0) return;
+  const uint32_t first = start - j0;
+  const int c0 = p.by_tpc(first);
+  if (c0 != (int)blockIdx.x) return;
+  const int n = p.by_tpc(first + p.tiles_o - 1) - c0 + 1;
+  const int bh = p.by_per_o(u), b = p.by_heads(bh), h = bh - b * a.n.heads;
+  const int t0 = (u - bh * p.per_o) * p.unit_rows + blockIdx.y * 32;
+  for (int t = t0 + (threadIdx.x >> 5); t < min(t0 + 32, a.n.q_len); t += 8) {
+    const int64_t row = (int64_t)bh * a.n.q_len + t;
+    join_row(a, row, 0, n, a.out.at(b, t, h), a.lse ? a.lse + row : nullptr);
+  }
+}
+
+// Folded rows, one warp a row.
+__global__ void __launch_bounds__(256) join_folded_kernel(const __grid_constant__ FwdArgs a) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const FwdPlan& p = a.p;
+  const int rows = a.n.kv_heads * p.fold_rows;  // below 2^31: checked at the call
+  for (int rid = (blockIdx.x * blockDim.x + threadIdx.x) >> 5; rid < rows; rid += (gridDim.x * blockDim.x) >> 5) {
+    const int hk = p.by_rows(rid), fr = rid - hk * p.fold_rows;
+    const int bt = p.by_group(fr), b = p.by_q_len(bt), tok = bt - b * a.n.q_len;
+    const int h = hk * a.n.group + (fr - bt * a.n.group);
+    auto runs = [&](uint32_t start, int tiles) {
+      return p.tpc ? (int)(p.by_tpc(start + tiles - 1) - p.by_tpc(start)) + 1 : 1;
+    };
+    int n_p = 0, n = 0;
+    if (p.units_p) n_p = n = runs((uint32_t)(hk * p.per_p + fr / p.unit_rows) * p.tiles_p, p.tiles_p);
+    if (p.units_o) {
+      const int in_b = fr - b * a.n.q_len * a.n.group;
+      n += runs((uint32_t)(p.units_p * p.tiles_p) +
+                    (uint32_t)((b * a.n.kv_heads + hk) * p.per_o + in_b / p.unit_rows) * p.tiles_o, p.tiles_o);
     }
-    if (p.units_o) no = p.tpc ? (int)((start_o + p.tiles_o - 1) / p.tpc - start_o / p.tpc) + 1 : 1;
-    if (np + no == 1) continue;  // written by its unit
-    const float2* ml = a.part_ml + rid * p.slots;
-    float m = -1e30f;
-    for (int i = lane; i < np + no; i += 32) m = fmaxf(m, ml[i < np ? i : p.slots_p + i - np].x);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    float l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int i = 0; i < np + no; ++i) {
-      const int slot = i < np ? i : p.slots_p + i - np;
-      const float2 e = ml[slot];
-      if (e.y == 0.f) continue;  // no keys: its o was not written
-      const float w = ex2(e.x - m);
-      const float4 v = *reinterpret_cast<const float4*>(a.part_o + (rid * p.slots + slot) * 128 + 4 * lane);
-      l += e.y * w;
-      acc.x = fmaf(v.x, w, acc.x);
-      acc.y = fmaf(v.y, w, acc.y);
-      acc.z = fmaf(v.z, w, acc.z);
-      acc.w = fmaf(v.w, w, acc.w);
-    }
-    const float inv = 1.0f / fmaxf(l, 1e-30f);
-    *reinterpret_cast<uint2*>(a.out.at(b, tok, h) + 4 * lane) =
-        make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
-    if (a.lse && lane == 0) a.lse[row] = l == 0.f ? -INFINITY : (m + lg2(l)) * 0.69314718055994531f;
+    if (n == 1) continue;  // written by its unit
+    const int64_t row = ((int64_t)b * a.n.heads + h) * a.n.q_len + tok;
+    join_row(a, rid, n_p, n, a.out.at(b, tok, h), a.lse ? a.lse + row : nullptr);
   }
 }
 
@@ -787,13 +853,17 @@ FwdPlan plan_fwd(const CrossShape& n) {
   // whole units in turn cost up to one unit more than the even share; the
   // linear split costs the partial results' traffic and the combine launch,
   // about the time of 4 tiles
-  if ((units + kSms - 1) / kSms * longest > share + share / 10 + 4) p.tpc = (int32_t)share;
+  if ((units + kSms - 1) / kSms * longest > share + share / 10 + 4 && total < INT_MAX) p.tpc = (int32_t)share;
   p.ctas = (int32_t)(p.tpc ? (total + p.tpc - 1) / p.tpc : (units < kSms ? units : kSms));
   p.slots_p = p.units_p ? (p.tpc ? (p.tiles_p - 1) / p.tpc + 2 : 1) : 0;
   p.slots = p.slots_p + (p.units_o ? (p.tpc ? (p.tiles_o - 1) / p.tpc + 2 : 1) : 0);
   p.combine = (p.units_p && p.units_o) || (p.tpc && p.tpc % (int32_t)longest != 0);
   p.part_rows = p.combine ? (p.mode == kDense ? (int64_t)n.batch * n.heads * n.q_len : (int64_t)n.kv_heads * p.fold_rows)
                           : 0;
+  auto div = [](int64_t d) { return make_div((uint32_t)(d > 0 ? d : 1)); };
+  p.by_per_p = div(p.per_p), p.by_per_o = div(p.per_o), p.by_tiles_p = div(p.tiles_p), p.by_tiles_o = div(p.tiles_o);
+  p.by_heads = div(n.heads), p.by_kv_heads = div(n.kv_heads), p.by_group = div(n.group), p.by_q_len = div(n.q_len);
+  p.by_rows = div(p.fold_rows), p.by_tpc = div(p.tpc);
   return p;
 }
 
@@ -808,14 +878,14 @@ cudaError_t launch_fwd(const FwdArgs& a, const CUtensorMap* m, cudaStream_t s) {
   std::call_once(once[dev], [dev] {
     cudaError_t e =
         cudaFuncSetAttribute(cross_fwd_kernel<SINGLE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<SINGLE>());
-    // the register split needs exactly 168 a thread at launch
+    // the register split needs exactly 128 a thread at launch
     cudaFuncAttributes fa;
     if (e == cudaSuccess) e = cudaFuncGetAttributes(&fa, cross_fwd_kernel<SINGLE>);
-    if (e == cudaSuccess && fa.numRegs != 168) e = cudaErrorInvalidConfiguration;
+    if (e == cudaSuccess && fa.numRegs != 128) e = cudaErrorInvalidConfiguration;
     set_result[dev] = e;
   });
   if (set_result[dev] != cudaSuccess) return set_result[dev];
-  cross_fwd_kernel<SINGLE><<<a.p.ctas, kThreads, smem_bytes<SINGLE>(), s>>>(m[0], m[1], m[2], m[3], m[4], a);
+  cross_fwd_kernel<SINGLE><<<a.p.ctas, kThreads, smem_bytes<SINGLE>(), s>>>(m[0], m[1], m[2], m[3], m[4], m[5], a);
   return cudaGetLastError();
 }
 
@@ -852,9 +922,11 @@ cudaError_t launch_cross_fwd(const CrossLaunch& L, cudaStream_t s, std::string* 
   a.k_b = L.k.b != 0, a.k_h = L.k.h != 0;
   a.v_b = L.v.b != 0, a.v_h = L.v.h != 0;
   a.pk_h = L.pk.h != 0, a.pv_h = L.pv.h != 0;
-  CUtensorMap m[5] = {};
+  CUtensorMap m[6] = {};
   const CrossShape& n = L.n;
-  if (a.p.mode == kDense && !make_map4(&m[0], L.q, n.q_len, n.heads, n.batch, err)) return cudaErrorInvalidValue;
+  if (a.p.mode == kDense && (!make_map4(&m[0], L.q, n.q_len, n.heads, n.batch, err) ||
+                             !make_map4(&m[5], L.out, n.q_len, n.heads, n.batch, err, 32)))
+    return cudaErrorInvalidValue;
   if (n.kv_len && (!make_map4(&m[1], L.k, n.kv_len, n.kv_heads, n.batch, err) ||
                    !make_map4(&m[2], L.v, n.kv_len, n.kv_heads, n.batch, err)))
     return cudaErrorInvalidValue;
@@ -865,7 +937,7 @@ cudaError_t launch_cross_fwd(const CrossLaunch& L, cudaStream_t s, std::string* 
   if (e != cudaSuccess || !a.p.combine) return e;
   // placed while the attention kernel runs; waits for its end before it reads
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(warps_grid(rows));
+  cfg.gridDim = a.p.mode == kDense ? dim3(a.p.ctas - 1, a.p.unit_rows / 32) : dim3(warps_grid(rows));
   cfg.blockDim = dim3(256);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -873,7 +945,7 @@ cudaError_t launch_cross_fwd(const CrossLaunch& L, cudaStream_t s, std::string* 
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, combine_kernel, a);
+  return cudaLaunchKernelEx(&cfg, a.p.mode == kDense ? join_dense_kernel : join_folded_kernel, a);
 }
 
 }  // namespace h3

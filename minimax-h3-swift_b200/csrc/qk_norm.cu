@@ -16,18 +16,6 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kGroups = kThreads / 8;   // rows a CTA has in hand at a time
 
-// n / d for n < 2^31, d >= 1: m = ceil(2^(31 + s) / d) with 2^s >= d
-struct Div {
-  uint32_t m, s;
-  __device__ uint32_t operator()(uint32_t n) const { return (uint32_t)(((uint64_t)n * m) >> (31 + s)); }
-};
-
-Div make_div(uint32_t d) {
-  uint32_t s = 0;
-  while ((1ull << s) < d) ++s;
-  return {(uint32_t)(((1ull << (31 + s)) + d - 1) / d), s};
-}
-
 struct Operand {
   QkNormOperand o;
   Div heads, tokens;

@@ -186,6 +186,225 @@ constexpr uint32_t idesc_bf16(bool b_mn_major) {
          ((128u >> 4) << 24);
 }
 
+// The low word of a shared-memory matrix descriptor; the high word (128-byte
+// swizzle, version 1, 1024 bytes between groups of eight rows) is the same for
+// every tile here: 0x40004040.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lbo) {
+  return ((addr >> 4) & 0x3FFF) | ((lbo >> 4) << 16);
+}
+
+// Products of 128 x 128 x 128 as one group, one lane elected for all of it and
+// the descriptors stepped in 32 bits: a lean issuer, since one that spills to
+// local memory (shared memory leaves next to no L1) reads it back from L2
+// between products.
+// D (+)= A B^T, both tiles K-major in shared memory (desc_lo(tile, 16)).
+__device__ __forceinline__ void mma_tile_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, t, e;\n\t.reg .b32 ra, rb;\n\t.reg .b64 da, db;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.eq.u32 t, 0, 0;\n\t"
+      "add.u32 ra, %1, 0;\n\t"
+      "add.u32 rb, %2, 0;\n\t"
+      "mov.b64 da, {ra, 0x40004040};\n\t"
+      "mov.b64 db, {rb, 0x40004040};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t"
+      "add.u32 ra, %1, 2;\n\t"
+      "add.u32 rb, %2, 2;\n\t"
+      "mov.b64 da, {ra, 0x40004040};\n\t"
+      "mov.b64 db, {rb, 0x40004040};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, t;\n\t"
+      "add.u32 ra, %1, 4;\n\t"
+      "add.u32 rb, %2, 4;\n\t"
+      "mov.b64 da, {ra, 0x40004040};\n\t"
+      "mov.b64 db, {rb, 0x40004040};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, t;\n\t"
+      "add.u32 ra, %1, 6;\n\t"
+      "add.u32 rb, %2, 6;\n\t"
+      "mov.b64 da, {ra, 0x40004040};\n\t"
+      "mov.b64 db, {rb, 0x40004040};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, t;\n\t"
+      "add.u32 ra, %1, 1024;\n\t"
+      "add.u32 rb, %2, 1024;\n\t"
+      "mov.b64 da, {ra, 0x40004040};\n\t"
+      "mov.b64 db, {rb, 0x40004040};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, t;\n\t"
+      "add.u32 ra, %1, 1026;\n\t"
+      "add.u32 rb, %2, 1026;\n\t"
+      "mov.b64 da, {ra, 0x40004040};\n\t"
+      "mov.b64 db, {rb, 0x40004040};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, t;\n\t"
+      "add.u32 ra, %1, 1028;\n\t"
+      "add.u32 rb, %2, 1028;\n\t"
+      "mov.b64 da, {ra, 0x40004040};\n\t"
+      "mov.b64 db, {rb, 0x40004040};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, t;\n\t"
+      "add.u32 ra, %1, 1030;\n\t"
+      "add.u32 rb, %2, 1030;\n\t"
+      "mov.b64 da, {ra, 0x40004040};\n\t"
+      "mov.b64 db, {rb, 0x40004040};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, t;\n\t"
+      "}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
+// D (+)= A B, A packed bf16 at 64 TMEM columns, B a tile with the summed axis
+// along its rows (desc_lo(tile, kHalfBytes)).
+__device__ __forceinline__ void mma_tile_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, t, e;\n\t.reg .b32 ra, rb;\n\t.reg .b64 db;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.eq.u32 t, 0, 0;\n\t"
+      "add.u32 ra, %1, 0;\n\t"
+      "add.u32 rb, %2, 0;\n\t"
+      "mov.b64 db, {rb, 0x40004040};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [ra], db, %3, p;\n\t"
+      "add.u32 ra, %1, 8;\n\t"
+      "add.u32 rb, %2, 128;\n\t"
+      "mov.b64 db, {rb, 0x40004040};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [ra], db, %3, t;\n\t"
+      "add.u32 ra, %1, 16;\n\t"
+      "add.u32 rb, %2, 256;\n\t"
+      "mov.b64 db, {rb, 0x40004040};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [ra], db, %3, t;\n\t"
+      "add.u32 ra, %1, 24;\n\t"
+      "add.u32 rb, %2, 384;\n\t"
+      "mov.b64 db, {rb, 0x40004040};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [ra], db, %3, t;\n\t"
+      "add.u32 ra, %1, 32;\n\t"
+      "add.u32 rb, %2, 512;\n\t"
+      "mov.b64 db, {rb, 0x40004040};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [ra], db, %3, t;\n\t"
+      "add.u32 ra, %1, 40;\n\t"
+      "add.u32 rb, %2, 640;\n\t"
+      "mov.b64 db, {rb, 0x40004040};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [ra], db, %3, t;\n\t"
+      "add.u32 ra, %1, 48;\n\t"
+      "add.u32 rb, %2, 768;\n\t"
+      "mov.b64 db, {rb, 0x40004040};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [ra], db, %3, t;\n\t"
+      "add.u32 ra, %1, 56;\n\t"
+      "add.u32 rb, %2, 896;\n\t"
+      "mov.b64 db, {rb, 0x40004040};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [ra], db, %3, t;\n\t"
+      "}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
+// Steps 0-5 and 6-7 of mma_tile_ts (a and b as for all of it).
+__device__ __forceinline__ void mma_tile_ts_0_6(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, t, e;\n\t.reg .b32 ra, rb;\n\t.reg .b64 db;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.eq.u32 t, 0, 0;\n\t"
+      "add.u32 ra, %1, 0;\n\t"
+      "add.u32 rb, %2, 0;\n\t"
+      "mov.b64 db, {rb, 0x40004040};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [ra], db, %3, p;\n\t"
+      "add.u32 ra, %1, 8;\n\t"
+      "add.u32 rb, %2, 128;\n\t"
+      "mov.b64 db, {rb, 0x40004040};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [ra], db, %3, t;\n\t"
+      "add.u32 ra, %1, 16;\n\t"
+      "add.u32 rb, %2, 256;\n\t"
+      "mov.b64 db, {rb, 0x40004040};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [ra], db, %3, t;\n\t"
+      "add.u32 ra, %1, 24;\n\t"
+      "add.u32 rb, %2, 384;\n\t"
+      "mov.b64 db, {rb, 0x40004040};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [ra], db, %3, t;\n\t"
+      "add.u32 ra, %1, 32;\n\t"
+      "add.u32 rb, %2, 512;\n\t"
+      "mov.b64 db, {rb, 0x40004040};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [ra], db, %3, t;\n\t"
+      "add.u32 ra, %1, 40;\n\t"
+      "add.u32 rb, %2, 640;\n\t"
+      "mov.b64 db, {rb, 0x40004040};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [ra], db, %3, t;\n\t"
+      "}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
+__device__ __forceinline__ void mma_tile_ts_6_8(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, t, e;\n\t.reg .b32 ra, rb;\n\t.reg .b64 db;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.eq.u32 t, 0, 0;\n\t"
+      "add.u32 ra, %1, 48;\n\t"
+      "add.u32 rb, %2, 768;\n\t"
+      "mov.b64 db, {rb, 0x40004040};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [ra], db, %3, p;\n\t"
+      "add.u32 ra, %1, 56;\n\t"
+      "add.u32 rb, %2, 896;\n\t"
+      "mov.b64 db, {rb, 0x40004040};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [ra], db, %3, t;\n\t"
+      "}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
+// Steps 0-3 and 4-7, for an A in two places (b as for all of it; a of the
+// second is that of step 4).
+__device__ __forceinline__ void mma_tile_ts_0_4(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, t, e;\n\t.reg .b32 ra, rb;\n\t.reg .b64 db;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.eq.u32 t, 0, 0;\n\t"
+      "add.u32 ra, %1, 0;\n\t"
+      "add.u32 rb, %2, 0;\n\t"
+      "mov.b64 db, {rb, 0x40004040};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [ra], db, %3, p;\n\t"
+      "add.u32 ra, %1, 8;\n\t"
+      "add.u32 rb, %2, 128;\n\t"
+      "mov.b64 db, {rb, 0x40004040};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [ra], db, %3, t;\n\t"
+      "add.u32 ra, %1, 16;\n\t"
+      "add.u32 rb, %2, 256;\n\t"
+      "mov.b64 db, {rb, 0x40004040};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [ra], db, %3, t;\n\t"
+      "add.u32 ra, %1, 24;\n\t"
+      "add.u32 rb, %2, 384;\n\t"
+      "mov.b64 db, {rb, 0x40004040};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [ra], db, %3, t;\n\t"
+      "}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
+__device__ __forceinline__ void mma_tile_ts_4_8(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, t, e;\n\t.reg .b32 ra, rb;\n\t.reg .b64 db;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.eq.u32 t, 0, 0;\n\t"
+      "add.u32 ra, %1, 0;\n\t"
+      "add.u32 rb, %2, 512;\n\t"
+      "mov.b64 db, {rb, 0x40004040};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [ra], db, %3, p;\n\t"
+      "add.u32 ra, %1, 8;\n\t"
+      "add.u32 rb, %2, 640;\n\t"
+      "mov.b64 db, {rb, 0x40004040};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [ra], db, %3, t;\n\t"
+      "add.u32 ra, %1, 16;\n\t"
+      "add.u32 rb, %2, 768;\n\t"
+      "mov.b64 db, {rb, 0x40004040};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [ra], db, %3, t;\n\t"
+      "add.u32 ra, %1, 24;\n\t"
+      "add.u32 rb, %2, 896;\n\t"
+      "mov.b64 db, {rb, 0x40004040};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [ra], db, %3, t;\n\t"
+      "}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
 // Four-dimensional form: coordinates (d, token, head, batch).
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2,
                                             int c3) {
@@ -194,6 +413,33 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       "[%2];" ::"r"(dst),
       "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
       : "memory");
+}
+
+// 4D tiled TMA store from shared memory (this thread's bulk group), and the
+// wait until at most N of the thread's groups still read shared memory.
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2, int c3) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(map),
+               "r"(src), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void tma_store_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+
+// 32 bytes to global memory, a whole sector in one store; p needs 16-byte
+// alignment only (rows are no further aligned), so it is two stores where p is
+// not on a sector.
+__device__ __forceinline__ void store32(uint16_t* p, const uint32_t* w) {
+  if (!((uintptr_t)p & 31)) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                 "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+  } else {
+    reinterpret_cast<uint4*>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    reinterpret_cast<uint4*>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  }
 }
 
 // Orders this thread's shared-memory writes before later reads by TMA or MMA.
