@@ -222,7 +222,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(smem_u32(&bars->ml_full[t]), 128);
     }
     for (int r = 0; r < 3; ++r) {
-      mbar_init(smem_u32(&bars->kv_full[r]), 1);
+      // dense: the K/V producer, and of a segment's first entry the Q loader
+      // (one wait of the issuer for all of it; of others the producer again)
+      mbar_init(smem_u32(&bars->kv_full[r]), dense ? 2 : 1);
       mbar_init(smem_u32(&bars->k_empty[r]), 1);
       mbar_init(smem_u32(&bars->v_empty[r]), 1);
     }
@@ -283,6 +285,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             const uint32_t bar = smem_u32(&bars->kv_full[r]);
             bars->info[ec & 15] = info;
+            if (!SINGLE && dense && i > 0) mbar_arrive(bar);
             mbar_expect_tx(bar, 2 * kTileBytes);
             const uint32_t dk = smem_u32(sKV + 2 * r * kTileBytes), dv = dk + kTileBytes;
             if (pre) {
@@ -308,11 +311,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (ok && wait(&bars->k_empty[r], ph ^ 1) && wait(&bars->v_empty[r], ph ^ 1)) {
           bars->info[ec & 15] = kEnd;
           mbar_arrive(smem_u32(&bars->kv_full[r]));
+          if (!SINGLE && dense) mbar_arrive(smem_u32(&bars->kv_full[r]));
         } else {
-          // abort: every load in flight lands before anyone may exit
+          // abort: every load in flight lands before anyone may exit (an entry
+          // that the Q loader did not join never completes: a short limit)
           volatile int32_t zero = 0;
-          for (int e = max(0, issued - L::kRing); e < issued; ++e)
-            mbar_wait(smem_u32(&bars->kv_full[e % L::kRing]), (e / L::kRing) & 1, &zero, nullptr);
+          for (int e = max(0, issued - L::kRing); e < issued; ++e, zero = 0)
+            mbar_wait(smem_u32(&bars->kv_full[e % L::kRing]), (e / L::kRing) & 1, &zero, nullptr, 10000000);
         }
       }
     } else if (warp == 1) {
@@ -325,8 +330,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) got = wait(bar, par & 1) ? 1 : 0;
         return __shfl_sync(0xffffffff, got, 0) != 0;
       };
-      // phase bits: 0 K/V ring, 1 + t Q, 3 + t P, 5 + t O
-      uint32_t ph = 0x60;
+      // phase bits: 0 K/V ring, 1 + t Q, 3 + t P
+      uint32_t ph = 0;
       // entry whose PV is due: ring slot, its first / last flags as bits 4, 5; or -1
       int pend0 = -1, pend1 = -1;
       const uint32_t q_lo = desc_lo(smem_u32(sQ), 16), k_lo = desc_lo(smem_u32(sKV), 16);
@@ -339,10 +344,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         constexpr int t = decltype(tile)::value;
         int& pend = t == 0 ? pend0 : pend1;
         const int slot = pend & 15, other = t == 0 ? pend1 : pend0;
-        if (pend & 16) {  // the epilogue of the half's last segment has read O
-          if (!iwait(&bars->o_empty[t], ph >> (5 + t))) return false;
-          ph ^= 1u << (5 + t);
-        }
         if (!iwait(&bars->p_half[t], ph >> (3 + t))) return false;
         tc_fence_after();
         const uint32_t b = v_lo + 2 * slot * kTileLo;
@@ -358,7 +359,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       auto issue_s = [&](auto tile, int info) -> bool {
         constexpr int t = decltype(tile)::value;
-        if (!SINGLE && (info & (1 << (kFirst + t)))) {
+        if (!SINGLE && !dense && (info & (1 << (kFirst + t)))) {
           if (!iwait(&bars->q_full[t], ph >> (1 + t))) return false;
           tc_fence_after();
           ph ^= 1u << (1 + t);
@@ -418,27 +419,29 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (dense) {
       // -------------------------------------------------- Q tiles (TMA)
       if (warp == 3 && lane == 0) {
+        // A segment's Q tiles complete its first entry's barrier.  That the
+        // last segment's S has read Q (q_empty) says that every barrier of
+        // its entries has completed, so this arrival falls in the right phase.
         SegIter it(a.p);
         Seg s{};
-        int qn0 = 0, qn1 = 0;
-        bool ok = true;
-        auto load = [&](int t, int& qn) {
-          if (!wait(&bars->q_empty[t], (qn & 1) ^ 1)) return false;
-          const uint32_t bar = smem_u32(&bars->q_full[t]), dst = smem_u32(sQ + t * kTileBytes);
-          mbar_expect_tx(bar, kTileBytes);
-          tma_load_4d(dst, &tm_q, bar, 0, s.row0 + 128 * t, s.h * a.q_h, s.b * a.q_b);
-          tma_load_4d(dst + kHalfBytes, &tm_q, bar, 64, s.row0 + 128 * t, s.h * a.q_h, s.b * a.q_b);
-          ++qn;
-          return true;
-        };
-        while (ok && it.next(a, bars->lens, s)) {
+        int qn0 = 0, qn1 = 0, ec = 0;
+        while (it.next(a, bars->lens, s)) {
           if (s.n == 0) continue;
-          ok = load(0, qn0) && (s.row0 + 128 >= s.row_end || load(1, qn1));
-        }
-        if (!ok) {
-          volatile int32_t zero = 0;
-          if (qn0) mbar_wait(smem_u32(&bars->q_full[0]), (qn0 - 1) & 1, &zero, nullptr);
-          if (qn1) mbar_wait(smem_u32(&bars->q_full[1]), (qn1 - 1) & 1, &zero, nullptr);
+          const bool act1 = s.row0 + 128 < s.row_end;
+          const uint32_t bar = smem_u32(&bars->kv_full[ec % L::kRing]);
+          auto load = [&](int t) {
+            const uint32_t dst = smem_u32(sQ + t * kTileBytes);
+            tma_load_4d(dst, &tm_q, bar, 0, s.row0 + 128 * t, s.h * a.q_h, s.b * a.q_b);
+            tma_load_4d(dst + kHalfBytes, &tm_q, bar, 64, s.row0 + 128 * t, s.h * a.q_h, s.b * a.q_b);
+          };
+          if (!wait(&bars->q_empty[0], (qn0++ & 1) ^ 1)) break;
+          mbar_expect_tx(bar, act1 ? 2 * kTileBytes : kTileBytes);
+          load(0);
+          if (act1) {
+            if (!wait(&bars->q_empty[1], (qn1++ & 1) ^ 1)) break;
+            load(1);
+          }
+          ec += s.n;
         }
       }
     } else {
@@ -503,7 +506,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       ec += s.n;
       if (nt == 0) continue;
       float m = -1e30f, l = 0.f;
-      for (int x = 0; x < nt; ++x) {
+      for (int x = 0; ok && x < nt; ++x) {
         const int valid = SegIter::valid(a, s, s.j0 + i0 + x * step);
         if (!wait_w(&bars->s_full[t], ns & 1)) {
           ok = false;
@@ -567,6 +570,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           H3_TMEM_ST16(tS + 16 * c, pk);
           if (c == 2) {  // keys 0-95 of P are in TMEM: the first six PV steps may start
+            // (once the epilogue has read O and (m, l) of the last segment: waited
+            // for here, not by the issuer, whose waits delay both halves)
+            if (x == 0 && nseg > 0) ok = wait_w(&bars->o_empty[t], (nseg - 1) & 1);
             tmem_wait_st();
             tc_fence_before();
             mbar_arrive(smem_u32(&bars->p_half[t]));
@@ -577,8 +583,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_before();
         mbar_arrive(smem_u32(&bars->p_full[t]));
       }
-      // the epilogue has read the last segment's
-      if (!ok || (nseg > 0 && !wait_w(&bars->o_empty[t], (nseg - 1) & 1))) break;
+      if (!ok) break;
       bars->ml[t][r] = make_float2(m, l);
       ++nseg;
       mbar_arrive(smem_u32(&bars->ml_full[t]));
