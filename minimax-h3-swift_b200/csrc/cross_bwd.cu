@@ -3,15 +3,14 @@
 //   P = 2^(scale log2(e) q.k - lse2);  delta_i = do_i.o_i;  dS = P (do v^T - delta)
 //   dq = scale dS k;  dk = scale dS^T q;  dv = P^T do   (sums over the heads of a group)
 //
-// Two passes, so that every sum has one owner and a fixed order (no atomics):
+// delta_kernel goes over do and out once; then two passes, so that every sum
+// has one owner and a fixed order (no atomics):
 //   dq_kernel    a CTA holds 128 queries and walks the keys: S, dP, dq += dS K
 //   dkv_kernel   a CTA holds 128 keys and walks the queries of all heads of
 //                the group: S^T, dP^T, dv += P^T do, dk += dS^T Q
 // Seven products of 128x128x128 a tile pair instead of the five that a single
 // pass with atomics on dq would make.  P and dS enter their products in bf16
-// from TMEM (they never touch shared memory); sums are fp32.  dq_kernel also
-// writes delta and -lse2 for dkv_kernel, padded to whole blocks of queries
-// (-inf there, so that P is 0).
+// from TMEM (they never touch shared memory); sums are fp32.
 //
 // Roles of a CTA's 12 warps: 0 TMA producer, 1 MMA issuer, 2 TMEM owner (and
 // a second issuer in dq_kernel), 4-7 and 8-11 elementwise: each warpgroup takes 64 of a tile's 128 columns of
@@ -121,20 +120,75 @@ __device__ __forceinline__ void release_tmem(int warp, uint32_t tmem, volatile i
   }
 }
 
+// ------------------------------------------------------------------ delta
+__device__ __forceinline__ float dot8(const uint4& x, const uint4& y) {
+  const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    s = fmaf(__uint_as_float(xw[i] << 16), __uint_as_float(yw[i] << 16), s);
+    s = fmaf(__uint_as_float(xw[i] & 0xffff0000u), __uint_as_float(yw[i] & 0xffff0000u), s);
+  }
+  return s;
+}
+
+// delta = do.out and -lse log2(e) of every row, padded to whole blocks of
+// queries (0 and -inf there, so that P is 0).  HBM-bound: 512 bytes a row.
+// 16 lanes take a row; a CTA has 16 tokens of kHeads heads, a group its
+// token's heads one after the other (neighbours in memory), all in flight.
+constexpr int kHeads = 8;
+
+__global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ BwdArgs a) {
+  const int c = threadIdx.x & 15, tok = blockIdx.x * 16 + (threadIdx.x >> 4);
+  const bool live = tok < a.n.q_len;
+  const int per_b = (a.n.heads + kHeads - 1) / kHeads;
+  for (int y = blockIdx.y; y < per_b * a.n.batch; y += gridDim.y) {
+    const int b = y / per_b, h0 = (y - b * per_b) * kHeads;
+    uint4 o[kHeads], g[kHeads];
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+      o[i] = g[i] = make_uint4(0, 0, 0, 0);
+      if (live && h0 + i < a.n.heads) {
+        o[i] = __ldcs(reinterpret_cast<const uint4*>(a.out.at(b, tok, h0 + i)) + c);
+        g[i] = *(reinterpret_cast<const uint4*>(a.dout.at(b, tok, h0 + i)) + c);
+      }
+    }
+    const int64_t bh = (int64_t)b * a.n.heads + h0 + c;  // lane c < kHeads: its head's
+    const bool mine = c < kHeads && h0 + c < a.n.heads;
+    const float lse = mine && live ? a.lse[bh * a.n.q_len + tok] : INFINITY;
+    float delta = 0.f;
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+      float v = dot8(o[i], g[i]);
+#pragma unroll
+      for (int m = 8; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+      if (c == i) delta = v;
+    }
+    if (mine) {
+      const int64_t pad = bh * a.q_blocks * 128 + tok;
+      a.nl2[pad] = lse * -kLog2e;
+      a.delta[pad] = delta;
+    }
+  }
+}
+
 // --------------------------------------------------------------------- dq
 // Shared memory: q and do of the unit, three K and two V tiles (224 KB).
 // TMEM columns: dq 0, S 128, dP 256, dS (two buffers) 384 and 448.  Of block
 // e+1, S and dP run while block e is in the elementwise warps; dq of e
 // follows, so a K tile is held for two blocks and needs the third buffer to
-// be loaded ahead.  delta comes from do in shared memory and out rows that the
-// elementwise warps fetch into registers a unit ahead.  Global rows are read
-// and written eight lanes a row (128 bytes of it): a thread a row, 32 lines an
-// instruction, kept the load/store unit busy for 4,000 cycles a unit each way.
+// be loaded ahead.  Four more warps (12-15) write dq, eight lanes a row (a
+// thread a row, 32 lines an instruction, kept the load/store unit busy for
+// 4,000 cycles a unit), so that the elementwise warps only go from block to
+// block.  Working delta out in here, by either kind of warp, took 5,000 to
+// 12,000 cycles a unit of three to eight blocks of 2,200: code that runs once
+// a unit waits for its instructions, constants and rows each time.
 struct __align__(16) DqBarriers {
-  float red[2][128];                 // halves of delta
+  float nl2[2][128], delta[2][128];  // by unit parity
   uint64_t q_full, q_empty, g_full, g_empty;
   uint64_t k_full[3], k_empty[3], v_full[2], v_empty[2];
-  uint64_t s_full, s_empty, dp_full, dp_empty, dq_full, dq_empty, red_full, done;
+  uint64_t n_full[2];                // -lse2 and delta of unit u on [u & 1]
+  uint64_t s_full, s_empty, dp_full, dp_empty, dq_full, dq_empty, done;
   // block e on [e & 1]: S and dP of e + 1 are issued before the issuer waits
   // for dS of e, so one barrier could complete twice before that wait
   uint64_t ds_full[2];
@@ -143,6 +197,7 @@ struct __align__(16) DqBarriers {
   int32_t info[8];
   int32_t lens[kLens];
 };
+constexpr int kDqThreads = 512;
 constexpr int kDqTiles = 7 * kTileBytes;
 constexpr int kDqSmem = kDqTiles + (int)sizeof(DqBarriers);
 static_assert(kDqSmem <= 227 * 1024, "shared memory");
@@ -180,18 +235,7 @@ __device__ __forceinline__ void transpose8(uint4 (&v)[8]) {
   }
 }
 
-__device__ __forceinline__ float dot8(const uint4& x, const uint4& y) {
-  const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
-  float s = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    s = fmaf(__uint_as_float(xw[i] << 16), __uint_as_float(yw[i] << 16), s);
-    s = fmaf(__uint_as_float(xw[i] & 0xffff0000u), __uint_as_float(yw[i] & 0xffff0000u), s);
-  }
-  return s;
-}
-
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kDqThreads, 1)
     dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
               const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_g,
               const __grid_constant__ BwdArgs a, int units) {
@@ -210,18 +254,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(smem_u32(&bars->v_full[i]), 1);
       mbar_init(smem_u32(&bars->v_empty[i]), 1);
       mbar_init(smem_u32(&bars->ds_full[i]), 256);
+      mbar_init(smem_u32(&bars->n_full[i]), 1);
     }
     mbar_init(smem_u32(&bars->q_full), 1);
     mbar_init(smem_u32(&bars->q_empty), 1);
     mbar_init(smem_u32(&bars->g_full), 1);
-    mbar_init(smem_u32(&bars->g_empty), 257);  // the unit's last product and 256 readers of do
-    mbar_init(smem_u32(&bars->red_full), 256);
+    mbar_init(smem_u32(&bars->g_empty), 1);
     mbar_init(smem_u32(&bars->s_full), 1);
     mbar_init(smem_u32(&bars->s_empty), 256);
     mbar_init(smem_u32(&bars->dp_full), 1);
     mbar_init(smem_u32(&bars->dp_empty), 256);
     mbar_init(smem_u32(&bars->dq_full), 1);
-    mbar_init(smem_u32(&bars->dq_empty), 256);
+    mbar_init(smem_u32(&bars->dq_empty), 128);
     mbar_init(smem_u32(&bars->done), 2);
     bars->abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -232,19 +276,35 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     return mbar_wait(smem_u32(bar), parity, abort_flag, a.status, a.wait_limit_ns);
   };
-  // Register split of the launch's 384 x 168: 128 x 72 + 256 x 216.
+  // Register split of the launch's 512 x 128: 128 x 48 + 256 x 192 + 128 x 80.
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
     if (warp == 0 && lane == 0) {
-      // a K tile, then what is needed next, so that no load waits behind one
-      // whose buffer frees later
+      // in the order in which the buffers free.  q and do have one each, so
+      // what is not hidden of their latency is paid every unit: those of the
+      // next unit are brought into L2 meanwhile (4,000 cycles from HBM under
+      // load, 1,200 from there).
       int e = 0, qn = 0, nv = 0, ng = 0;  // K tiles, q tiles, V tiles, do tiles loaded
       int kr = 0;
       uint32_t kp = 0;
       bool ok = true;
       for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
         const DqUnit x(a, bars->lens, u);
+        if (x.n == 0) continue;
         const int hk = a.by_group(x.h);
+        if (!(ok = wait(&bars->q_empty, (qn & 1) ^ 1))) break;
+        uint32_t bar = smem_u32(&bars->q_full);
+        mbar_expect_tx(bar, kTileBytes);
+        tma_tile(smem_u32(sQ), &tm_q, bar, x.t0, x.h * a.q_h, x.b * a.q_b);
+        ++qn;
+        if (u + (int)gridDim.x < units) {
+          const DqUnit y(a, bars->lens, u + gridDim.x);
+#pragma unroll
+          for (int c = 0; c < 128; c += 64) {
+            tma_prefetch_4d(&tm_q, c, y.t0, y.h * a.q_h, y.b * a.q_b);
+            tma_prefetch_4d(&tm_g, c, y.t0, y.h * a.g_h, y.b * a.g_b);
+          }
+        }
         for (int j = 0; j < x.n; ++j) {
           if (!(ok = wait(&bars->k_empty[kr], kp ^ 1))) break;
           const int valid = x.len - 128 * j;
@@ -252,7 +312,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           // there: the issuer clears them (0 x NaN would reach dq)
           bars->info[e & 7] = (j == 0 ? kFirst : 0) | (j == x.n - 1 ? kLast : 0) |
                               (valid < 128 && x.len < a.n.kv_len ? valid << kZeroShift : 0);
-          uint32_t bar = smem_u32(&bars->k_full[kr]);
+          bar = smem_u32(&bars->k_full[kr]);
           mbar_expect_tx(bar, kTileBytes);
           tma_tile(smem_u32(sK + kr * kTileBytes), &tm_k, bar, 128 * j, hk * a.k_h, x.b * a.k_b);
           ++e;
@@ -260,23 +320,23 @@ __global__ void __launch_bounds__(kThreads, 1)
             kr = 0;
             kp ^= 1;
           }
-          if (j == 0) {
-            if (!(ok = wait(&bars->q_empty, (qn & 1) ^ 1))) break;
-            bar = smem_u32(&bars->q_full);
-            mbar_expect_tx(bar, kTileBytes);
-            tma_tile(smem_u32(sQ), &tm_q, bar, x.t0, x.h * a.q_h, x.b * a.q_b);
-            ++qn;
-          }
           if (!(ok = wait(&bars->v_empty[nv & 1], ((nv >> 1) & 1) ^ 1))) break;
           bar = smem_u32(&bars->v_full[nv & 1]);
           mbar_expect_tx(bar, kTileBytes);
           tma_tile(smem_u32(sV + (nv & 1) * kTileBytes), &tm_v, bar, 128 * j, hk * a.v_h, x.b * a.v_b);
           ++nv;
           if (j == 0) {
+            // (g_empty: dP of the last unit, whose last block follows on the
+            // elementwise warps' reading -lse2 and delta of the unit before)
             if (!(ok = wait(&bars->g_empty, (ng & 1) ^ 1))) break;
             bar = smem_u32(&bars->g_full);
             mbar_expect_tx(bar, kTileBytes);
             tma_tile(smem_u32(sG), &tm_g, bar, x.t0, x.h * a.g_h, x.b * a.g_b);
+            bar = smem_u32(&bars->n_full[ng & 1]);
+            mbar_expect_tx(bar, 1024);
+            const int64_t pad = ((int64_t)x.b * a.n.heads + x.h) * a.q_blocks * 128 + x.t0;
+            bulk_512(smem_u32(bars->nl2[ng & 1]), a.nl2 + pad, bar);
+            bulk_512(smem_u32(bars->delta[ng & 1]), a.delta + pad, bar);
             ++ng;
           }
         }
@@ -293,6 +353,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           mbar_wait(smem_u32(&bars->v_full[x & 1]), (x >> 1) & 1, &zero, nullptr);
         if (qn) mbar_wait(smem_u32(&bars->q_full), (qn - 1) & 1, &zero, nullptr);
         if (ng) mbar_wait(smem_u32(&bars->g_full), (ng - 1) & 1, &zero, nullptr);
+        for (int x = max(0, ng - 2); x < ng; ++x)
+          mbar_wait(smem_u32(&bars->n_full[x & 1]), (x >> 1) & 1, &zero, nullptr);
       }
     } else if (warp == 1 || warp == 2) {
       // Two issuers, one of S and one of dP and dq, so that the waits of one
@@ -371,53 +433,21 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       tc_commit_w(smem_u32(&bars->done));
     }
-  } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+  } else if (warp < 12) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     // one outcome a warp: the TMEM accesses need its lanes together
     auto wait_w = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
     const int w = (warp - 4) >> 2, q = warp & 3, r = 32 * q + lane;
     const uint32_t lane_base = tmem + ((uint32_t)(32 * q) << 16);
     const uint64_t sl2 = dup2(a.scale * kLog2e);
-    // the next unit with keys: 16 bytes of rows 4i + lane / 8 of this warp's
-    // half rows of out, and this thread's row's lse
-    uint4 o[8];
-    float lse = INFINITY;  // rows past the end: P = 0
-    auto fetch = [&](int u) {
-      while (u < units) {
-        const DqUnit x(a, bars->lens, u);
-        if (x.n) {
-          const int tok = x.t0 + r, t1 = x.t0 + 32 * q + (lane >> 3);
-          lse = INFINITY;
-          if (tok < a.n.q_len) lse = a.lse[((int64_t)x.b * a.n.heads + x.h) * a.n.q_len + tok];
-          const uint16_t* po = a.out.at(x.b, t1, x.h) + 64 * w + 8 * (lane & 7);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            o[i] = make_uint4(0, 0, 0, 0);
-            if (t1 + 4 * i < a.n.q_len) o[i] = *reinterpret_cast<const uint4*>(po + (int64_t)4 * i * a.out.t);
-          }
-          return;
-        }
-        u += gridDim.x;
-      }
-    };
-    fetch(blockIdx.x);
     int e = 0, un = 0;
     bool ok = true;
     for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
       const DqUnit x(a, bars->lens, u);
-      const int tok = x.t0 + r;
-      // rows 8 (lane / 8) + i of this warp's 32, 16 bytes a lane
-      const int t1 = x.t0 + 32 * q + 8 * (lane >> 3);
-      uint16_t* go = a.dq.at(x.b, t1, x.h) + 64 * w + 8 * (lane & 7);
-      if (x.n == 0) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (t1 + i < a.n.q_len) *reinterpret_cast<uint4*>(go + i * a.dq.t) = make_uint4(0, 0, 0, 0);
-        continue;
-      }
-      const float nl2 = lse * -kLog2e;  // here, not in fetch, which must not wait for its loads
-      const uint64_t nl2x2 = dup2(nl2);
-      uint64_t ndelta = 0;
+      if (x.n == 0) continue;
+      if (!(ok = wait_w(&bars->n_full[un & 1], (un >> 1) & 1))) break;
+      const uint64_t nl2x2 = dup2(bars->nl2[un & 1][r]), ndelta = dup2(-bars->delta[un & 1][r]);
+      ++un;
       for (int j = 0; j < x.n; ++j, ++e) {
         if (!(ok = wait_w(&bars->s_full, e & 1))) break;
         tc_fence_after();
@@ -431,33 +461,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint64_t v = fma_2(pair2(s[2 * c], s[2 * c + 1]), sl2, nl2x2);
           p[2 * c] = ex2(lo2(v));
           p[2 * c + 1] = ex2(hi2(v));
-        }
-        if (j == 0) {
-          // delta: this warpgroup's 64 channels, then both halves
-          if (!(ok = wait_w(&bars->g_full, un & 1))) break;
-          // (every reader of the last unit's halves arrived on ds_full before
-          // this thread saw that unit's dq_full)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int row = 32 * q + 4 * i + (lane >> 3);
-            float v = dot8(*reinterpret_cast<const uint4*>(sG + w * kHalfBytes + row * 128 +
-                                                           (((lane & 7) ^ (row & 7)) << 4)), o[i]);
-            v += __shfl_xor_sync(0xffffffffu, v, 4);
-            v += __shfl_xor_sync(0xffffffffu, v, 2);
-            v += __shfl_xor_sync(0xffffffffu, v, 1);
-            if ((lane & 7) == 0) bars->red[w][row] = v;
-          }
-          mbar_arrive(smem_u32(&bars->g_empty));
-          mbar_arrive(smem_u32(&bars->red_full));
-          if (!(ok = wait_w(&bars->red_full, un & 1))) break;
-          const float delta = bars->red[0][r] + bars->red[1][r];
-          ndelta = dup2(-delta);
-          if (w == 0) {
-            const int64_t pad = ((int64_t)x.b * a.n.heads + x.h) * a.q_blocks * 128 + tok;
-            a.nl2[pad] = nl2;
-            a.delta[pad] = delta;
-          }
-          fetch(u + gridDim.x);
         }
         if (!(ok = wait_w(&bars->dp_full, e & 1))) break;
         tc_fence_after();
@@ -484,25 +487,50 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_before();
         mbar_arrive(smem_u32(&bars->ds_full[e & 1]));
       }
-      if (!ok || !wait_w(&bars->dq_full, un & 1)) break;
-      ++un;
-      tc_fence_after();
-      uint32_t v[64];
-      load64(lane_base + 64 * w, v);
-      tc_fence_before();
-      mbar_arrive(smem_u32(&bars->dq_empty));
-      uint4 k[8];
-#pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        const auto two = [&](int i) {
-          return pack_bf16(__uint_as_float(v[8 * c + i]) * a.scale, __uint_as_float(v[8 * c + i + 1]) * a.scale);
-        };
-        k[c] = make_uint4(two(0), two(2), two(4), two(6));
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    auto wait_w = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
+    const int q = warp & 3;
+    int un = 0;
+    for (int u = blockIdx.x; u < units; u += gridDim.x) {
+      const DqUnit x(a, bars->lens, u);
+      // rows 8 (lane / 8) + i of this warp's 32, 16 bytes of each half row a lane
+      const int t1 = x.t0 + 32 * q + 8 * (lane >> 3);
+      uint16_t* go = a.dq.at(x.b, t1, x.h) + 8 * (lane & 7);
+      if (x.n > 0) {
+        if (!wait_w(&bars->dq_full, un & 1)) break;
+        ++un;
+        tc_fence_after();
       }
-      transpose8(k);
+#pragma unroll 1
+      for (int w = 0; w < 2; ++w) {
+        uint4 k[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (t1 + i < a.n.q_len) *reinterpret_cast<uint4*>(go + i * a.dq.t) = k[i];
+        for (int c = 0; c < 4; ++c) {
+          uint32_t v[16];
+          if (x.n > 0) {
+            H3_TMEM_LD16(tmem + ((uint32_t)(32 * q) << 16) + 64 * w + 16 * c, v);
+            tmem_wait_ld();
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = 0u;
+          }
+          const auto two = [&](int i) {
+            return pack_bf16(__uint_as_float(v[i]) * a.scale, __uint_as_float(v[i + 1]) * a.scale);
+          };
+          k[2 * c] = make_uint4(two(0), two(2), two(4), two(6));
+          k[2 * c + 1] = make_uint4(two(8), two(10), two(12), two(14));
+        }
+        if (w == 1 && x.n > 0) {
+          tc_fence_before();
+          mbar_arrive(smem_u32(&bars->dq_empty));
+        }
+        transpose8(k);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (t1 + i < a.n.q_len) *reinterpret_cast<uint4*>(go + 64 * w + i * a.dq.t) = k[i];
+      }
     }
   }
   release_tmem(warp, tmem, abort_flag, &bars->done);
@@ -873,10 +901,10 @@ int dkv_ctas(const CrossShape& n) {
   return (int)(all < kSms ? all : kSms);
 }
 
-// Attributes of a kernel, set once a device; the register split needs exactly
-// 168 registers a thread at launch.
+// Attributes of a kernel, set once a device; its register split needs exactly
+// `regs` registers a thread at launch.
 template <typename K>
-cudaError_t prepare(K* kernel, int smem, std::once_flag* once, cudaError_t* result) {
+cudaError_t prepare(K* kernel, int smem, int regs, std::once_flag* once, cudaError_t* result) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
@@ -885,7 +913,7 @@ cudaError_t prepare(K* kernel, int smem, std::once_flag* once, cudaError_t* resu
     cudaError_t r = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     cudaFuncAttributes fa;
     if (r == cudaSuccess) r = cudaFuncGetAttributes(&fa, kernel);
-    if (r == cudaSuccess && fa.numRegs != 168) r = cudaErrorInvalidConfiguration;
+    if (r == cudaSuccess && fa.numRegs != regs) r = cudaErrorInvalidConfiguration;
     result[dev] = r;
   });
   return result[dev];
@@ -932,12 +960,14 @@ cudaError_t launch_cross_bwd(const CrossLaunch& L, cudaStream_t s, std::string* 
     return cudaErrorInvalidValue;
   static std::once_flag once_q[64], once_kv[64];
   static cudaError_t res_q[64], res_kv[64];
-  cudaError_t e = prepare(dq_kernel, kDqSmem, once_q, res_q);
-  if (e == cudaSuccess) e = prepare(dkv_kernel, kDkvSmem, once_kv, res_kv);
+  cudaError_t e = prepare(dq_kernel, kDqSmem, 128, once_q, res_q);
+  if (e == cudaSuccess) e = prepare(dkv_kernel, kDkvSmem, 168, once_kv, res_kv);
   if (e != cudaSuccess) return e;
   const int units = n.batch * n.heads * a.q_blocks;
-  dq_kernel<<<units < kSms ? units : kSms, kThreads, kDqSmem, s>>>(mq, mk, mv, mg, a, units);
   const int ctas = n.kv_len ? dkv_ctas(n) : 0;
+  const int groups = (n.heads + kHeads - 1) / kHeads * n.batch;
+  if (ctas) delta_kernel<<<dim3(a.q_blocks * 8, groups < 65535 ? groups : 65535), 256, 0, s>>>(a);
+  dq_kernel<<<units < kSms ? units : kSms, kDqThreads, kDqSmem, s>>>(mq, mk, mv, mg, a, units);
   if (ctas) dkv_kernel<<<ctas, kThreads, kDkvSmem, s>>>(mq, mk, mv, mg, a);
   if (ctas > 1) dkv_join_kernel<<<dim3(ctas - 1, 8), 256, 0, s>>>(a, ctas);
   return cudaGetLastError();

@@ -422,10 +422,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         // A segment's Q tiles complete its first entry's barrier.  That the
         // last segment's S has read Q (q_empty) says that every barrier of
         // its entries has completed, so this arrival falls in the right phase.
+        // The segment after it goes to L2 meanwhile: one buffer covers L2's
+        // latency, not HBM's.
         SegIter it(a.p);
-        Seg s{};
+        Seg s{}, following{};
         int qn0 = 0, qn1 = 0, ec = 0;
-        while (it.next(a, bars->lens, s)) {
+        bool more = it.next(a, bars->lens, following);
+        while (more) {
+          s = following;
+          more = it.next(a, bars->lens, following);
+          if (more && following.n > 0 && following.j0 == 0)
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              if (c < 2 || following.row0 + 128 < following.row_end)
+                tma_prefetch_4d(&tm_q, 64 * (c & 1), following.row0 + 64 * (c & 2), following.h * a.q_h,
+                                following.b * a.q_b);
           if (s.n == 0) continue;
           const bool act1 = s.row0 + 128 < s.row_end;
           const uint32_t bar = smem_u32(&bars->kv_full[ec % L::kRing]);

@@ -442,6 +442,13 @@ __device__ __forceinline__ void store32(uint16_t* p, const uint32_t* w) {
   }
 }
 
+// Brings a 4D box into L2.
+__device__ __forceinline__ void tma_prefetch_4d(const CUtensorMap* map, int c0, int c1, int c2, int c3) {
+  asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];" ::"l"(map), "r"(c0), "r"(c1),
+               "r"(c2), "r"(c3)
+               : "memory");
+}
+
 // Orders this thread's shared-memory writes before later reads by TMA or MMA.
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
