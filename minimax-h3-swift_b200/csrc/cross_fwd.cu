@@ -16,17 +16,17 @@
 //           the prefix's and then the member's own
 //   folded  q_len < 128: a row is (member, token, head of the group), so one
 //           K/V tile serves all query heads of its key head and, for the
-//           prefix, the whole batch; rows are gathered by two warps.  The
+//           prefix, the whole batch; rows are gathered.  The
 //           prefix and each member's own keys are units of their own.
 //           More than 128 rows: two row tiles share each K/V tile (dual).
 //           Up to 128: the two halves of the CTA take alternate K/V tiles of
 //           the same rows (single) and their results are joined through TMEM;
 //           one half alone would reach 5.3 of the 6.5 TB/s that HBM gives.
 //
-// Roles of a CTA's 16 warps: 0 K/V producer (TMA); 1 MMA issuer; 2-3 query
-// rows (folded: gather; dense: one thread of 3 by TMA), 2 also owns TMEM; 4-7
-// and 8-11 softmax of half 0 and 1, thread = row = TMEM lane; 12-15 epilogue
-// of both halves.  TMEM: half t has S (then P, packed bf16, over its first 64
+// Roles of a CTA's 16 warps: 0 K/V producer (TMA); 1 MMA issuer; 2 owns TMEM;
+// 3 query tiles of dense rows (TMA); 4-7 and 8-11 softmax of half 0 and 1,
+// thread = row = TMEM lane; 12-15 epilogue of both halves and, for folded
+// rows, the gather of the next queries.  TMEM: half t has S (then P, packed bf16, over its first 64
 // columns) at 256t and O at 256t + 128.  K/V entries run through a ring of 2
 // (3 in single mode, where each entry is needed for two steps); the producer
 // hands each entry's flags to the issuer through shared memory.  The next
@@ -47,31 +47,38 @@ constexpr int kSms = 148;
 
 enum { kDense = 0, kSingle = 1, kDual = 2 };
 
-struct FwdPlan {
-  int32_t mode;
-  int32_t np, nb;             // key tiles of the prefix and of kv_len
-  int32_t per_p, per_o;       // row blocks of a key head (prefix), of a member's (key) head (own)
-  int32_t units_p, units_o;   // units of the prefix (folded only) and the others
-  int32_t tiles_p, tiles_o;   // key tiles of such a unit
-  int32_t unit_rows;          // rows of a block: 128 or 256
-  int32_t fold_rows;          // folded: rows of a key head over the batch
+// The units of one source of keys: the prefix (folded rows only), or the
+// members' own keys (dense rows: the prefix's and their own).
+struct Source {
+  int32_t per;                // row blocks of a key head (prefix), of a member's (key) head (own)
+  int32_t units;
+  int32_t tiles;              // key tiles of a unit
+  int32_t rows;               // rows of a block: 128 or 256
   int32_t tpc;                // key tiles a CTA in the linear split; 0: whole units in turn
-  int32_t ctas;
-  int32_t slots_p, slots;     // partial results a row, at most: from the prefix's units, in all
-  int32_t combine;
-  int64_t part_rows;
-  Div by_per_p, by_per_o, by_tiles_p, by_tiles_o, by_heads, by_kv_heads, by_group, by_q_len, by_rows, by_tpc;
+  int32_t start;              // first position of its units in that split
+  // partial results: slots of a unit at most, rows of a slot; o as
+  // [units, slots, 32, stride] groups of four channels, ml as [units, slots,
+  // stride], so that a warp's 32 rows are contiguous
+  int32_t slots, stride;
+  Div by_per, by_tiles, by_tpc;
 };
 
 struct FwdArgs {
   CrossShape n;
-  FwdPlan p;
+  Source src[2];              // prefix, own
+  int32_t units_p, units_o;   // units of either
+  int32_t tpc;
+  int32_t mode;
+  int32_t np;                 // key tiles of the prefix
+  int32_t fold_rows;          // folded: rows of a key head over the batch
+  int32_t two_sources;        // every row has results of both
+  Div by_heads, by_kv_heads, by_group, by_q_len;
   Rows q, out;
   const int32_t* kv_lens;
   float* lse;
   float scale_log2;
-  float* part_o;              // [part_rows, slots, 128]
-  float2* part_ml;            // [part_rows, slots]
+  float4* part_o[2];
+  float2* part_ml[2];
   int32_t* status;
   uint64_t wait_limit_ns;
   // 1 where an operand's tensor map has the axis, 0 where it is broadcast
@@ -80,6 +87,7 @@ struct FwdArgs {
 
 // One run of key tiles of one unit.
 struct Seg {
+  int own, unit;              // source and unit of it
   int b, hk, h;               // h: dense only
   int row0, row_end;          // tokens (dense) or folded rows
   int npre, len;              // tiles of the unit that are the prefix's; valid own keys
@@ -90,70 +98,69 @@ struct Seg {
 
 struct SegIter {
   uint32_t pos, end;          // key tiles of the linear split, or units
-  __device__ explicit SegIter(const FwdPlan& p) {
-    if (p.tpc) {
-      const uint32_t total = (uint32_t)(p.units_p * p.tiles_p + p.units_o * p.tiles_o);
-      pos = blockIdx.x * p.tpc;
-      end = min(total, pos + p.tpc);
+  __device__ explicit SegIter(const FwdArgs& a) {
+    if (a.tpc) {
+      const uint32_t total = (uint32_t)(a.units_p * a.src[0].tiles + a.units_o * a.src[1].tiles);
+      pos = blockIdx.x * a.tpc;
+      end = min(total, pos + a.tpc);
     } else {
       pos = blockIdx.x;
-      end = p.units_p + p.units_o;
+      end = a.units_p + a.units_o;
     }
   }
   __device__ bool next(const FwdArgs& a, const int32_t* lens, Seg& s) {
     if (pos >= end) return false;
-    const FwdPlan& p = a.p;
-    int u, j1, tiles;
+    int j1, tiles;
     s.slot = 0;
-    if (p.tpc) {
-      const uint32_t pre = p.units_p * p.tiles_p;
-      const bool own = pos >= pre;
-      const uint32_t off = own ? pos - pre : pos;
-      tiles = own ? p.tiles_o : p.tiles_p;
-      const int v = own ? p.by_tiles_o(off) : p.by_tiles_p(off);
-      u = own ? p.units_p + v : v;
-      s.j0 = (int)off - v * tiles;
+    if (a.tpc) {
+      const uint32_t pre = a.units_p * a.src[0].tiles;
+      s.own = pos >= pre;
+      const uint32_t off = s.own ? pos - pre : pos;
+      tiles = a.src[s.own].tiles;
+      s.unit = a.src[s.own].by_tiles(off);
+      s.j0 = (int)off - s.unit * tiles;
       j1 = min(tiles, s.j0 + (int)(end - pos));
-      s.slot = blockIdx.x - p.by_tpc(pos - s.j0);
+      s.slot = blockIdx.x - a.src[s.own].by_tpc(pos - s.j0);
       pos += j1 - s.j0;
     } else {
-      u = pos;
-      tiles = u < p.units_p ? p.tiles_p : p.tiles_o;
+      s.own = (int)pos >= a.units_p;
+      s.unit = (int)pos - (s.own ? a.units_p : 0);
+      tiles = a.src[s.own].tiles;
       s.j0 = 0;
       j1 = tiles;
       pos += gridDim.x;
     }
+    const Source& c = a.src[s.own];
+    const int x = c.by_per(s.unit), rt = s.unit - x * c.per;
     int limit;
-    if (u < p.units_p) {
-      s.hk = p.by_per_p(u);
-      s.row0 = (u - s.hk * p.per_p) * p.unit_rows;
-      s.row_end = min(p.fold_rows, s.row0 + p.unit_rows);
+    if (!s.own) {
+      s.hk = x;
+      s.row0 = rt * c.rows;
+      s.row_end = min(a.fold_rows, s.row0 + c.rows);
       s.b = 0;
       s.len = 0;
-      s.npre = limit = p.np;
+      s.npre = limit = a.np;
     } else {
-      const int v = u - p.units_p, x = p.by_per_o(v), rt = v - x * p.per_o;
-      if (p.mode == kDense) {
-        s.b = p.by_heads(x);
+      if (a.mode == kDense) {
+        s.b = a.by_heads(x);
         s.h = x - s.b * a.n.heads;
-        s.hk = p.by_group(s.h);
-        s.row0 = rt * p.unit_rows;
-        s.row_end = min(a.n.q_len, s.row0 + p.unit_rows);
-        s.npre = p.np;
+        s.hk = a.by_group(s.h);
+        s.row0 = rt * c.rows;
+        s.row_end = min(a.n.q_len, s.row0 + c.rows);
+        s.npre = a.np;
       } else {
-        s.b = p.by_kv_heads(x);
+        s.b = a.by_kv_heads(x);
         s.hk = x - s.b * a.n.kv_heads;
         const int rows = a.n.q_len * a.n.group;
-        s.row0 = s.b * rows + rt * p.unit_rows;
-        s.row_end = min((s.b + 1) * rows, s.row0 + p.unit_rows);
+        s.row0 = s.b * rows + rt * c.rows;
+        s.row_end = min((s.b + 1) * rows, s.row0 + c.rows);
         s.npre = 0;
-        s.slot += p.slots_p;
       }
       s.len = s.b < kLens ? lens[s.b] : kv_len_of(a.kv_lens, a.n.kv_len, s.b);
       limit = s.npre + ((s.len + 127) >> 7);
     }
     s.n = max(0, min(j1, limit) - s.j0);
-    s.direct = s.j0 == 0 && j1 == tiles && (p.units_p == 0 || p.units_o == 0);
+    s.direct = s.j0 == 0 && j1 == tiles && !a.two_sources;
     return true;
   }
   // valid keys of tile j of the segment's unit
@@ -208,11 +215,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   Barriers* bars = (Barriers*)(smem + L::kTiles);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int32_t* abort_flag = &bars->abort;
-  const bool dense = a.p.mode == kDense;
+  const bool dense = a.mode == kDense;
 
   if (threadIdx.x == 0) {
     for (int t = 0; t < 2; ++t) {
-      mbar_init(smem_u32(&bars->q_full[t]), dense ? 1 : 64);
+      mbar_init(smem_u32(&bars->q_full[t]), 128);  // folded only
       mbar_init(smem_u32(&bars->q_empty[t]), 1);
       mbar_init(smem_u32(&bars->s_full[t]), 1);
       mbar_init(smem_u32(&bars->p_half[t]), 128);
@@ -254,7 +261,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 0) {
       // ------------------------------------------------------- TMA producer
       if (lane == 0) {
-        SegIter it(a.p);
+        SegIter it(a);
         Seg s{};
         int ec = 0, r = 0, issued = 0;
         uint32_t ph = 0;
@@ -424,7 +431,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // its entries has completed, so this arrival falls in the right phase.
         // The segment after it goes to L2 meanwhile: one buffer covers L2's
         // latency, not HBM's.
-        SegIter it(a.p);
+        SegIter it(a);
         Seg s{}, following{};
         int qn0 = 0, qn1 = 0, ec = 0;
         bool more = it.next(a, bars->lens, following);
@@ -455,45 +462,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           ec += s.n;
         }
       }
-    } else {
-      // -------------------------------------------- gather of folded Q rows
-      // 16 lanes take a row, 4 rows a pass of the 64 threads; rows past the
-      // block are zero.  Swizzle: 16-byte chunk c of row r sits at c ^ (r & 7).
-      const int g = threadIdx.x - 64, c = g & 15;
-      SegIter it(a.p);
-      Seg s{};
-      int qn0 = 0, qn1 = 0;
-      auto gather = [&](int t, int& qn) {
-        if (!wait(&bars->q_empty[t], (qn & 1) ^ 1)) return false;
-        ++qn;
-        uint8_t* dst = sQ + t * kTileBytes + (c >> 3) * kHalfBytes;
-        for (int r0 = g >> 4; r0 < 128; r0 += 16) {
-          uint4 v[4];
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int row = s.row0 + 128 * t + r0 + 4 * x;
-            v[x] = make_uint4(0, 0, 0, 0);
-            if (row < s.row_end) {
-              const int tok = a.p.by_group(row), b = a.p.by_q_len(tok);
-              v[x] = *reinterpret_cast<const uint4*>(
-                  a.q.at(b, tok - b * a.n.q_len, s.hk * a.n.group + (row - tok * a.n.group)) + 8 * c);
-            }
-          }
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int r = r0 + 4 * x;
-            *reinterpret_cast<uint4*>(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[x];
-          }
-        }
-        fence_async_shared();
-        mbar_arrive(smem_u32(&bars->q_full[t]));
-        return true;
-      };
-      while (it.next(a, bars->lens, s)) {
-        if (s.n == 0) continue;
-        if (!gather(0, qn0)) break;
-        if (!SINGLE && s.row0 + 128 < s.row_end && !gather(1, qn1)) break;
-      }
     }
   } else if (warp < 12) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
@@ -506,7 +474,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tS = lane_base + 256 * t, tO = tS + 128;
     const float sl2 = a.scale_log2;
     const uint64_t sl2x2 = dup2(sl2);
-    SegIter it(a.p);
+    SegIter it(a);
     Seg s{};
     int ec = 0, ns = 0, nseg = 0;
     bool ok = true;
@@ -606,7 +574,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int q = warp & 3, r = 32 * q + lane;
     const uint32_t tO = tmem + ((uint32_t)(32 * q) << 16) + 128;
     uint8_t* stage = smem + 6 * kTileBytes + q * 8192;  // dense: two boxes of 32 rows x 64 columns
-    SegIter it(a.p);
+    SegIter it(a);
     Seg s{};
     int ec = 0, n0 = 0, n1 = 0;  // segments of either half
     // half t's (m, l) and O are there
@@ -666,24 +634,25 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool live = row < s.row_end;
       int tok = row, b = s.b, h = s.h;
       if (!dense) {
-        const int bt = a.p.by_group(row);
-        b = a.p.by_q_len(bt);
+        const int bt = a.by_group(row);
+        b = a.by_q_len(bt);
         tok = bt - b * a.n.q_len;
         h = s.hk * a.n.group + (row - bt * a.n.group);
       }
       const int64_t out_row = ((int64_t)b * a.n.heads + h) * a.n.q_len + tok;
-      const int64_t part = (dense ? out_row : (int64_t)s.hk * a.p.fold_rows + row) * a.p.slots + s.slot;
+      const Source& c1 = a.src[s.own];
+      const int64_t part = (int64_t)s.unit * c1.slots + s.slot;
       if (s.direct) {
         const float inv = 1.0f / fmaxf(ml.y, 1e-30f);
         f0 *= inv;
         f1 *= inv;
         if (live && a.lse) a.lse[out_row] = ml.y == 0.f ? -INFINITY : (ml.x + lg2(ml.y)) * 0.69314718055994531f;
       } else if (live) {
-        a.part_ml[part] = ml;
+        a.part_ml[s.own][part * c1.stride + 128 * t + r] = ml;
       }
       if (!has0 && !has1 && !s.direct) return;
       uint16_t* go = a.out.p + (live ? b * a.out.b + tok * a.out.t + h * a.out.h : 0);
-      float* po = a.part_o + part * 128;
+      float4* po = a.part_o[s.own] + part * 32 * c1.stride + 128 * t + r;
 #pragma unroll 1
       for (int c = 0; c < 128; c += 16) {
         uint32_t x[16], y[16];
@@ -705,11 +674,54 @@ __global__ void __launch_bounds__(kThreads, 1)
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            *reinterpret_cast<uint4*>(po + c + 4 * e) = make_uint4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+            po[(c / 4 + e) * c1.stride] = make_float4(__uint_as_float(x[4 * e]), __uint_as_float(x[4 * e + 1]),
+                                                      __uint_as_float(x[4 * e + 2]), __uint_as_float(x[4 * e + 3]));
         }
       }
     };
+    // Folded: the next segment's Q rows, once the last S has read this one's.
+    // 16 lanes take a row, 8 rows a pass of the 128 threads, 8 passes in
+    // flight; rows past the block are zero.  Swizzle: 16-byte chunk c of row r
+    // sits at c ^ (r & 7).
+    auto gather = [&](const Seg& g, int t, int& qn) {
+      if (!wait_w(&bars->q_empty[t], (qn & 1) ^ 1)) return false;
+      ++qn;
+      const int c = lane & 15;
+      uint8_t* dst = sQ + t * kTileBytes + (c >> 3) * kHalfBytes;
+#pragma unroll 1
+      for (int r0 = 2 * q + (lane >> 4); r0 < 128; r0 += 64) {
+        uint4 v[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const int row = g.row0 + 128 * t + r0 + 8 * x;
+          v[x] = make_uint4(0, 0, 0, 0);
+          if (row < g.row_end) {
+            const int tok = a.by_group(row), b = a.by_q_len(tok);
+            v[x] = *reinterpret_cast<const uint4*>(
+                a.q.at(b, tok - b * a.n.q_len, g.hk * a.n.group + (row - tok * a.n.group)) + 8 * c);
+          }
+        }
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const int r = r0 + 8 * x;
+          *reinterpret_cast<uint4*>(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[x];
+        }
+      }
+      fence_async_shared();
+      mbar_arrive(smem_u32(&bars->q_full[t]));
+      return true;
+    };
+    int qn0 = 0, qn1 = 0;
+    auto gather_next = [&](SegIter ahead) {
+      Seg g{};
+      while (ahead.next(a, bars->lens, g))
+        if (g.n > 0)
+          return gather(g, 0, qn0) && (SINGLE || g.row0 + 128 >= g.row_end || gather(g, 1, qn1));
+      return true;
+    };
+    if (!dense && !gather_next(it)) it.pos = it.end;
     while (it.next(a, bars->lens, s)) {
+      if (!dense && s.n > 0 && !gather_next(it)) break;
       float2 ml0 = make_float2(-1e30f, 0.f);
       if (SINGLE) {
         float2 ml1 = ml0;
@@ -752,79 +764,126 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Joins n partial results of a row, the first n_p in slots 0.., the others in
-// slots slots_p..: o = sum 2^(m_s - M) o_s / sum 2^(m_s - M) l_s.  One warp a
-// row, lane l holds channels 4l..4l+3.
-__device__ __forceinline__ void join_row(const FwdArgs& a, int64_t rid, int n_p, int n, uint16_t* out, float* lse) {
-  const int lane = threadIdx.x & 31;
-  const float2* ml = a.part_ml + rid * a.p.slots;
-  float m = -1e30f;
-  for (int i = lane; i < n; i += 32) m = fmaxf(m, ml[i < n_p ? i : a.p.slots_p + i - n_p].x);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  float l = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int i = 0; i < n; ++i) {
-    const int slot = i < n_p ? i : a.p.slots_p + i - n_p;
-    const float2 e = ml[slot];
-    if (e.y == 0.f) continue;  // no keys: its o was not written
-    const float w = ex2(e.x - m);
-    const float4 v = *reinterpret_cast<const float4*>(a.part_o + (rid * a.p.slots + slot) * 128 + 4 * lane);
-    l += e.y * w;
-    acc.x = fmaf(v.x, w, acc.x);
-    acc.y = fmaf(v.y, w, acc.y);
-    acc.z = fmaf(v.z, w, acc.z);
-    acc.w = fmaf(v.w, w, acc.w);
+// The partial results of a row from one source: n slots of a unit.
+struct Runs {
+  const float4* o;
+  const float2* ml;
+  int n, stride;
+  __device__ Runs(const FwdArgs& a, int own, int unit, int row) {
+    const Source& c = a.src[own];
+    const uint32_t first = c.start + (uint32_t)unit * c.tiles;
+    n = c.tpc ? (int)(c.by_tpc(first + c.tiles - 1) - c.by_tpc(first)) + 1 : 1;
+    stride = c.stride;
+    o = a.part_o[own] + (int64_t)unit * c.slots * 32 * stride + row;
+    ml = a.part_ml[own] + (int64_t)unit * c.slots * stride + row;
   }
-  const float inv = 1.0f / fmaxf(l, 1e-30f);
-  *reinterpret_cast<uint2*>(out + 4 * lane) =
-      make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
-  if (lse && lane == 0) *lse = l == 0.f ? -INFINITY : (m + lg2(l)) * 0.69314718055994531f;
+};
+
+// A softmax over some of the keys: maximum, sum and 16 channels of o.
+struct Some {
+  float m, l, o[16];
+  __device__ void add(float m2, float l2, const float* o2) {
+    const float top = fmaxf(m, m2), f = ex2(m - top), g = l2 == 0.f ? 0.f : ex2(m2 - top);
+    m = top;
+    l = l * f + l2 * g;
+#pragma unroll
+    for (int c = 0; c < 16; ++c) o[c] = o[c] * f + (l2 == 0.f ? 0.f : o2[c] * g);  // l2 = 0: o2 was not written
+  }
+};
+
+// Joins the slots of 32 rows, in a fixed order.  A lane has a row, the 32 warps
+// of the block 16 channels of every fourth slot each; a slot's o is read along
+// with its (m, l), four slots at a time, since what this costs is latency
+// (with 8 warps, the maximum first and the slots one after the other: 10 us
+// behind the kernel whose results it joins, against 4).
+constexpr int kJoinThreads = 1024;
+
+__device__ __forceinline__ void join_rows(const Runs* runs, int sources, bool live, uint16_t* out, float* lse) {
+  __shared__ float box[2][18][256];
+  const int w = (threadIdx.x >> 5) & 7, part = threadIdx.x >> 8, at = threadIdx.x & 255;
+  Some a;
+  a.m = -1e30f;
+  a.l = 0.f;
+#pragma unroll
+  for (int c = 0; c < 16; ++c) a.o[c] = 0.f;
+  if (live)
+    for (int k = 0; k < sources; ++k) {
+      const Runs& r = runs[k];
+#pragma unroll 2
+      for (int i = part; i < r.n; i += 4) {
+        const float2 e = r.ml[i * r.stride];
+        float4 v[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) v[c] = r.o[((int64_t)i * 32 + 4 * w + c) * r.stride];
+        a.add(e.x, e.y, reinterpret_cast<const float*>(v));
+      }
+    }
+  auto put = [&](int b) {
+    box[b][0][at] = a.m;
+    box[b][1][at] = a.l;
+#pragma unroll
+    for (int c = 0; c < 16; ++c) box[b][2 + c][at] = a.o[c];
+  };
+  auto take = [&](int b) {
+    float o[16];
+#pragma unroll
+    for (int c = 0; c < 16; ++c) o[c] = box[b][2 + c][at];
+    a.add(box[b][0][at], box[b][1][at], o);
+  };
+  if (part >= 2) put(part - 2);
+  __syncthreads();
+  if (part < 2) take(part);
+  __syncthreads();
+  if (part == 1) put(0);
+  __syncthreads();
+  if (part == 0 && live) {
+    take(0);
+    const float inv = 1.0f / fmaxf(a.l, 1e-30f);
+    uint32_t k[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) k[e] = pack_bf16(a.o[2 * e] * inv, a.o[2 * e + 1] * inv);
+    store32(out + 16 * w, k);
+    if (lse && w == 0) *lse = a.l == 0.f ? -INFINITY : (a.m + lg2(a.l)) * 0.69314718055994531f;
+  }
 }
 
 // Dense units: block (x, y) joins rows 32y..32y+31 of the unit that the start
 // of CTA x + 1's run cuts (if it is the first such start inside the unit).
-__global__ void __launch_bounds__(256) join_dense_kernel(const __grid_constant__ FwdArgs a) {
+__global__ void __launch_bounds__(kJoinThreads) join_dense_kernel(const __grid_constant__ FwdArgs a) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const FwdPlan& p = a.p;
-  const uint32_t start = (blockIdx.x + 1) * p.tpc;
-  const int u = p.by_tiles_o(start), j0 = start - u * p.tiles_o;
-  if (u >= p.units_o || j0 == 0) return;
-  const uint32_t first = start - j0;
-  const int c0 = p.by_tpc(first);
-  if (c0 != (int)blockIdx.x) return;
-  const int n = p.by_tpc(first + p.tiles_o - 1) - c0 + 1;
-  const int bh = p.by_per_o(u), b = p.by_heads(bh), h = bh - b * a.n.heads;
-  const int t0 = (u - bh * p.per_o) * p.unit_rows + blockIdx.y * 32;
-  for (int t = t0 + (threadIdx.x >> 5); t < min(t0 + 32, a.n.q_len); t += 8) {
-    const int64_t row = (int64_t)bh * a.n.q_len + t;
-    join_row(a, row, 0, n, a.out.at(b, t, h), a.lse ? a.lse + row : nullptr);
-  }
+  const Source& c = a.src[1];
+  const uint32_t start = (blockIdx.x + 1) * c.tpc;
+  const int u = c.by_tiles(start), j0 = start - u * c.tiles;
+  if (u >= c.units || j0 == 0 || c.by_tpc(start - j0) != blockIdx.x) return;
+  const int bh = c.by_per(u), b = a.by_heads(bh), h = bh - b * a.n.heads;
+  const int r = blockIdx.y * 32 + (threadIdx.x & 31), t = (u - bh * c.per) * c.rows + r;
+  const Runs runs(a, 1, u, r);
+  join_rows(&runs, 1, t < a.n.q_len, a.out.at(b, t, h), a.lse ? a.lse + (int64_t)bh * a.n.q_len + t : nullptr);
 }
 
-// Folded rows, one warp a row.
-__global__ void __launch_bounds__(256) join_folded_kernel(const __grid_constant__ FwdArgs a) {
+// Folded rows: block (x, y) joins rows 32x..32x+31 of key head y.
+__global__ void __launch_bounds__(kJoinThreads) join_folded_kernel(const __grid_constant__ FwdArgs a) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const FwdPlan& p = a.p;
-  const int rows = a.n.kv_heads * p.fold_rows;  // below 2^31: checked at the call
-  for (int rid = (blockIdx.x * blockDim.x + threadIdx.x) >> 5; rid < rows; rid += (gridDim.x * blockDim.x) >> 5) {
-    const int hk = p.by_rows(rid), fr = rid - hk * p.fold_rows;
-    const int bt = p.by_group(fr), b = p.by_q_len(bt), tok = bt - b * a.n.q_len;
+  const int fr0 = blockIdx.x * 32 + (threadIdx.x & 31);
+  const bool live = fr0 < a.fold_rows;
+  const int fr = live ? fr0 : 0;
+  const int bt = a.by_group(fr), b = a.by_q_len(bt), tok = bt - b * a.n.q_len;
+  const Source &p = a.src[0], &o = a.src[1];
+  const int in_b = fr - b * a.n.q_len * a.n.group;
+  for (int hk = blockIdx.y; hk < a.n.kv_heads; hk += gridDim.y) {
     const int h = hk * a.n.group + (fr - bt * a.n.group);
-    auto runs = [&](uint32_t start, int tiles) {
-      return p.tpc ? (int)(p.by_tpc(start + tiles - 1) - p.by_tpc(start)) + 1 : 1;
-    };
-    int n_p = 0, n = 0;
-    if (p.units_p) n_p = n = runs((uint32_t)(hk * p.per_p + fr / p.unit_rows) * p.tiles_p, p.tiles_p);
-    if (p.units_o) {
-      const int in_b = fr - b * a.n.q_len * a.n.group;
-      n += runs((uint32_t)(p.units_p * p.tiles_p) +
-                    (uint32_t)((b * a.n.kv_heads + hk) * p.per_o + in_b / p.unit_rows) * p.tiles_o, p.tiles_o);
-    }
-    if (n == 1) continue;  // written by its unit
+    const int up = hk * p.per + fr / p.rows, uo = (b * a.n.kv_heads + hk) * o.per + in_b / o.rows;
     const int64_t row = ((int64_t)b * a.n.heads + h) * a.n.q_len + tok;
-    join_row(a, rid, n_p, n, a.out.at(b, tok, h), a.lse ? a.lse + row : nullptr);
+    float* lse = a.lse ? a.lse + row : nullptr;
+    uint16_t* out = a.out.at(b, tok, h);
+    if (a.two_sources) {
+      const Runs runs[2] = {Runs(a, 0, up, fr % p.rows), Runs(a, 1, uo, in_b % o.rows)};
+      join_rows(runs, 2, live, out, lse);
+    } else {
+      const Runs runs = p.units ? Runs(a, 0, up, fr % p.rows) : Runs(a, 1, uo, in_b % o.rows);
+      join_rows(&runs, 1, live && runs.n > 1, out, lse);  // else written by its unit
+    }
+    __syncthreads();
   }
 }
 
@@ -840,51 +899,72 @@ __global__ void __launch_bounds__(256) no_keys_kernel(CrossShape n, Rows out, fl
   }
 }
 
+// Everything about a call that its sizes decide.
+struct FwdPlan {
+  FwdArgs a;                  // sizes and split only
+  int ctas;                   // 0: no keys at all
+  bool join;
+  size_t part_bytes[2];       // partial results of either source
+};
+
 FwdPlan plan_fwd(const CrossShape& n) {
+  auto div = [](int64_t d) { return make_div((uint32_t)(d > 0 ? d : 1)); };
   FwdPlan p{};
-  p.np = (n.prefix_len + 127) / 128;
-  p.nb = (n.kv_len + 127) / 128;
+  FwdArgs& a = p.a;
+  a.n = n;
+  a.np = (n.prefix_len + 127) / 128;
+  const int nb = (n.kv_len + 127) / 128;
+  Source* src = a.src;
   if (n.q_len >= 128) {
-    p.mode = kDense;
-    p.unit_rows = 256;
-    p.per_o = (n.q_len + 255) / 256;
-    p.units_o = p.np + p.nb ? n.batch * n.heads * p.per_o : 0;
-    p.tiles_o = p.np + p.nb;
+    a.mode = kDense;
+    src[1].rows = src[1].stride = 256;
+    src[1].per = (n.q_len + 255) / 256;
+    src[1].tiles = a.np + nb;
+    src[1].units = src[1].tiles ? n.batch * n.heads * src[1].per : 0;
   } else {
-    const int own_rows = n.q_len * n.group;
-    p.fold_rows = n.batch * own_rows;
-    p.mode = (p.np ? p.fold_rows : own_rows) <= 128 ? kSingle : kDual;
-    p.unit_rows = p.mode == kSingle ? 128 : 256;
-    p.per_p = (p.fold_rows + p.unit_rows - 1) / p.unit_rows;
-    p.per_o = (own_rows + p.unit_rows - 1) / p.unit_rows;
-    p.units_p = p.np ? n.kv_heads * p.per_p : 0;
-    p.units_o = p.nb ? n.batch * n.kv_heads * p.per_o : 0;
-    p.tiles_p = p.np;
-    p.tiles_o = p.nb;
+    // (a member's rows alone rarely fill two tiles where the batch's do, but a
+    // launch of their own in single mode measured 129 us against 112 for 32
+    // members over a 64k prefix)
+    const int rows[2] = {n.batch * n.q_len * n.group, n.q_len * n.group};
+    a.fold_rows = rows[0];
+    a.mode = rows[a.np ? 0 : 1] <= 128 ? kSingle : kDual;
+    for (int k = 0; k < 2; ++k) {
+      src[k].rows = a.mode == kSingle ? 128 : 256;
+      src[k].per = (rows[k] + src[k].rows - 1) / src[k].rows;
+      src[k].tiles = k ? nb : a.np;
+      src[k].units = src[k].tiles ? n.kv_heads * src[k].per * (k ? n.batch : 1) : 0;
+      src[k].stride = src[k].per == 1 ? rows[k] : src[k].rows;
+    }
   }
-  const int64_t units = (int64_t)p.units_p + p.units_o;
-  const int64_t total = (int64_t)p.units_p * p.tiles_p + (int64_t)p.units_o * p.tiles_o;
-  const int64_t longest = p.units_p ? (p.tiles_p > p.tiles_o ? p.tiles_p : p.tiles_o) : p.tiles_o;
+  a.units_p = src[0].units, a.units_o = src[1].units;
+  a.two_sources = a.units_p && a.units_o;
+  const int64_t units = (int64_t)a.units_p + a.units_o;
+  const int64_t pre = (int64_t)a.units_p * src[0].tiles, total = pre + (int64_t)a.units_o * src[1].tiles;
+  int64_t longest = 0;
+  for (int k = 0; k < 2; ++k)
+    if (src[k].units && src[k].tiles > longest) longest = src[k].tiles;
   const int64_t share = (total + kSms - 1) / kSms;
   // whole units in turn cost up to one unit more than the even share; the
-  // linear split costs the partial results' traffic and the combine launch,
-  // about the time of 4 tiles
-  if ((units + kSms - 1) / kSms * longest > share + share / 10 + 4 && total < INT_MAX) p.tpc = (int32_t)share;
-  p.ctas = (int32_t)(p.tpc ? (total + p.tpc - 1) / p.tpc : (units < kSms ? units : kSms));
-  p.slots_p = p.units_p ? (p.tpc ? (p.tiles_p - 1) / p.tpc + 2 : 1) : 0;
-  p.slots = p.slots_p + (p.units_o ? (p.tpc ? (p.tiles_o - 1) / p.tpc + 2 : 1) : 0);
-  p.combine = (p.units_p && p.units_o) || (p.tpc && p.tpc % (int32_t)longest != 0);
-  p.part_rows = p.combine ? (p.mode == kDense ? (int64_t)n.batch * n.heads * n.q_len : (int64_t)n.kv_heads * p.fold_rows)
-                          : 0;
-  auto div = [](int64_t d) { return make_div((uint32_t)(d > 0 ? d : 1)); };
-  p.by_per_p = div(p.per_p), p.by_per_o = div(p.per_o), p.by_tiles_p = div(p.tiles_p), p.by_tiles_o = div(p.tiles_o);
-  p.by_heads = div(n.heads), p.by_kv_heads = div(n.kv_heads), p.by_group = div(n.group), p.by_q_len = div(n.q_len);
-  p.by_rows = div(p.fold_rows), p.by_tpc = div(p.tpc);
+  // linear split costs the partial results' traffic and the join, about the
+  // time of 4 tiles
+  if ((units + kSms - 1) / kSms * longest > share + share / 10 + 4 && total < INT_MAX) a.tpc = (int32_t)share;
+  p.ctas = (int)(a.tpc ? (total + a.tpc - 1) / a.tpc : (units < kSms ? units : kSms));
+  p.join = a.two_sources || (a.tpc && a.tpc % (int32_t)longest != 0);
+  for (int k = 0; k < 2; ++k) {
+    if (src[k].units) {
+      src[k].tpc = a.tpc;
+      src[k].start = k && a.tpc ? (int32_t)pre : 0;
+      src[k].slots = a.tpc ? (src[k].tiles - 1) / a.tpc + 2 : 1;
+    }
+    src[k].by_per = div(src[k].per), src[k].by_tiles = div(src[k].tiles), src[k].by_tpc = div(src[k].tpc);
+    if (p.join) p.part_bytes[k] = ((size_t)src[k].units * src[k].slots * src[k].stride * (512 + 8) + 255) / 256 * 256;
+  }
+  a.by_heads = div(n.heads), a.by_kv_heads = div(n.kv_heads), a.by_group = div(n.group), a.by_q_len = div(n.q_len);
   return p;
 }
 
 template <bool SINGLE>
-cudaError_t launch_fwd(const FwdArgs& a, const CUtensorMap* m, cudaStream_t s) {
+cudaError_t launch_fwd(const FwdArgs& a, int ctas, const CUtensorMap* m, cudaStream_t s) {
   static std::once_flag once[64];
   static cudaError_t set_result[64];
   int dev = 0;
@@ -901,7 +981,7 @@ cudaError_t launch_fwd(const FwdArgs& a, const CUtensorMap* m, cudaStream_t s) {
     set_result[dev] = e;
   });
   if (set_result[dev] != cudaSuccess) return set_result[dev];
-  cross_fwd_kernel<SINGLE><<<a.p.ctas, kThreads, smem_bytes<SINGLE>(), s>>>(m[0], m[1], m[2], m[3], m[4], m[5], a);
+  cross_fwd_kernel<SINGLE><<<ctas, kThreads, smem_bytes<SINGLE>(), s>>>(m[0], m[1], m[2], m[3], m[4], m[5], a);
   return cudaGetLastError();
 }
 
@@ -912,26 +992,28 @@ unsigned warps_grid(int64_t rows) { return (unsigned)((rows + 7) / 8 < kSms * 8 
 size_t cross_fwd_workspace(const CrossShape& n) {
   if (!n.batch || !n.q_len) return 0;
   const FwdPlan p = plan_fwd(n);
-  return (size_t)(p.part_rows * p.slots) * (128 * sizeof(float) + sizeof(float2));
+  return p.part_bytes[0] + p.part_bytes[1];
 }
 
 cudaError_t launch_cross_fwd(const CrossLaunch& L, cudaStream_t s, std::string* err) {
-  const int64_t rows = (int64_t)L.n.batch * L.n.heads * L.n.q_len;
+  const CrossShape& n = L.n;
+  const int64_t rows = (int64_t)n.batch * n.heads * n.q_len;
   if (rows == 0) return cudaSuccess;
-  FwdArgs a{};
-  a.n = L.n;
-  a.p = plan_fwd(L.n);
-  if (a.p.units_p + a.p.units_o == 0) {
-    no_keys_kernel<<<warps_grid(rows), 256, 0, s>>>(L.n, L.out, L.lse);
+  FwdPlan p = plan_fwd(n);
+  if (!p.ctas) {
+    no_keys_kernel<<<warps_grid(rows), 256, 0, s>>>(n, L.out, L.lse);
     return cudaGetLastError();
   }
+  FwdArgs& a = p.a;
   a.q = L.q;
   a.out = L.out;
   a.kv_lens = L.kv_lens;
   a.lse = L.lse;
   a.scale_log2 = L.scale * 1.4426950408889634f;
-  a.part_o = (float*)L.ws;
-  a.part_ml = (float2*)(a.part_o + a.p.part_rows * a.p.slots * 128);
+  for (int k = 0; k < 2; ++k) {
+    a.part_o[k] = (float4*)(L.ws + (k ? p.part_bytes[0] : 0));
+    a.part_ml[k] = (float2*)(a.part_o[k] + (size_t)a.src[k].units * a.src[k].slots * a.src[k].stride * 32);
+  }
   a.status = L.status;
   a.wait_limit_ns = L.wait_limit_ns;
   a.q_b = L.q.b != 0, a.q_h = L.q.h != 0;
@@ -939,9 +1021,9 @@ cudaError_t launch_cross_fwd(const CrossLaunch& L, cudaStream_t s, std::string* 
   a.v_b = L.v.b != 0, a.v_h = L.v.h != 0;
   a.pk_h = L.pk.h != 0, a.pv_h = L.pv.h != 0;
   CUtensorMap m[6] = {};
-  const CrossShape& n = L.n;
-  if (a.p.mode == kDense && (!make_map4(&m[0], L.q, n.q_len, n.heads, n.batch, err) ||
-                             !make_map4(&m[5], L.out, n.q_len, n.heads, n.batch, err, 32)))
+  const bool dense = a.mode == kDense;
+  if (dense && (!make_map4(&m[0], L.q, n.q_len, n.heads, n.batch, err) ||
+                !make_map4(&m[5], L.out, n.q_len, n.heads, n.batch, err, 32)))
     return cudaErrorInvalidValue;
   if (n.kv_len && (!make_map4(&m[1], L.k, n.kv_len, n.kv_heads, n.batch, err) ||
                    !make_map4(&m[2], L.v, n.kv_len, n.kv_heads, n.batch, err)))
@@ -949,19 +1031,20 @@ cudaError_t launch_cross_fwd(const CrossLaunch& L, cudaStream_t s, std::string* 
   if (n.prefix_len && (!make_map4(&m[3], L.pk, n.prefix_len, n.kv_heads, 1, err) ||
                        !make_map4(&m[4], L.pv, n.prefix_len, n.kv_heads, 1, err)))
     return cudaErrorInvalidValue;
-  cudaError_t e = a.p.mode == kSingle ? launch_fwd<true>(a, m, s) : launch_fwd<false>(a, m, s);
-  if (e != cudaSuccess || !a.p.combine) return e;
+  cudaError_t e = a.mode == kSingle ? launch_fwd<true>(a, p.ctas, m, s) : launch_fwd<false>(a, p.ctas, m, s);
+  if (e != cudaSuccess || !p.join) return e;
   // placed while the attention kernel runs; waits for its end before it reads
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = a.p.mode == kDense ? dim3(a.p.ctas - 1, a.p.unit_rows / 32) : dim3(warps_grid(rows));
-  cfg.blockDim = dim3(256);
+  cfg.gridDim = dense ? dim3(p.ctas - 1, 8)
+                      : dim3((a.fold_rows + 31) / 32, n.kv_heads < 65535 ? n.kv_heads : 65535);
+  cfg.blockDim = dim3(kJoinThreads);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, a.p.mode == kDense ? join_dense_kernel : join_folded_kernel, a);
+  return cudaLaunchKernelEx(&cfg, dense ? join_dense_kernel : join_folded_kernel, a);
 }
 
 }  // namespace h3
