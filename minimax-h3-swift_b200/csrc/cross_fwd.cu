@@ -96,6 +96,8 @@ struct Seg {
   bool direct;                // the whole result of its rows
 };
 
+// (dense rows have no units of the prefix)
+template <int MODE>
 struct SegIter {
   uint32_t pos, end;          // key tiles of the linear split, or units
   __device__ explicit SegIter(const FwdArgs& a) {
@@ -113,8 +115,8 @@ struct SegIter {
     int j1, tiles;
     s.slot = 0;
     if (a.tpc) {
-      const uint32_t pre = a.units_p * a.src[0].tiles;
-      s.own = pos >= pre;
+      const uint32_t pre = MODE == kDense ? 0 : a.units_p * a.src[0].tiles;
+      s.own = MODE == kDense || pos >= pre;
       const uint32_t off = s.own ? pos - pre : pos;
       tiles = a.src[s.own].tiles;
       s.unit = a.src[s.own].by_tiles(off);
@@ -123,8 +125,8 @@ struct SegIter {
       s.slot = blockIdx.x - a.src[s.own].by_tpc(pos - s.j0);
       pos += j1 - s.j0;
     } else {
-      s.own = (int)pos >= a.units_p;
-      s.unit = (int)pos - (s.own ? a.units_p : 0);
+      s.own = MODE == kDense || (int)pos >= a.units_p;
+      s.unit = (int)pos - (MODE != kDense && s.own ? a.units_p : 0);
       tiles = a.src[s.own].tiles;
       s.j0 = 0;
       j1 = tiles;
@@ -141,7 +143,7 @@ struct SegIter {
       s.len = 0;
       s.npre = limit = a.np;
     } else {
-      if (a.mode == kDense) {
+      if (MODE == kDense) {
         s.b = a.by_heads(x);
         s.h = x - s.b * a.n.heads;
         s.hk = a.by_group(s.h);
@@ -160,7 +162,7 @@ struct SegIter {
       limit = s.npre + ((s.len + 127) >> 7);
     }
     s.n = max(0, min(j1, limit) - s.j0);
-    s.direct = s.j0 == 0 && j1 == tiles && !a.two_sources;
+    s.direct = s.j0 == 0 && j1 == tiles && (MODE == kDense || !a.two_sources);
     return true;
   }
   // valid keys of tile j of the segment's unit
@@ -169,10 +171,10 @@ struct SegIter {
   }
 };
 
-template <bool SINGLE>
+template <int MODE>
 struct Layout {
-  static constexpr int kRing = SINGLE ? 3 : 2;      // K/V entries
-  static constexpr int kQTiles = SINGLE ? 1 : 2;
+  static constexpr int kRing = MODE == kSingle ? 3 : 2;  // K/V entries
+  static constexpr int kQTiles = MODE == kSingle ? 1 : 2;
   // the rest of 224 KB in dense mode: two 4 KB output buffers an epilogue warp
   static constexpr int kTiles = 7 * kTileBytes;
 };
@@ -190,24 +192,24 @@ struct __align__(8) Barriers {
 };
 
 // flags of an entry: bit t: half t takes it; 2 + t / 4 + t: first / last of the segment for half t
-enum { kFirst = 2, kLast = 4, kSegFirst = 1 << 6, kSegLast = 1 << 7, kEnd = 1 << 8, kZeroShift = 16 };
+enum { kFirst = 2, kLast = 4, kSegFirst = 1 << 6, kSegLast = 1 << 7, kEnd = 1 << 8, kApart = 1 << 9, kZeroShift = 16 };
 
-template <bool SINGLE>
-constexpr int smem_bytes() {
-  return Layout<SINGLE>::kTiles + (int)sizeof(Barriers);
-}
-static_assert(smem_bytes<true>() <= 227 * 1024 && smem_bytes<false>() <= 227 * 1024, "shared memory");
+constexpr int kSmemBytes = 7 * kTileBytes + (int)sizeof(Barriers);
+static_assert(kSmemBytes <= 227 * 1024, "shared memory");
+
+constexpr int kApartTiles = 8;  // key tiles from which a segment's halves start apart
 
 // Instruction descriptor, kind::f16: bf16 x bf16 -> f32, M = N = 128.
 constexpr uint32_t kIdS = idesc_bf16(false), kIdPV = idesc_bf16(true);
 
-template <bool SINGLE>
+template <int MODE>
 __global__ void __launch_bounds__(kThreads, 1)
     cross_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                      const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_pk,
                      const __grid_constant__ CUtensorMap tm_pv, const __grid_constant__ CUtensorMap tm_o,
                      const __grid_constant__ FwdArgs a) {
-  using L = Layout<SINGLE>;
+  using L = Layout<MODE>;
+  constexpr bool SINGLE = MODE == kSingle, dense = MODE == kDense;
   extern __shared__ __align__(1024) uint8_t smem[];
   if (!tiles_aligned(smem, a.status)) return;
   uint8_t* sQ = smem;
@@ -215,7 +217,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   Barriers* bars = (Barriers*)(smem + L::kTiles);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int32_t* abort_flag = &bars->abort;
-  const bool dense = a.mode == kDense;
 
   if (threadIdx.x == 0) {
     for (int t = 0; t < 2; ++t) {
@@ -261,7 +262,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 0) {
       // ------------------------------------------------------- TMA producer
       if (lane == 0) {
-        SegIter it(a);
+        SegIter<MODE> it(a);
         Seg s{};
         int ec = 0, r = 0, issued = 0;
         uint32_t ph = 0;
@@ -278,13 +279,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                      (i == 0 ? kSegFirst : 0) | (i == s.n - 1 ? kSegLast : 0);
             } else {
               const int act = act1 ? 3 : 1;
-              info = act | (i == 0 ? act << kFirst : 0) | (i == s.n - 1 ? act << kLast : 0);
+              info = act | (i == 0 ? act << kFirst : 0) | (i == s.n - 1 ? act << kLast : 0) |
+                     (i == 0 && act1 && s.n >= kApartTiles ? kApart : 0);
             }
             const bool pre = j < s.npre;
             // value rows past the member's length hold whatever the caller
             // left there, and 0 x NaN would reach the result: the issuer
             // clears them (TMA itself clears rows past the operand's end)
-            const int valid = SegIter::valid(a, s, j);
+            const int valid = SegIter<MODE>::valid(a, s, j);
             if (!pre && valid < 128 && s.len < a.n.kv_len) info |= valid << kZeroShift;
             if (!wait(&bars->k_empty[r], ph ^ 1) || !wait(&bars->v_empty[r], ph ^ 1)) {
               ok = false;
@@ -409,6 +411,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (info & 1) ok = issue_s(T0{}, info);
         if (!SINGLE && ok && pend1 >= 0) ok = issue_pv(T1{});
+        // Any distance between the halves of 1,024 cycles up (that of their
+        // products) lasts.  At half a period their exponentials do not meet on
+        // the MUFU units, so half 1 begins a long segment when half 0's first
+        // weights are out (4,096 keys: 2.48 ms against 2.56; below 8 tiles the
+        // wait costs what it gains).
+        if (dense && ok && (info & kApart)) ok = iwait(&bars->p_half[0], ph >> 3);
         if (ok && (info & 2)) ok = issue_s(T1{}, info);
         if (!ok) break;
         tc_commit_w(smem_u32(&bars->k_empty[r]));
@@ -423,7 +431,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (ok && pend1 >= 0) issue_pv(T1{});
       // aborted or not: MMAs retire in order, so this covers all of them
       tc_commit_w(smem_u32(&bars->done));
-    } else if (dense) {
+    } else if constexpr (dense) {
       // -------------------------------------------------- Q tiles (TMA)
       if (warp == 3 && lane == 0) {
         // A segment's Q tiles complete its first entry's barrier.  That the
@@ -431,7 +439,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // its entries has completed, so this arrival falls in the right phase.
         // The segment after it goes to L2 meanwhile: one buffer covers L2's
         // latency, not HBM's.
-        SegIter it(a);
+        SegIter<MODE> it(a);
         Seg s{}, following{};
         int qn0 = 0, qn1 = 0, ec = 0;
         bool more = it.next(a, bars->lens, following);
@@ -474,7 +482,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tS = lane_base + 256 * t, tO = tS + 128;
     const float sl2 = a.scale_log2;
     const uint64_t sl2x2 = dup2(sl2);
-    SegIter it(a);
+    SegIter<MODE> it(a);
     Seg s{};
     int ec = 0, ns = 0, nseg = 0;
     bool ok = true;
@@ -486,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (nt == 0) continue;
       float m = -1e30f, l = 0.f;
       for (int x = 0; ok && x < nt; ++x) {
-        const int valid = SegIter::valid(a, s, s.j0 + i0 + x * step);
+        const int valid = SegIter<MODE>::valid(a, s, s.j0 + i0 + x * step);
         if (!wait_w(&bars->s_full[t], ns & 1)) {
           ok = false;
           break;
@@ -574,7 +582,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int q = warp & 3, r = 32 * q + lane;
     const uint32_t tO = tmem + ((uint32_t)(32 * q) << 16) + 128;
     uint8_t* stage = smem + 6 * kTileBytes + q * 8192;  // dense: two boxes of 32 rows x 64 columns
-    SegIter it(a);
+    SegIter<MODE> it(a);
     Seg s{};
     int ec = 0, n0 = 0, n1 = 0;  // segments of either half
     // half t's (m, l) and O are there
@@ -712,7 +720,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       return true;
     };
     int qn0 = 0, qn1 = 0;
-    auto gather_next = [&](SegIter ahead) {
+    auto gather_next = [&](SegIter<MODE> ahead) {
       Seg g{};
       while (ahead.next(a, bars->lens, g))
         if (g.n > 0)
@@ -963,7 +971,7 @@ FwdPlan plan_fwd(const CrossShape& n) {
   return p;
 }
 
-template <bool SINGLE>
+template <int MODE>
 cudaError_t launch_fwd(const FwdArgs& a, int ctas, const CUtensorMap* m, cudaStream_t s) {
   static std::once_flag once[64];
   static cudaError_t set_result[64];
@@ -973,15 +981,15 @@ cudaError_t launch_fwd(const FwdArgs& a, int ctas, const CUtensorMap* m, cudaStr
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   std::call_once(once[dev], [dev] {
     cudaError_t e =
-        cudaFuncSetAttribute(cross_fwd_kernel<SINGLE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<SINGLE>());
+        cudaFuncSetAttribute(cross_fwd_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
     // the register split needs exactly 128 a thread at launch
     cudaFuncAttributes fa;
-    if (e == cudaSuccess) e = cudaFuncGetAttributes(&fa, cross_fwd_kernel<SINGLE>);
+    if (e == cudaSuccess) e = cudaFuncGetAttributes(&fa, cross_fwd_kernel<MODE>);
     if (e == cudaSuccess && fa.numRegs != 128) e = cudaErrorInvalidConfiguration;
     set_result[dev] = e;
   });
   if (set_result[dev] != cudaSuccess) return set_result[dev];
-  cross_fwd_kernel<SINGLE><<<ctas, kThreads, smem_bytes<SINGLE>(), s>>>(m[0], m[1], m[2], m[3], m[4], m[5], a);
+  cross_fwd_kernel<MODE><<<ctas, kThreads, kSmemBytes, s>>>(m[0], m[1], m[2], m[3], m[4], m[5], a);
   return cudaGetLastError();
 }
 
@@ -1031,7 +1039,9 @@ cudaError_t launch_cross_fwd(const CrossLaunch& L, cudaStream_t s, std::string* 
   if (n.prefix_len && (!make_map4(&m[3], L.pk, n.prefix_len, n.kv_heads, 1, err) ||
                        !make_map4(&m[4], L.pv, n.prefix_len, n.kv_heads, 1, err)))
     return cudaErrorInvalidValue;
-  cudaError_t e = a.mode == kSingle ? launch_fwd<true>(a, p.ctas, m, s) : launch_fwd<false>(a, p.ctas, m, s);
+  cudaError_t e = dense               ? launch_fwd<kDense>(a, p.ctas, m, s)
+                  : a.mode == kSingle ? launch_fwd<kSingle>(a, p.ctas, m, s)
+                                      : launch_fwd<kDual>(a, p.ctas, m, s);
   if (e != cudaSuccess || !p.join) return e;
   // placed while the attention kernel runs; waits for its end before it reads
   cudaLaunchConfig_t cfg = {};
