@@ -14,12 +14,15 @@ namespace h3 {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kGroups = kThreads / 8;   // rows a CTA has in hand at a time
+constexpr int kCtas = 2;                // an SM
+constexpr int kGroups = kThreads / 8;   // rows a CTA works on at a time
 
 struct Operand {
   QkNormOperand o;
   Div heads, tokens;
   uint32_t rows;
+  uint32_t runs;              // of 4 << shift rows, one warp's
+  int shift;
 };
 
 struct NormArgs {
@@ -71,12 +74,13 @@ struct Channels {
       v[1] = make_uint4(w[4], w[5], w[6], w[7]);
     }
   }
-  __device__ void store(uint16_t* p, const float* a, const float* b) const {
+  // a, b: eight values each, two a word
+  __device__ void store(uint16_t* p, const uint64_t* a, const uint64_t* b) const {
     uint32_t w[8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      w[i] = pack_bf16(a[2 * i], a[2 * i + 1]);
-      w[4 + i] = pack_bf16(b[2 * i], b[2 * i + 1]);
+      w[i] = pack_bf16(__uint_as_float((uint32_t)a[i]), __uint_as_float((uint32_t)(a[i] >> 32)));
+      w[4 + i] = pack_bf16(__uint_as_float((uint32_t)b[i]), __uint_as_float((uint32_t)(b[i] >> 32)));
     }
     if (VEC) {
       *reinterpret_cast<uint4*>(p + first(0)) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -91,13 +95,30 @@ struct Channels {
   }
 };
 
-__device__ __forceinline__ void unpack(const uint4& u, float* f) {
+// Two fp32 values side by side, two operations an instruction.
+using f2 = uint64_t;
+__device__ __forceinline__ f2 two(uint32_t lo, uint32_t hi) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+  return r;
+}
+__device__ __forceinline__ f2 mul(f2 a, f2 b) {
+  f2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 fma(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ float lo_of(f2 v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float hi_of(f2 v) { return __uint_as_float((uint32_t)(v >> 32)); }
+
+__device__ __forceinline__ void unpack(const uint4& u, f2* f) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[2 * i] = __uint_as_float(w[i] << 16);
-    f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-  }
+  for (int i = 0; i < 4; ++i) f[i] = two(w[i] << 16, w[i] & 0xffff0000u);
 }
 
 __device__ __forceinline__ float sum8(float v) {
@@ -106,148 +127,302 @@ __device__ __forceinline__ float sum8(float v) {
   return v + __shfl_xor_sync(0xffffffffu, v, 1);
 }
 
-// Turns the thread's pairs by the token's table entries (t0, t1; t2, t3), or
-// by their transpose.
-template <bool VEC, bool BACK>
-__device__ __forceinline__ void rotate(const QkNormOperand& o, const Place& at, int t, float* a, float* b) {
-  if (!o.table || 8 * t >= o.half) return;
-  const uint16_t* row = o.table + at.b * o.table_batch + (int64_t)at.s * o.half * 4 + 32 * t;
+// The rotation of the thread's eight pairs at one token: table entries
+// (t0, t1; t2, t3) as bf16, kept from row to row while the token stays.
+template <bool VEC>
+struct Rotation {
+  uint4 e[4];
+  bool on;                    // the thread's pairs are turned
+  uint32_t b = 0xffffffffu, s = 0;
+  __device__ Rotation(const QkNormOperand& o, int t) : on(o.table && 8 * t < o.half) {}
+  static __device__ const uint16_t* entries(const QkNormOperand& o, uint32_t b, uint32_t s, int t) {
+    return o.table + b * o.table_batch + (int64_t)s * o.half * 4 + 32 * t;
+  }
+  __device__ __forceinline__ void at(const QkNormOperand& o, uint32_t tb, uint32_t ts, int t) {
+    if (!on || (tb == b && ts == s)) return;
+    b = tb, s = ts;
+    const uint16_t* row = entries(o, b, s, t);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint4 e;
-    if (VEC) {
-      e = *reinterpret_cast<const uint4*>(row + 8 * i);
-    } else {  // 8-byte aligned entries; those past half are not there
-      const uint2 id = make_uint2(0x3f80u, 0x3f800000u);
-      const uint2* p = reinterpret_cast<const uint2*>(row) + 2 * i;
-      const uint2 e0 = 8 * t + 2 * i < o.half ? p[0] : id, e1 = 8 * t + 2 * i + 1 < o.half ? p[1] : id;
-      e = make_uint4(e0.x, e0.y, e1.x, e1.y);
-    }
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const uint32_t lo = k ? e.z : e.x, hi = k ? e.w : e.y;
-      const float t0 = __uint_as_float(lo << 16), t1 = __uint_as_float(lo & 0xffff0000u);
-      const float t2 = __uint_as_float(hi << 16), t3 = __uint_as_float(hi & 0xffff0000u);
-      float &x = a[2 * i + k], &y = b[2 * i + k];
-      const float u = x;
-      x = t0 * u + (BACK ? t2 : t1) * y;
-      y = (BACK ? t1 : t2) * u + t3 * y;
+    for (int i = 0; i < 4; ++i) {
+      if (VEC) {
+        e[i] = *reinterpret_cast<const uint4*>(row + 8 * i);
+      } else {  // 8-byte aligned entries; those past half are not there
+        const uint2 id = make_uint2(0x3f80u, 0x3f800000u);
+        const uint2* q = reinterpret_cast<const uint2*>(row) + 2 * i;
+        const uint2 e0 = 8 * t + 2 * i < o.half ? q[0] : id, e1 = 8 * t + 2 * i + 1 < o.half ? q[1] : id;
+        e[i] = make_uint4(e0.x, e0.y, e1.x, e1.y);
+      }
     }
   }
+  // by the table's matrices, or by their transposes
+  template <bool BACK>
+  __device__ __forceinline__ void turn(f2* a, f2* c) const {
+    if (!on) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f2 t0 = two(e[i].x << 16, e[i].z << 16), t1 = two(e[i].x & 0xffff0000u, e[i].z & 0xffff0000u);
+      const f2 t2 = two(e[i].y << 16, e[i].w << 16), t3 = two(e[i].y & 0xffff0000u, e[i].w & 0xffff0000u);
+      const f2 u = a[i];
+      a[i] = fma(t0, u, mul(BACK ? t2 : t1, c[i]));
+      c[i] = fma(BACK ? t1 : t2, u, mul(t3, c[i]));
+    }
+  }
+};
+
+// Rows of a group of eight threads, in order: a warp takes runs of 4 << shift
+// consecutive rows (its four groups one row each at a time), so that the rows
+// of a token, and with them a table entry, mostly follow one another.  N
+// operands' offsets go along; only the start of a run divides.
+template <int N>
+struct Cursor {
+  const Operand& p;
+  uint32_t run, row, left;    // the warp's run, the group's row, rows until the next run
+  uint32_t b, s, h;
+  int64_t off[N];
+  const Rows* of[N];
+  __device__ Cursor(const Operand& p_, const Rows& r0) : p(p_) {
+    of[0] = &r0;
+    seek((blockIdx.x * kThreads + threadIdx.x) >> 5);
+  }
+  __device__ Cursor(const Operand& p_, const Rows& r0, const Rows& r1) : p(p_) {
+    of[0] = &r0;
+    of[N - 1] = &r1;
+    seek((blockIdx.x * kThreads + threadIdx.x) >> 5);
+  }
+  __device__ void seek(uint32_t to) {
+    run = to;
+    row = (run << (2 + p.shift)) + ((threadIdx.x >> 3) & 3);
+    left = 1u << p.shift;
+    const Place at = place(row, p);
+    b = at.b, s = at.s, h = at.h;
+#pragma unroll
+    for (int i = 0; i < N; ++i) off[i] = b * of[i]->b + s * of[i]->t + h * of[i]->h;
+  }
+  __device__ __forceinline__ bool more() const { return run < p.runs; }  // the same for the whole warp
+  __device__ __forceinline__ bool live() const { return row < p.rows; }
+  __device__ __forceinline__ void next() {
+    if (--left == 0) {
+      seek(run + gridDim.x * (kThreads / 32));
+      return;
+    }
+    row += 4;
+    h += 4;
+#pragma unroll
+    for (int i = 0; i < N; ++i) off[i] += 4 * of[i]->h;
+    while (h >= (uint32_t)p.o.heads) {
+      h -= p.o.heads;
+      ++s;
+#pragma unroll
+      for (int i = 0; i < N; ++i) off[i] += of[i]->t - p.o.heads * of[i]->h;
+      if (s == (uint32_t)p.o.tokens) {
+        s = 0;
+        ++b;
+#pragma unroll
+        for (int i = 0; i < N; ++i) off[i] += of[i]->b - p.o.tokens * of[i]->t;
+      }
+    }
+  }
+};
+
+__device__ __forceinline__ void copy16(void* dst, const uint16_t* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
+               : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// Two rows a group of eight threads in flight; 3 CTAs of 256 threads an SM.
+// Both bounds are near: bytes in flight and instructions.  A thread's own 32
+// bytes a row run through a ring of six rows in shared memory that only it
+// reads (no barrier), 96 KB an SM; the table's entries stay in registers from
+// row to row, positions advance without divisions, and the arithmetic takes
+// two values an instruction.  FWD_FIGURE
 template <bool VEC>
-__global__ void __launch_bounds__(kThreads, 3) qk_norm_fwd_kernel(const __grid_constant__ NormArgs a) {
-  constexpr int U = 2;
-  const int t = threadIdx.x & 7, g = threadIdx.x >> 3;
+__global__ void __launch_bounds__(kThreads, kCtas) qk_norm_fwd_kernel(const __grid_constant__ NormArgs a) {
+  constexpr int kStages = 6;
+  __shared__ uint4 ring[VEC ? kStages : 1][2][kThreads];
+  const int t = threadIdx.x & 7;
 #pragma unroll 1
   for (int k = 0; k < 2; ++k) {
     const Operand& p = a.op[k];
     if (p.rows == 0) continue;
     const Channels<VEC> ch(t, p.o.half);
-    uint4 w[2];
-    ch.load(p.o.w, w);
-    for (uint32_t r0 = blockIdx.x * (U * kGroups); r0 < p.rows; r0 += gridDim.x * (U * kGroups)) {
-      uint4 raw[U][2];
-      Place at[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const uint32_t row = r0 + u * kGroups + g;
-        at[u] = place(row < p.rows ? row : r0, p);
-        ch.load(p.o.x.at(at[u].b, at[u].s, at[u].h), raw[u]);
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        float x[8], y[8], wx[8], wy[8];
-        unpack(raw[u][0], x);
-        unpack(raw[u][1], y);
-        unpack(w[0], wx);
-        unpack(w[1], wy);
-        float ss = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) ss += x[i] * x[i] + y[i] * y[i];
-        const float r = 1.0f / sqrtf(sum8(ss) * (1.0f / 128.0f) + a.eps);
-        if (r0 + u * kGroups + g >= p.rows) continue;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          x[i] *= r * wx[i];
-          y[i] *= r * wy[i];
+    const int c0 = ch.first(0), c1 = ch.second(0);
+    Cursor<1> in(p, p.o.x), at(p, p.o.y);
+    auto fetch = [&](int slot) {
+      if (in.more()) {
+        if (in.live()) {
+          const uint16_t* x = p.o.x.p + in.off[0];
+          copy16(&ring[slot][0][threadIdx.x], x + c0);
+          copy16(&ring[slot][1][threadIdx.x], x + c1);
         }
-        rotate<VEC, false>(p.o, at[u], t, x, y);
-        ch.store(p.o.y.at(at[u].b, at[u].s, at[u].h), x, y);
+        in.next();
+      }
+      copies_commit();
+    };
+    if constexpr (VEC) {
+#pragma unroll
+      for (int i = 0; i < kStages; ++i) fetch(i);
+    }
+    uint4 raw[2];
+    f2 wx[4], wy[4];
+    ch.load(p.o.w, raw);
+    unpack(raw[0], wx);
+    unpack(raw[1], wy);
+    Rotation<VEC> rot(p.o, t);
+    int slot = 0;
+#pragma unroll 1
+    for (; at.more(); at.next()) {
+      const bool live = at.live();
+      if (live) rot.at(p.o, at.b, at.s, t);
+      if constexpr (VEC) {
+        copies_wait<kStages - 1>();
+        raw[0] = ring[slot][0][threadIdx.x];
+        raw[1] = ring[slot][1][threadIdx.x];
+      } else {
+        if (live) ch.load(p.o.x.p + in.off[0], raw);
+        in.next();
+      }
+      f2 x[4], y[4];
+      unpack(raw[0], x);
+      unpack(raw[1], y);
+      f2 ss = mul(x[0], x[0]);
+#pragma unroll
+      for (int i = 1; i < 4; ++i) ss = fma(x[i], x[i], ss);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ss = fma(y[i], y[i], ss);
+      const float r = rsqrtf(sum8(lo_of(ss) + hi_of(ss)) * (1.0f / 128.0f) + a.eps);
+      const f2 r2 = dup2(r);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[i] = mul(x[i], mul(r2, wx[i]));
+        y[i] = mul(y[i], mul(r2, wy[i]));
+      }
+      rot.template turn<false>(x, y);
+      if (live) ch.store(p.o.y.p + at.off[0], x, y);
+      if constexpr (VEC) {
+        fetch(slot);
+        if (++slot == kStages) slot = 0;
       }
     }
+    if constexpr (VEC) copies_wait<0>();
   }
 }
 
-// The same walk; each thread sums dw of its 16 channels in registers, the CTA
-// joins its groups in shared memory and leaves one partial sum an operand.
+// The same walk over x and the gradient, 64 bytes a row in a ring of three;
+// each thread sums dw of its 16 channels in registers, the CTA joins its
+// groups in shared memory and leaves one partial sum an operand.  BWD_FIGURE
 template <bool VEC>
-__global__ void __launch_bounds__(kThreads, 2) qk_norm_bwd_kernel(const __grid_constant__ NormArgs a) {
-  constexpr int U = 2;
-  __shared__ float part[kGroups][128];
+__global__ void __launch_bounds__(kThreads, kCtas) qk_norm_bwd_kernel(const __grid_constant__ NormArgs a) {
+  constexpr int kStages = 3;
+  __shared__ union {
+    uint4 ring[VEC ? kStages : 1][4][kThreads];
+    float part[kGroups][128];
+  } sm;
   const int t = threadIdx.x & 7, g = threadIdx.x >> 3;
   asm volatile("griddepcontrol.launch_dependents;");
 #pragma unroll 1
   for (int k = 0; k < 2; ++k) {
     const Operand& p = a.op[k];
     const Channels<VEC> ch(t, p.o.half);
-    float da[8] = {}, db[8] = {};
-    uint4 w[2];
-    ch.load(p.o.w, w);
-    for (uint32_t r0 = blockIdx.x * (U * kGroups); r0 < p.rows; r0 += gridDim.x * (U * kGroups)) {
-      uint4 raw[U][2], rawg[U][2];
-      Place at[U];
+    f2 da[4] = {}, db[4] = {};
+    if (p.rows) {
+      const int c0 = ch.first(0), c1 = ch.second(0);
+      Cursor<2> in(p, p.o.x, p.o.g);
+      Cursor<1> at(p, p.o.y);
+      auto fetch = [&](int slot) {
+        if (in.more()) {
+          if (in.live()) {
+            const uint16_t *x = p.o.x.p + in.off[0], *go = p.o.g.p + in.off[1];
+            copy16(&sm.ring[slot][0][threadIdx.x], x + c0);
+            copy16(&sm.ring[slot][1][threadIdx.x], x + c1);
+            copy16(&sm.ring[slot][2][threadIdx.x], go + c0);
+            copy16(&sm.ring[slot][3][threadIdx.x], go + c1);
+          }
+          in.next();
+        }
+        copies_commit();
+      };
+      if constexpr (VEC) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const uint32_t row = r0 + u * kGroups + g;
-        at[u] = place(row < p.rows ? row : r0, p);
-        ch.load(p.o.x.at(at[u].b, at[u].s, at[u].h), raw[u]);
-        ch.load(p.o.g.at(at[u].b, at[u].s, at[u].h), rawg[u]);
+        for (int i = 0; i < kStages; ++i) fetch(i);
       }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        float x[8], y[8], gx[8], gy[8], wx[8], wy[8];
-        unpack(raw[u][0], x);
-        unpack(raw[u][1], y);
-        unpack(rawg[u][0], gx);
-        unpack(rawg[u][1], gy);
+      uint4 w[2], raw[2], rawg[2];
+      ch.load(p.o.w, w);
+      Rotation<VEC> rot(p.o, t);
+      int slot = 0;
+#pragma unroll 1
+      for (; at.more(); at.next()) {
+        const bool live = at.live();
+        if (live) rot.at(p.o, at.b, at.s, t);
+        if constexpr (VEC) {
+          copies_wait<kStages - 1>();
+          raw[0] = sm.ring[slot][0][threadIdx.x];
+          raw[1] = sm.ring[slot][1][threadIdx.x];
+          rawg[0] = sm.ring[slot][2][threadIdx.x];
+          rawg[1] = sm.ring[slot][3][threadIdx.x];
+        } else {
+          if (live) {
+            ch.load(p.o.x.p + in.off[0], raw);
+            ch.load(p.o.g.p + in.off[1], rawg);
+          }
+          in.next();
+        }
+        f2 x[4], y[4], gx[4], gy[4], wx[4], wy[4];
+        unpack(raw[0], x);
+        unpack(raw[1], y);
+        unpack(rawg[0], gx);
+        unpack(rawg[1], gy);
         unpack(w[0], wx);
         unpack(w[1], wy);
-        rotate<VEC, true>(p.o, at[u], t, gx, gy);
-        float ss = 0.f, c = 0.f;
+        rot.template turn<true>(gx, gy);
+        f2 ss = mul(x[0], x[0]), c2 = mul(mul(gx[0], wx[0]), x[0]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          ss += x[i] * x[i] + y[i] * y[i];
-          c += gx[i] * wx[i] * x[i] + gy[i] * wy[i] * y[i];
+        for (int i = 1; i < 4; ++i) {
+          ss = fma(x[i], x[i], ss);
+          c2 = fma(mul(gx[i], wx[i]), x[i], c2);
         }
-        const float r = 1.0f / sqrtf(sum8(ss) * (1.0f / 128.0f) + a.eps);
-        c = sum8(c) * r * r * (1.0f / 128.0f);
-        if (r0 + u * kGroups + g >= p.rows) continue;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          da[i] += gx[i] * (x[i] * r);
-          db[i] += gy[i] * (y[i] * r);
-          x[i] = r * (gx[i] * wx[i] - x[i] * c);
-          y[i] = r * (gy[i] * wy[i] - y[i] * c);
+        for (int i = 0; i < 4; ++i) {
+          ss = fma(y[i], y[i], ss);
+          c2 = fma(mul(gy[i], wy[i]), y[i], c2);
         }
-        ch.store(p.o.y.at(at[u].b, at[u].s, at[u].h), x, y);
+        const float r = rsqrtf(sum8(lo_of(ss) + hi_of(ss)) * (1.0f / 128.0f) + a.eps);
+        const float c = sum8(lo_of(c2) + hi_of(c2)) * r * r * (1.0f / 128.0f);
+        if (live) {
+          const f2 r2 = dup2(r), mc = dup2(-c);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            da[i] = fma(gx[i], mul(x[i], r2), da[i]);
+            db[i] = fma(gy[i], mul(y[i], r2), db[i]);
+            x[i] = mul(r2, fma(x[i], mc, mul(gx[i], wx[i])));
+            y[i] = mul(r2, fma(y[i], mc, mul(gy[i], wy[i])));
+          }
+          ch.store(p.o.y.p + at.off[0], x, y);
+        }
+        if constexpr (VEC) {
+          fetch(slot);
+          if (++slot == kStages) slot = 0;
+        }
       }
+      if constexpr (VEC) copies_wait<0>();
     }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      part[g][ch.first(i)] = da[i];
-      part[g][ch.second(i)] = db[i];
+      sm.part[g][ch.first(i)] = i & 1 ? hi_of(da[i >> 1]) : lo_of(da[i >> 1]);
+      sm.part[g][ch.second(i)] = i & 1 ? hi_of(db[i >> 1]) : lo_of(db[i >> 1]);
     }
     __syncthreads();
     if (threadIdx.x < 128) {
       float s = 0.f;
 #pragma unroll 8
-      for (int i = 0; i < kGroups; ++i) s += part[i][threadIdx.x];
+      for (int i = 0; i < kGroups; ++i) s += sm.part[i][threadIdx.x];
       a.ws[((int64_t)blockIdx.x * 2 + k) * 128 + threadIdx.x] = s;
     }
+    __syncthreads();
   }
 }
 
@@ -269,9 +444,7 @@ __global__ void __launch_bounds__(1024) qk_norm_dw_kernel(const __grid_constant_
   }
 }
 
-constexpr int kSms = 148;
-constexpr int kFwdCtas = kSms * 3, kBwdCtas = kSms * 2;
-
+constexpr int kGrid = 148 * kCtas;
 // Sixteen-byte accesses need a rotation of whole vectors and a table aligned to them.
 bool vectors(const QkNormOperand& o) {
   return o.half % 8 == 0 && !((uintptr_t)o.table & 15) && !(o.table_batch & 7);
@@ -286,6 +459,9 @@ NormArgs args_of(const QkNormLaunch& l, uint32_t* most) {
     p.rows = (uint32_t)((int64_t)l.batch * p.o.tokens * p.o.heads);
     p.heads = make_div((uint32_t)p.o.heads);
     p.tokens = make_div((uint32_t)(p.o.tokens > 0 ? p.o.tokens : 1));
+    // runs of up to 32 rows where every warp of the full grid has one
+    while (p.shift < 3 && p.rows / (8u << p.shift) >= (uint32_t)kGrid * (kThreads / 32)) ++p.shift;
+    p.runs = (p.rows + (4u << p.shift) - 1) >> (2 + p.shift);
     *most = p.rows > *most ? p.rows : *most;
   }
   a.eps = l.eps;
@@ -293,30 +469,32 @@ NormArgs args_of(const QkNormLaunch& l, uint32_t* most) {
   return a;
 }
 
-unsigned grid_of(uint32_t rows, int most) {
-  const uint32_t want = (rows + 2 * kGroups - 1) / (2 * kGroups);
-  return want < 1 ? 1 : want < (uint32_t)most ? want : (unsigned)most;
+unsigned grid_of(uint32_t rows) {
+  const uint32_t want = (rows + kGroups - 1) / kGroups;
+  return want < 1 ? 1 : want < kGrid ? want : kGrid;
 }
 
 }  // namespace
 
-size_t qk_norm_bwd_workspace() { return (size_t)kBwdCtas * 2 * 128 * sizeof(float); }
+size_t qk_norm_bwd_workspace() { return (size_t)kGrid * 2 * 128 * sizeof(float); }
 
 cudaError_t launch_qk_norm_fwd(const QkNormLaunch& l, cudaStream_t s) {
+  const bool vec = vectors(l.op[0]) && vectors(l.op[1]);
   uint32_t rows;
   const NormArgs a = args_of(l, &rows);
   if (rows == 0) return cudaSuccess;
-  const unsigned grid = grid_of(rows, kFwdCtas);
-  if (vectors(l.op[0]) && vectors(l.op[1])) qk_norm_fwd_kernel<true><<<grid, kThreads, 0, s>>>(a);
+  const unsigned grid = grid_of(rows);
+  if (vec) qk_norm_fwd_kernel<true><<<grid, kThreads, 0, s>>>(a);
   else qk_norm_fwd_kernel<false><<<grid, kThreads, 0, s>>>(a);
   return cudaGetLastError();
 }
 
 cudaError_t launch_qk_norm_bwd(const QkNormLaunch& l, cudaStream_t s) {
+  const bool vec = vectors(l.op[0]) && vectors(l.op[1]);
   uint32_t rows;
   const NormArgs a = args_of(l, &rows);
-  const unsigned grid = grid_of(rows, kBwdCtas);
-  if (vectors(l.op[0]) && vectors(l.op[1])) qk_norm_bwd_kernel<true><<<grid, kThreads, 0, s>>>(a);
+  const unsigned grid = grid_of(rows);
+  if (vec) qk_norm_bwd_kernel<true><<<grid, kThreads, 0, s>>>(a);
   else qk_norm_bwd_kernel<false><<<grid, kThreads, 0, s>>>(a);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
