@@ -214,27 +214,6 @@ struct DqUnit {
   }
 };
 
-// 8x8 transpose over groups of eight lanes: v[i] of lane j and v[j] of lane i
-// change places, so that a thread's row becomes 16 bytes of each of eight rows.
-__device__ __forceinline__ void transpose8(uint4 (&v)[8]) {
-  const int p = threadIdx.x & 7;
-#pragma unroll
-  for (int s = 1; s < 8; s <<= 1) {
-    const bool up = p & s;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (i & s) continue;
-      uint4 m = up ? v[i] : v[i | s];
-      m.x = __shfl_xor_sync(0xffffffffu, m.x, s);
-      m.y = __shfl_xor_sync(0xffffffffu, m.y, s);
-      m.z = __shfl_xor_sync(0xffffffffu, m.z, s);
-      m.w = __shfl_xor_sync(0xffffffffu, m.w, s);
-      if (up) v[i] = m;
-      else v[i | s] = m;
-    }
-  }
-}
-
 __global__ void __launch_bounds__(kDqThreads, 1)
     dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
               const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_g,
@@ -276,7 +255,7 @@ __global__ void __launch_bounds__(kDqThreads, 1)
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     return mbar_wait(smem_u32(bar), parity, abort_flag, a.status, a.wait_limit_ns);
   };
-  // Register split of the launch's 512 x 128: 128 x 48 + 256 x 192 + 128 x 80.
+  // Register split of the launch's 512 x 128: 128 x 48 + 256 x 176 + 128 x 112.
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
     if (warp == 0 && lane == 0) {
@@ -434,7 +413,7 @@ __global__ void __launch_bounds__(kDqThreads, 1)
       tc_commit_w(smem_u32(&bars->done));
     }
   } else if (warp < 12) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
     // one outcome a warp: the TMEM accesses need its lanes together
     auto wait_w = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
     const int w = (warp - 4) >> 2, q = warp & 3, r = 32 * q + lane;
@@ -489,48 +468,41 @@ __global__ void __launch_bounds__(kDqThreads, 1)
       }
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
     auto wait_w = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
     const int q = warp & 3;
     int un = 0;
     for (int u = blockIdx.x; u < units; u += gridDim.x) {
       const DqUnit x(a, bars->lens, u);
-      // rows 8 (lane / 8) + i of this warp's 32, 16 bytes of each half row a lane
-      const int t1 = x.t0 + 32 * q + 8 * (lane >> 3);
-      uint16_t* go = a.dq.at(x.b, t1, x.h) + 8 * (lane & 7);
+      const int t = x.t0 + 32 * q + lane;
+      uint16_t* go = a.dq.at(x.b, t, x.h);
+      // all of dq comes out before anything else is done with it: the next
+      // unit's first product into it waits, and behind that product its dP
+      // (out by halves: 348 us at 15,731 x 56 rows and 332 keys against 280)
+      uint32_t k[64];
       if (x.n > 0) {
         if (!wait_w(&bars->dq_full, un & 1)) break;
         ++un;
         tc_fence_after();
-      }
-#pragma unroll 1
-      for (int w = 0; w < 2; ++w) {
-        uint4 k[8];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          uint32_t v[16];
-          if (x.n > 0) {
-            H3_TMEM_LD16(tmem + ((uint32_t)(32 * q) << 16) + 64 * w + 16 * c, v);
-            tmem_wait_ld();
-          } else {
+          uint32_t v[32];
+          H3_TMEM_LD16(tmem + ((uint32_t)(32 * q) << 16) + 32 * c, (&v[0]));
+          H3_TMEM_LD16(tmem + ((uint32_t)(32 * q) << 16) + 32 * c + 16, (&v[16]));
+          tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] = 0u;
-          }
-          const auto two = [&](int i) {
-            return pack_bf16(__uint_as_float(v[i]) * a.scale, __uint_as_float(v[i + 1]) * a.scale);
-          };
-          k[2 * c] = make_uint4(two(0), two(2), two(4), two(6));
-          k[2 * c + 1] = make_uint4(two(8), two(10), two(12), two(14));
+          for (int i = 0; i < 16; ++i)
+            k[16 * c + i] = pack_bf16(__uint_as_float(v[2 * i]) * a.scale, __uint_as_float(v[2 * i + 1]) * a.scale);
         }
-        if (w == 1 && x.n > 0) {
-          tc_fence_before();
-          mbar_arrive(smem_u32(&bars->dq_empty));
-        }
-        transpose8(k);
+        tc_fence_before();
+        mbar_arrive(smem_u32(&bars->dq_empty));
+      } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (t1 + i < a.n.q_len) *reinterpret_cast<uint4*>(go + 64 * w + i * a.dq.t) = k[i];
+        for (int i = 0; i < 64; ++i) k[i] = 0u;
       }
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        if (t < a.n.q_len) store32(go + 16 * c, &k[8 * c]);
     }
   }
   release_tmem(warp, tmem, abort_flag, &bars->done);
