@@ -136,7 +136,9 @@ __device__ __forceinline__ float dot8(const uint4& x, const uint4& y) {
 // queries (0 and -inf there, so that P is 0).  HBM-bound: 512 bytes a row.
 // 16 lanes take a row; a CTA has 16 tokens of kHeads heads, a group its
 // token's heads one after the other (neighbours in memory), all in flight.
-constexpr int kHeads = 8;
+// 1.3 million rows of 512 bytes: 109 us, 6.2 TB/s (8 heads a CTA, at half the
+// occupancy: 134).
+constexpr int kHeads = 4;
 
 __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ BwdArgs a) {
   const int c = threadIdx.x & 15, tok = blockIdx.x * 16 + (threadIdx.x >> 4);
@@ -177,10 +179,8 @@ __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ BwdA
 // TMEM columns: dq 0, S 128, dP 256, dS (two buffers) 384 and 448.  Of block
 // e+1, S and dP run while block e is in the elementwise warps; dq of e
 // follows, so a K tile is held for two blocks and needs the third buffer to
-// be loaded ahead.  Four more warps (12-15) write dq, eight lanes a row (a
-// thread a row, 32 lines an instruction, kept the load/store unit busy for
-// 4,000 cycles a unit), so that the elementwise warps only go from block to
-// block.  Working delta out in here, by either kind of warp, took 5,000 to
+// be loaded ahead.  Four more warps (12-15) take dq out and write it, so that
+// the elementwise warps only go from block to block.  Working delta out in here, by either kind of warp, took 5,000 to
 // 12,000 cycles a unit of three to eight blocks of 2,200: code that runs once
 // a unit waits for its instructions, constants and rows each time.
 struct __align__(16) DqBarriers {
@@ -657,7 +657,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     } else if (warp == 1) {
       // dv(e-1) S(e) dk(e-1) dP(e): the order keeps P^T (dS^T) in place until
-      // its product has read it.  (A second issuer for dk and dP: 7% slower.)
+      // its product has read it.  The elementwise warps wait for dv(e-1) and
+      // S(e) in turn, 1,300 of a block's 3,500 cycles, yet what was tried
+      // against that is slower: P^T through shared memory with S a block ahead
+      // leaves q two buffers (397 us against 292 at 15,731 x 56 rows and 332
+      // keys), a product of N = 64 for either warpgroup reads K and V twice
+      // (341), and a second issuer for dk and dP takes 7% more.
       auto iwait = [&](uint64_t* bar, uint32_t par) -> bool {
         int got = 0;
         if (lane == 0) got = wait(bar, par) ? 1 : 0;
