@@ -141,6 +141,7 @@ __device__ __forceinline__ float dot8(const uint4& x, const uint4& y) {
 constexpr int kHeads = 4;
 
 __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ BwdArgs a) {
+  asm volatile("griddepcontrol.launch_dependents;");
   const int c = threadIdx.x & 15, tok = blockIdx.x * 16 + (threadIdx.x >> 4);
   const bool live = tok < a.n.q_len;
   const int per_b = (a.n.heads + kHeads - 1) / kHeads;
@@ -252,6 +253,9 @@ __global__ void __launch_bounds__(kDqThreads, 1)
   if (threadIdx.x >= 128 && threadIdx.x < 128 + kLens && threadIdx.x - 128 < a.n.batch)
     bars->lens[threadIdx.x - 128] = kv_len_of(a.kv_lens, a.n.kv_len, threadIdx.x - 128);
   const uint32_t tmem = alloc_tmem(warp, &bars->tmem_base);
+  asm volatile("griddepcontrol.launch_dependents;");
+  // placed while the kernel before runs; nothing is read or written before its end
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     return mbar_wait(smem_u32(bar), parity, abort_flag, a.status, a.wait_limit_ns);
   };
@@ -599,6 +603,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   const uint32_t tmem = alloc_tmem(warp, &bars->tmem_base);
+  asm volatile("griddepcontrol.launch_dependents;");
+  // placed while the kernel before runs; nothing is read or written before its end
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     return mbar_wait(smem_u32(bar), parity, abort_flag, a.status, a.wait_limit_ns);
   };
@@ -828,35 +835,36 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // Adds the partial sums of the key tiles that were cut.  Block (x, y): the
 // tile that the start of CTA x + 1's run cuts (if it is the first such start
-// inside the tile), rows 16y..16y+15 of dk and dv.
+// inside the tile), rows 16 (y % 8).. and column groups 16 (y / 8).. of the 64
+// that dk and dv have.  What it costs is latency, so eight sums are in flight
+// (one after the other in a quarter of the threads: 13 us for 20 tiles).
 __global__ void __launch_bounds__(256) dkv_join_kernel(const __grid_constant__ BwdArgs a, int ctas) {
   const int c = blockIdx.x + 1;
   DkvWalk own(a, c, ctas);
   const int64_t start = own.pos, share = DkvWalk(a, 1, ctas).pos;  // share: CTA 1 starts there
-  if (start >= own.end) return;
-  if (!own.next(a) || own.it0 == 0) return;
+  const bool cut = start < own.end && own.next(a) && own.it0 > 0;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (!cut) return;
   const int64_t first = start - own.it0, last = first + own.steps - 1;
   const int c0 = (int)(first / share), c1 = (int)(last / share);
   if (c0 != c - 1) return;  // an earlier start cuts the tile too
-  // 16 rows x 32 column groups x 2 results over 256 threads
-  const int r = blockIdx.y * 16 + (threadIdx.x & 15), key = own.tile * 128 + r;
+  const int r = (blockIdx.y & 7) * 16 + (threadIdx.x & 15), key = own.tile * 128 + r;
   if (key >= a.n.kv_len) return;
-  for (int k = threadIdx.x >> 4; k < 64; k += 16) {
-    const int which = k >> 5, cg = k & 31;
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i = c0; i <= c1; ++i) {
-      const float4 v = reinterpret_cast<const float4*>(
-          a.part + (((int64_t)i * 2 + (i == c0 ? 1 : 0)) * 2 + which) * 16384)[cg * 128 + r];
-      sum.x += v.x;
-      sum.y += v.y;
-      sum.z += v.z;
-      sum.w += v.w;
-    }
-    const float f = which ? 1.0f : a.scale;
-    uint2 o = make_uint2(pack_bf16(sum.x * f, sum.y * f), pack_bf16(sum.z * f, sum.w * f));
-    if (key >= own.len) o = make_uint2(0, 0);
-    *reinterpret_cast<uint2*>((which ? a.dv : a.dk).at(own.b, key, own.hk) + 4 * cg) = o;
+  const int k = (blockIdx.y >> 3) * 16 + (threadIdx.x >> 4), which = k >> 5, cg = k & 31;
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int i = c0; i <= c1; ++i) {
+    const float4 v = reinterpret_cast<const float4*>(
+        a.part + (((int64_t)i * 2 + (i == c0 ? 1 : 0)) * 2 + which) * 16384)[cg * 128 + r];
+    sum.x += v.x;
+    sum.y += v.y;
+    sum.z += v.z;
+    sum.w += v.w;
   }
+  const float f = which ? 1.0f : a.scale;
+  uint2 o = make_uint2(pack_bf16(sum.x * f, sum.y * f), pack_bf16(sum.z * f, sum.w * f));
+  if (key >= own.len) o = make_uint2(0, 0);
+  *reinterpret_cast<uint2*>((which ? a.dv : a.dk).at(own.b, key, own.hk) + 4 * cg) = o;
 }
 
 __global__ void __launch_bounds__(256) zero_kv_kernel(CrossShape n, Rows dk, Rows dv) {
@@ -894,6 +902,23 @@ cudaError_t prepare(K* kernel, int smem, int regs, std::once_flag* once, cudaErr
     result[dev] = r;
   });
   return result[dev];
+}
+
+// A launch that may be placed before the kernel before it ends; the kernel
+// waits for that itself (griddepcontrol.wait) before it reads its results.
+template <typename... P, typename... A>
+cudaError_t launch_after(void (*kernel)(P...), dim3 grid, int threads, int smem, cudaStream_t s, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 }  // namespace
@@ -943,11 +968,14 @@ cudaError_t launch_cross_bwd(const CrossLaunch& L, cudaStream_t s, std::string* 
   const int units = n.batch * n.heads * a.q_blocks;
   const int ctas = n.kv_len ? dkv_ctas(n) : 0;
   const int groups = (n.heads + kHeads - 1) / kHeads * n.batch;
-  if (ctas) delta_kernel<<<dim3(a.q_blocks * 8, groups < 65535 ? groups : 65535), 256, 0, s>>>(a);
-  dq_kernel<<<units < kSms ? units : kSms, kDqThreads, kDqSmem, s>>>(mq, mk, mv, mg, a, units);
-  if (ctas) dkv_kernel<<<ctas, kThreads, kDkvSmem, s>>>(mq, mk, mv, mg, a);
-  if (ctas > 1) dkv_join_kernel<<<dim3(ctas - 1, 8), 256, 0, s>>>(a, ctas);
-  return cudaGetLastError();
+  if (ctas) {
+    delta_kernel<<<dim3(a.q_blocks * 8, groups < 65535 ? groups : 65535), 256, 0, s>>>(a);
+    e = cudaGetLastError();
+  }
+  if (e == cudaSuccess) e = launch_after(dq_kernel, units < kSms ? units : kSms, kDqThreads, kDqSmem, s, mq, mk, mv, mg, a, units);
+  if (ctas && e == cudaSuccess) e = launch_after(dkv_kernel, ctas, kThreads, kDkvSmem, s, mq, mk, mv, mg, a);
+  if (ctas > 1 && e == cudaSuccess) e = launch_after(dkv_join_kernel, dim3(ctas - 1, 32), 256, 0, s, a, ctas);
+  return e;
 }
 
 }  // namespace h3

@@ -327,3 +327,19 @@ def sdpa(q, k, v, head_dim: int, backend: Optional[H3AttentionBackend] = None,
             return torch.stack([x.transpose(0, 1).reshape(q.shape[1], -1) for x in outs])
         o = SDPABackend().attend(qh, kh, vh, scale, None, None)
     return o.transpose(0, 1).reshape(q.shape[0], q.shape[1] * head_dim)
+
+
+def cross_sdpa(q, k, v, head_dim: int, kv_lens=None):
+    """``sdpa`` for keys of another sequence: ``q`` ``[S, H, D]`` or
+    ``[B, S, H, D]``, ``k`` and ``v`` ``[N, Hk, D]`` (with ``q``'s batch axis;
+    H a multiple of Hk), bf16 in, ``[S, H*D]`` (``[B, S, H*D]``) out.
+    ``kv_lens`` (int32 ``[B]`` on the device) counts each member's valid keys;
+    a member without any gives zeros."""
+    import torch
+
+    if not isinstance(q, torch.Tensor) or not q.is_cuda:
+        raise ValueError("q must be a CUDA tensor")
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    Runtime.get(q.device.index).cross_attn_fwd(q=q, k=k, v=v, out=out, scale=1.0 / float(head_dim) ** 0.5,
+                                               kv_lens=kv_lens)
+    return out.flatten(-2)

@@ -229,3 +229,13 @@ def test_python_refuses_host_tensors_and_types(lib):
     for op in (0, 1, 2):
         assert _cross_workspace(op, 2, 5, 7, 3, 4, 2) == _ask(lib, a, op)[1]
     assert _norm_workspace() == _ask(lib, _norm(lib), 1)[1] > 0
+
+
+def test_cross_sdpa_refuses_host_tensors():
+    import torch
+
+    from h3attention import cross_sdpa
+
+    x = torch.zeros(3, 2, 128, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="must be a CUDA tensor"):
+        cross_sdpa(x, x, x, 128)

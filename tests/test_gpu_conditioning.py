@@ -382,6 +382,9 @@ NORM = [
     (1, 100, 50, 3, 3, 48, 64, False), (3, 17, 20, 4, 2, None, 33, True), (2, 9, 40, 2, 1, 1, 8, True),
     (1, 1000, 77, 40, 8, 46, None, False), (1, 0, 5, 2, 1, 64, 64, False), (2, 5, 0, 2, 1, None, None, False),
     (0, 5, 5, 2, 1, 64, 64, False), (1, 700, 3, 14, 14, 64, 64, True),
+    # runs of 2, 4 and 8 rows a group that end inside tokens, members and the operand
+    (3, 6001, 600, 5, 1, 64, 40, False), (20001, 1, 2, 1, 1, 64, 64, True), (2, 40001, 3, 1, 1, 48, None, False),
+    (2, 9001, 5003, 5, 3, 33, None, False),
 ]
 
 
@@ -482,6 +485,21 @@ def _layer_state(seed, B=2, S=300, N=150, H=4, Hk=2):
     for n, like in (("qn", q), ("out", q), ("dqn", q), ("dq", q), ("kn", k), ("dkn", k), ("dk", k), ("dv", v)):
         st[n] = torch.empty_like(like)
     return st
+
+
+@pytest.mark.parametrize("batch", [None, 2])
+def test_cross_sdpa_is_the_call(gpu, batch):
+    import torch
+
+    from h3attention import cross_sdpa
+
+    q, k, v, _ = _inputs(batch or 1, 140, 50, 4, 2, 60)
+    lens = _lens_tensor([17] * (batch or 1))
+    want = torch.empty_like(q)
+    _rt().cross_attn_fwd(q=q, k=k, v=v, out=want, scale=SCALE, kv_lens=lens)
+    if batch is None:
+        q, k, v, want = q[0], k[0], v[0], want[0]
+    assert torch.equal(cross_sdpa(q, k, v, D, kv_lens=lens), want.flatten(-2))
 
 
 def test_layer_of_norm_and_cross_attention_has_the_gradients_of_the_whole(gpu):
