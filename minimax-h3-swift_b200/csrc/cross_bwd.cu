@@ -189,7 +189,7 @@ struct __align__(16) DqBarriers {
   uint64_t q_full, q_empty, g_full, g_empty;
   uint64_t k_full[3], k_empty[3], v_full[2], v_empty[2];
   uint64_t n_full[2];                // -lse2 and delta of unit u on [u & 1]
-  uint64_t s_full, s_empty, dp_full, dp_empty, dq_full, dq_empty, done;
+  uint64_t s_full, s_empty, dp_full, dp_empty, dq_full, dq_empty, sum_full[2], done;
   // block e on [e & 1]: S and dP of e + 1 are issued before the issuer waits
   // for dS of e, so one barrier could complete twice before that wait
   uint64_t ds_full[2];
@@ -235,6 +235,7 @@ __global__ void __launch_bounds__(kDqThreads, 1)
       mbar_init(smem_u32(&bars->v_empty[i]), 1);
       mbar_init(smem_u32(&bars->ds_full[i]), 256);
       mbar_init(smem_u32(&bars->n_full[i]), 1);
+      mbar_init(smem_u32(&bars->sum_full[i]), 128);
     }
     mbar_init(smem_u32(&bars->q_full), 1);
     mbar_init(smem_u32(&bars->q_empty), 1);
@@ -423,13 +424,15 @@ __global__ void __launch_bounds__(kDqThreads, 1)
     const int w = (warp - 4) >> 2, q = warp & 3, r = 32 * q + lane;
     const uint32_t lane_base = tmem + ((uint32_t)(32 * q) << 16);
     const uint64_t sl2 = dup2(a.scale * kLog2e);
-    int e = 0, un = 0;
+    int e = 0, un = 0, n1 = 0;  // blocks, units, units of one block
     bool ok = true;
     for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
       const DqUnit x(a, bars->lens, u);
       if (x.n == 0) continue;
       if (!(ok = wait_w(&bars->n_full[un & 1], (un >> 1) & 1))) break;
-      const uint64_t nl2x2 = dup2(bars->nl2[un & 1][r]), ndelta = dup2(-bars->delta[un & 1][r]);
+      const uint64_t nl2x2 = dup2(bars->nl2[un & 1][r]);
+      uint64_t ndelta = 0;
+      if (x.n > 1) ndelta = dup2(-bars->delta[un & 1][r]);
       ++un;
       for (int j = 0; j < x.n; ++j, ++e) {
         if (!(ok = wait_w(&bars->s_full, e & 1))) break;
@@ -449,9 +452,41 @@ __global__ void __launch_bounds__(kDqThreads, 1)
         tc_fence_after();
         uint32_t d[64];
         load64(lane_base + 256 + 64 * w, d);
+        const int valid = x.len - 128 * j - 64 * w;  // this half's
+        if (x.n == 1) {
+          // All keys are here, so delta is sum(P dP) in fp32 and not do.out:
+          // the rounding of out shows in dS where keys are few (with one key
+          // dS is 0: hence also the division by the weights' own sum).  Half 1
+          // hands its sum over in the place of delta, half 0 the whole one in
+          // that of -lse2, which both have read; the places are the unit's
+          // until dp_empty.
+          float own = 0.f, ps = 0.f;
+#pragma unroll
+          for (int c = 0; c < 64; ++c)
+            if (c < valid) {
+              own = fmaf(p[c], __uint_as_float(d[c]), own);
+              ps += p[c];
+            }
+          float *other = &bars->delta[(un - 1) & 1][r], *all = &bars->nl2[(un - 1) & 1][r];
+          if (w == 1) {
+            *other = own;
+            fence_async_shared();
+            mbar_arrive(smem_u32(&bars->sum_full[1]));
+            if (!(ok = wait_w(&bars->sum_full[0], n1 & 1))) break;
+            own = *all;
+          } else {
+            if (!(ok = wait_w(&bars->sum_full[1], n1 & 1))) break;
+            own = x.len > 64 ? own + *other : ps > 0.f ? own / ps : 0.f;
+            *all = own;
+            fence_async_shared();
+            mbar_arrive(smem_u32(&bars->sum_full[0]));
+            a.delta[((int64_t)x.b * a.n.heads + x.h) * a.q_blocks * 128 + x.t0 + r] = own;  // for dkv_kernel
+          }
+          ++n1;
+          ndelta = dup2(-own);
+        }
         tc_fence_before();
         mbar_arrive(smem_u32(&bars->dp_empty));
-        const int valid = x.len - 128 * j - 64 * w;  // this half's
         uint32_t pk[32];
 #pragma unroll
         for (int c = 0; c < 32; ++c) {

@@ -11,6 +11,9 @@ is off by at most u = 2^-8 of the value):
   e = sum |do| (u |out| + u P|v|); dS = P (dp - delta) by P e, and by u |dS|
   as it enters its products in bf16: dq: u |dq| + scale (u |dS| + P e) |k|,
   dk likewise with |q|.
+* Up to 128 keys delta is sum(P dP) / sum(P) in fp32 instead, off by the
+  shares of fp32 below: 2 c each for the weights and the products, of the sum
+  of magnitudes sum P |do||v|.
 * fp32: a logit is a sum of 128 products, off by at most 2^-23 of the sum of
   their magnitudes at each addition: c = 2^-16 max(scale sum |q k|), and a
   weight by that share (2^-20 more for exp2, log2 and the sums).  All terms
@@ -54,7 +57,7 @@ def _assert_within(name, got, want, tol):
     assert worst <= 0, f"{name}: {worst} over the tolerance (max error {(got - want).abs().max().item()})"
 
 
-def _attention(q, k, v, scale, do=None):
+def _attention(q, k, v, scale, do=None, one_block=False):
     """One member in 64 bits: q, do [S, H, D], k, v [N, H, D] (heads already
     repeated).  Values and tolerances, by name."""
     import torch
@@ -81,6 +84,8 @@ def _attention(q, k, v, scale, do=None):
             dp, delta = g @ v.transpose(1, 2), (g * out).sum(-1, keepdim=True)
             ds = p * (dp - delta)
             e = (g.abs() * tol["out"]).sum(-1, keepdim=True)
+            if one_block:
+                e = 4 * c * (p * (g.abs() @ v.abs().transpose(1, 2))).sum(-1, keepdim=True)
             eds = (U + 2 * c) * ds.abs() + p * (e + 2 * c * (g.abs() @ v.abs().transpose(1, 2) + delta.abs()))
             val["dv"], val["dq"], val["dk"] = p.transpose(1, 2) @ g, scale * ds @ k, scale * ds.transpose(1, 2) @ q
             tol["dv"] = U * val["dv"].abs() + (U + 2 * c) * p.transpose(1, 2) @ g.abs() + 1e-30
@@ -89,7 +94,7 @@ def _attention(q, k, v, scale, do=None):
     return val, tol
 
 
-def _check_attention(q, k, v, lens, got, do=None, prefix=None, scale=SCALE):
+def _check_attention(q, k, v, lens, got, do=None, prefix=None, scale=SCALE, one_block=False):
     """Compares got (out, lse and gradients, [B, S, H, D] and [B, H, S]) member by member."""
     import torch
 
@@ -99,7 +104,7 @@ def _check_attention(q, k, v, lens, got, do=None, prefix=None, scale=SCALE):
         if prefix is not None:
             kk, vv = torch.cat([prefix[0], kk]), torch.cat([prefix[1], vv])
         kk, vv = kk.repeat_interleave(group, 1), vv.repeat_interleave(group, 1)
-        val, tol = _attention(q[b], kk, vv, scale, None if do is None else do[b])
+        val, tol = _attention(q[b], kk, vv, scale, None if do is None else do[b], one_block)
         _assert_within(f"out[{b}]", got["out"][b].transpose(0, 1), val["out"], tol["out"])
         if got.get("lse") is not None:
             if kk.shape[0] == 0:
@@ -267,6 +272,13 @@ def test_cross_long_strides(gpu):
         at().copy_(x)
         got = _run_cross(at() if n == "q" else q, at() if n == "k" else k, at() if n == "v" else v, None, do)
         _check_attention(q, k, v, [S], got, do)
+
+
+def test_cross_gradient_of_few_keys(gpu):
+    """Where keys are few dS is a small difference; with one key it is 0."""
+    lens = [1, 2, 3, 5, 64, 65, 128, 0]
+    q, k, v, do = _inputs(len(lens), 150, 128, 4, 2, 13)
+    _check_attention(q, k, v, lens, _run_cross(q, k, v, lens, do), do, one_block=True)
 
 
 def test_cross_is_deterministic(gpu):
