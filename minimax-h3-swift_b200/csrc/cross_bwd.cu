@@ -3,6 +3,7 @@
 //   P = 2^(scale log2(e) q.k - lse2);  delta_i = do_i.o_i;  dS = P (do v^T - delta)
 //   dq = scale dS k;  dk = scale dS^T q;  dv = P^T do   (sums over the heads of a group)
 //
+// (delta_i = sum_j P_ij dP_ij too, and is taken so up to 128 keys)
 // delta_kernel goes over do and out once; then two passes, so that every sum
 // has one owner and a fixed order (no atomics):
 //   dq_kernel    a CTA holds 128 queries and walks the keys: S, dP, dq += dS K
@@ -13,8 +14,9 @@
 // from TMEM (they never touch shared memory); sums are fp32.
 //
 // Roles of a CTA's 12 warps: 0 TMA producer, 1 MMA issuer, 2 TMEM owner (and
-// a second issuer in dq_kernel), 4-7 and 8-11 elementwise: each warpgroup takes 64 of a tile's 128 columns of
-// every row (thread = row = TMEM lane).  Every wait is bounded (attn_tc.cu).
+// a second issuer in dq_kernel), 4-7 and 8-11 elementwise: each warpgroup takes
+// 64 of a tile's 128 columns of every row (thread = row = TMEM lane).  Every
+// wait is bounded (attn_tc.cu).
 //
 // dkv_kernel's work, all (key tile, query block) pairs in a row, is cut into
 // equal runs, one a CTA; a key tile that is cut leaves fp32 partial sums that
@@ -183,7 +185,10 @@ __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ BwdA
 // be loaded ahead.  Four more warps (12-15) take dq out and write it, so that
 // the elementwise warps only go from block to block.  Working delta out in here, by either kind of warp, took 5,000 to
 // 12,000 cycles a unit of three to eight blocks of 2,200: code that runs once
-// a unit waits for its instructions, constants and rows each time.
+// a unit waits for its instructions, constants and rows each time.  15,731 x
+// 56 rows and 332 keys: 265-285 us; 2 x 16,384 x 40 and 1,024 ragged keys:
+// 705, 2,200 cycles a block (its products 1,536, the exponentials of a tile
+// 1,024 of the MUFU units between two TMEM round trips).
 struct __align__(16) DqBarriers {
   float nl2[2][128], delta[2][128];  // by unit parity
   uint64_t q_full, q_empty, g_full, g_empty;
@@ -551,8 +556,10 @@ __global__ void __launch_bounds__(kDqThreads, 1)
 // Shared memory: K and V of the unit, three q and two do tiles (224 KB), -lse2
 // and delta of two query blocks.  TMEM columns: dk 0, dv 128, S^T 256, dP^T
 // 384; a warpgroup writes its half of P^T (dS^T) over its own half of S^T
-// (dP^T), so neither waits for the other's loads.  A q tile is held from S(e) to dk(e), over one block's time
-// and a half, so it needs the third buffer to be loaded ahead.
+// (dP^T), so neither waits for the other's loads.  A q tile is held from S(e)
+// to dk(e), over one block's time and a half, so it needs the third buffer to
+// be loaded ahead.  15,731 x 56 rows and 332 keys: 292 us, 3,500 cycles a
+// block, 2,048 of them in its four products (58% of the tensor pipe's time).
 struct __align__(16) DkvBarriers {
   float nl2[2][128], delta[2][128];
   uint64_t kv_full, kv_empty;

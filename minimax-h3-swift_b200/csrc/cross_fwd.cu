@@ -26,13 +26,23 @@
 // Roles of a CTA's 16 warps: 0 K/V producer (TMA); 1 MMA issuer; 2 owns TMEM;
 // 3 query tiles of dense rows (TMA); 4-7 and 8-11 softmax of half 0 and 1,
 // thread = row = TMEM lane; 12-15 epilogue of both halves and, for folded
-// rows, the gather of the next queries.  TMEM: half t has S (then P, packed bf16, over its first 64
-// columns) at 256t and O at 256t + 128.  K/V entries run through a ring of 2
-// (3 in single mode, where each entry is needed for two steps); the producer
-// hands each entry's flags to the issuer through shared memory.  The next
-// unit's Q and K/V loads, its first S and softmax overlap the epilogue of
-// this one, which with 3-4 key tiles a unit is a third of a unit's time.
+// rows, the gather of the next queries.  TMEM: half t has S (then P, packed
+// bf16, over its first 64 columns) at 256t and O at 256t + 128.  K/V entries
+// run through a ring of 2 (3 in single mode, where each entry is needed for
+// two steps); the producer hands each entry's flags to the issuer through
+// shared memory.  The next unit's Q and K/V loads, its first S and softmax
+// overlap the epilogue of this one, which with 3-4 key tiles a unit is a third
+// of a unit's time.
+//
+// What bounds it: dense, the alternation of each half's products (1,024
+// cycles a key tile) and softmax (2,200, of them 1,024 of the MUFU units), and
+// from 1,024 keys on the power cap (1.4-1.6 GHz): 32,768 x 40 rows against 512
+// keys 345-385 us (0.9-1.0 PFLOP/s), against 4,096 2.45-2.75 ms (1.0-1.1).
+// Below 256 keys the units' turn-over: 128 keys 165 us, 4.1 TB/s.  Single: HBM
+// (64 members of 4,096 keys and 8 key heads: 184 us, 5.8 TB/s), dual: softmax
+// (32 members of 5 rows over 65,536 keys and 512 of their own: 114 us).
 // Every wait is bounded (see attn_tc.cu).
+#include <algorithm>
 #include <climits>
 #include <mutex>
 #include <type_traits>
@@ -44,6 +54,11 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kSms = 148;
+// What a unit of folded rows costs beside its key tiles, in key tiles: its
+// queries and its results pass through one buffer each.  24 members with 64
+// keys of their own over 65,536 shared ones: 151 us without it, 79 with 2, 76
+// with 4; 32 members with 100 over 8,192: 38, 40, 46.
+constexpr int kUnitCost = 2;
 
 enum { kDense = 0, kSingle = 1, kDual = 2 };
 
@@ -53,6 +68,7 @@ struct Source {
   int32_t per;                // row blocks of a key head (prefix), of a member's (key) head (own)
   int32_t units;
   int32_t tiles;              // key tiles of a unit
+  int32_t pitch;              // its places in the linear split: its tiles and its own cost
   int32_t rows;               // rows of a block: 128 or 256
   int32_t tpc;                // key tiles a CTA in the linear split; 0: whole units in turn
   int32_t start;              // first position of its units in that split
@@ -60,7 +76,7 @@ struct Source {
   // [units, slots, 32, stride] groups of four channels, ml as [units, slots,
   // stride], so that a warp's 32 rows are contiguous
   int32_t slots, stride;
-  Div by_per, by_tiles, by_tpc;
+  Div by_per, by_pitch, by_tpc;
 };
 
 struct FwdArgs {
@@ -102,7 +118,7 @@ struct SegIter {
   uint32_t pos, end;          // key tiles of the linear split, or units
   __device__ explicit SegIter(const FwdArgs& a) {
     if (a.tpc) {
-      const uint32_t total = (uint32_t)(a.units_p * a.src[0].tiles + a.units_o * a.src[1].tiles);
+      const uint32_t total = (uint32_t)(a.units_p * a.src[0].pitch + a.units_o * a.src[1].pitch);
       pos = blockIdx.x * a.tpc;
       end = min(total, pos + a.tpc);
     } else {
@@ -111,20 +127,25 @@ struct SegIter {
     }
   }
   __device__ bool next(const FwdArgs& a, const int32_t* lens, Seg& s) {
-    if (pos >= end) return false;
     int j1, tiles;
     s.slot = 0;
     if (a.tpc) {
-      const uint32_t pre = MODE == kDense ? 0 : a.units_p * a.src[0].tiles;
-      s.own = MODE == kDense || pos >= pre;
-      const uint32_t off = s.own ? pos - pre : pos;
-      tiles = a.src[s.own].tiles;
-      s.unit = a.src[s.own].by_tiles(off);
-      s.j0 = (int)off - s.unit * tiles;
-      j1 = min(tiles, s.j0 + (int)(end - pos));
-      s.slot = blockIdx.x - a.src[s.own].by_tpc(pos - s.j0);
-      pos += j1 - s.j0;
+      do {
+        if (pos >= end) return false;
+        const uint32_t pre = MODE == kDense ? 0 : a.units_p * a.src[0].pitch;
+        s.own = MODE == kDense || pos >= pre;
+        const Source& c = a.src[s.own];
+        const uint32_t off = s.own ? pos - pre : pos;
+        tiles = c.tiles;
+        s.unit = c.by_pitch(off);
+        s.j0 = (int)off - s.unit * c.pitch;
+        j1 = min(c.pitch, s.j0 + (int)(end - pos));
+        s.slot = blockIdx.x - c.by_tpc(pos - s.j0);
+        pos += j1 - s.j0;
+      } while (MODE != kDense && s.j0 >= tiles);
+      if (MODE != kDense) j1 = min(j1, tiles);
     } else {
+      if (pos >= end) return false;
       s.own = MODE == kDense || (int)pos >= a.units_p;
       s.unit = (int)pos - (MODE != kDense && s.own ? a.units_p : 0);
       tiles = a.src[s.own].tiles;
@@ -779,7 +800,7 @@ struct Runs {
   int n, stride;
   __device__ Runs(const FwdArgs& a, int own, int unit, int row) {
     const Source& c = a.src[own];
-    const uint32_t first = c.start + (uint32_t)unit * c.tiles;
+    const uint32_t first = c.start + (uint32_t)unit * c.pitch;
     n = c.tpc ? (int)(c.by_tpc(first + c.tiles - 1) - c.by_tpc(first)) + 1 : 1;
     stride = c.stride;
     o = a.part_o[own] + (int64_t)unit * c.slots * 32 * stride + row;
@@ -861,7 +882,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_dense_kernel(const __grid_c
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const Source& c = a.src[1];
   const uint32_t start = (blockIdx.x + 1) * c.tpc;
-  const int u = c.by_tiles(start), j0 = start - u * c.tiles;
+  const int u = c.by_pitch(start), j0 = start - u * c.pitch;
   if (u >= c.units || j0 == 0 || c.by_tpc(start - j0) != blockIdx.x) return;
   const int bh = c.by_per(u), b = a.by_heads(bh), h = bh - b * a.n.heads;
   const int r = blockIdx.y * 32 + (threadIdx.x & 31), t = (u - bh * c.per) * c.rows + r;
@@ -946,11 +967,11 @@ FwdPlan plan_fwd(const CrossShape& n) {
   }
   a.units_p = src[0].units, a.units_o = src[1].units;
   a.two_sources = a.units_p && a.units_o;
-  const int64_t units = (int64_t)a.units_p + a.units_o;
-  const int64_t pre = (int64_t)a.units_p * src[0].tiles, total = pre + (int64_t)a.units_o * src[1].tiles;
-  int64_t longest = 0;
   for (int k = 0; k < 2; ++k)
-    if (src[k].units && src[k].tiles > longest) longest = src[k].tiles;
+    if (src[k].units) src[k].pitch = src[k].tiles + (a.mode == kDense ? 0 : kUnitCost);
+  const int64_t units = (int64_t)a.units_p + a.units_o;
+  const int64_t pre = (int64_t)a.units_p * src[0].pitch, total = pre + (int64_t)a.units_o * src[1].pitch;
+  const int64_t longest = std::max(src[0].pitch, src[1].pitch);
   const int64_t share = (total + kSms - 1) / kSms;
   // whole units in turn cost up to one unit more than the even share; the
   // linear split costs the partial results' traffic and the join, about the
@@ -964,7 +985,7 @@ FwdPlan plan_fwd(const CrossShape& n) {
       src[k].start = k && a.tpc ? (int32_t)pre : 0;
       src[k].slots = a.tpc ? (src[k].tiles - 1) / a.tpc + 2 : 1;
     }
-    src[k].by_per = div(src[k].per), src[k].by_tiles = div(src[k].tiles), src[k].by_tpc = div(src[k].tpc);
+    src[k].by_per = div(src[k].per), src[k].by_pitch = div(src[k].pitch), src[k].by_tpc = div(src[k].tpc);
     if (p.join) p.part_bytes[k] = ((size_t)src[k].units * src[k].slots * src[k].stride * (512 + 8) + 255) / 256 * 256;
   }
   a.by_heads = div(n.heads), a.by_kv_heads = div(n.kv_heads), a.by_group = div(n.group), a.by_q_len = div(n.q_len);
