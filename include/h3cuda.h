@@ -308,7 +308,9 @@ h3c_status h3c_attn_fwd_noalloc_status(void);
  * kept or cleared), so calls on several streams, host threads or captured
  * graphs are independent as long as each has its own workspace and outputs.
  * They are asynchronous on `stream`, allocate nothing and may be captured.
- * Results are deterministic: no sum depends on the order of atomics. */
+ * Results are deterministic: no sum depends on the order of atomics.  A
+ * bounded device wait that gives up is reported by h3c_device_status, as for
+ * h3c_attn_fwd. */
 
 /* A bf16 [batch, tokens, heads, 128] operand: element (b, s, h, d) sits at
  * ptr[b * batch_stride + s * token_stride + h * head_stride + d].  A stride of

@@ -42,16 +42,22 @@ _NORM = struct.Struct("@" + "Pqqq" * 4 + "6i" + "4P" + "qq" + "iifi" + "Pqqq" * 
 _NO_ROWS = (0, 0, 0, 0)
 
 
-def _rows(name, t, hsd: bool, device: int, want=None):
-    """``((pointer, batch, token and head stride), (batch, tokens, heads))``
-    of a bf16 tensor on ``device``: [B, S, H, 128] or [S, H, 128], with
-    ``hsd`` [B, H, S, 128] or [H, S, 128].  ``want``: the (batch, tokens,
-    heads) it must have."""
+def _kind(t):
+    """What a check of a tensor goes by."""
+    return t.shape, t.stride(), t.dtype, t.get_device()
+
+
+def _axes(name, kind, hsd: bool, device: int, want=None):
+    """``((batch, token and head stride), (batch, tokens, heads))`` of a bf16
+    tensor on ``device``: [B, S, H, 128] or [S, H, 128], with ``hsd``
+    [B, H, S, 128] or [H, S, 128].  ``want``: the (batch, tokens, heads) it
+    must have."""
     import torch
 
-    if t.dtype is not torch.bfloat16 or t.get_device() != device:
-        raise ValueError(f"{name} must be bfloat16 on cuda:{device}, got {t.dtype} on {t.device}")
-    size, stride = t.shape, t.stride()
+    size, stride, dtype, where = kind
+    if dtype is not torch.bfloat16 or where != device:
+        raise ValueError(f"{name} must be bfloat16 on cuda:{device}, got {dtype} on "
+                         f"{'the host' if where < 0 else f'cuda:{where}'}")
     if len(size) == 4:
         (b, s, h, d), (sb, ss, sh, sd) = size, stride
     elif len(size) == 3:
@@ -66,7 +72,51 @@ def _rows(name, t, hsd: bool, device: int, want=None):
         raise _lib.H3CError(_lib.H3C_ERR_UNSUPPORTED, f"{name}: head_dim must be 128, got {d}")
     if want is not None and (b, s, h) != want:
         raise ValueError(f"{name} must have {want} (batch, tokens, heads), got {(b, s, h)}")
-    return (t.data_ptr(), sb, ss, sh), (b, s, h)
+    return (sb, ss, sh), (b, s, h)
+
+
+# The checks of a call's operands and what follows from their shapes, strides,
+# types and device alone: a program makes the same call again and again, and
+# going through them took 3 of its 8 us in Python.
+@functools.lru_cache(maxsize=4096)
+def _cross_form(op, hsd, device, q, out, k, v, prefix, grads):
+    """Strides and sizes of a call, in the order of its arguments."""
+    aq, mine = _axes("q", q, hsd, device)
+    ao, _ = _axes("out", out, hsd, device, mine)
+    ak, keys = _axes("k", k, hsd, device)
+    av, _ = _axes("v", v, hsd, device, keys)
+    (B, S, H), (_, N, Hk) = mine, keys
+    if keys[0] != B:
+        raise ValueError(f"k must have the {B} members of q, got {keys[0]}")
+    P, ap = 0, ((0, 0), (0, 0))
+    if prefix is not None:
+        if len(prefix[0][0]) != 3 or len(prefix[1][0]) != 3:
+            raise ValueError("prefix_k and prefix_v have no batch axis")
+        (_, pks, pkh), (_, P, ph) = _axes("prefix_k", prefix[0], hsd, device)
+        (_, pvs, pvh), _ = _axes("prefix_v", prefix[1], hsd, device, (1, P, ph))
+        if ph != Hk:
+            raise ValueError(f"prefix_k must have the {Hk} heads of k, got {ph}")
+        ap = ((pks, pkh), (pvs, pvh))
+    ag = ((0, 0, 0),) * 4
+    if grads is not None:
+        ag = tuple(_axes(n, g, hsd, device, w)[0]
+                   for n, g, w in zip(("out_grad", "dq", "dk", "dv"), grads, (mine, mine, keys, keys)))
+    return aq, ao, ak, av, ap, ag, (B, S, N, H, Hk, 128), P, _cross_workspace(op, B, S, N, P, H, Hk)
+
+
+@functools.lru_cache(maxsize=4096)
+def _norm_form(hsd, device, q, k, yq, yk, grads):
+    aq, mine = _axes("q", q, hsd, device)
+    ak, keys = _axes("k", k, hsd, device)
+    if keys[0] != mine[0]:
+        raise ValueError(f"k must have the {mine[0]} members of q, got {keys[0]}")
+    names = ("q_out", "k_out") if grads is None else ("dq", "dk")
+    ayq, _ = _axes(names[0], yq, hsd, device, mine)
+    ayk, _ = _axes(names[1], yk, hsd, device, keys)
+    ag = None
+    if grads is not None:
+        ag = _axes("q_grad", grads[0], hsd, device, mine)[0], _axes("k_grad", grads[1], hsd, device, keys)[0]
+    return aq, ak, ayq, ayk, ag, (mine[0], mine[1], keys[1], mine[2], keys[2], 128)
 
 
 def _vector(name, t, dtype, shape, device: int) -> int:
@@ -234,53 +284,45 @@ class Runtime:
         import torch
 
         if stream is None:
-            return torch.empty(size, dtype=torch.uint8, device=self._torch_device())
+            return torch.empty(size, dtype=torch.uint8, device=self._torch_device)
         with torch.cuda.stream(stream):
-            return torch.empty(size, dtype=torch.uint8, device=self._torch_device())
+            return torch.empty(size, dtype=torch.uint8, device=self._torch_device)
 
+    @functools.cached_property
     def _torch_device(self):
         import torch
 
         return torch.device("cuda", self.device)
 
-    def _raw_stream(self, stream):
+    def _launch(self, call, args, stream):
+        """A conditioning call on ``stream`` (None: the device's current one,
+        asked for by its handle alone: a Stream object takes 1.3 us to make)."""
         import torch
 
-        return (torch.cuda.current_stream(self.device) if stream is None else stream).cuda_stream or None
+        status = call(self.ctx, args, torch._C._cuda_getCurrentRawStream(self.device) if stream is None
+                      else stream.cuda_stream)
+        if status:
+            self._check(status)
 
     def _cross(self, op, call, q, k, v, out, layout, scale, kv_lens, lse, stream, prefix=None, grads=None):
         import torch
 
-        hsd, dev = _hsd(layout), self.device
-        vq, mine = _rows("q", q, hsd, dev)
-        vo, _ = _rows("out", out, hsd, dev, mine)
-        B, S, H = mine
-        vk, keys = _rows("k", k, hsd, dev)
-        vv, _ = _rows("v", v, hsd, dev, keys)
-        if keys[0] != B:
-            raise ValueError(f"k must have the {B} members of q, got {keys[0]}")
-        Hk = keys[2]
-        P, vp = 0, (0, 0, 0, 0, 0, 0)
-        if prefix is not None:
-            if prefix[0].dim() != 3 or prefix[1].dim() != 3:
-                raise ValueError("prefix_k and prefix_v have no batch axis")
-            (pk, _, pks, pkh), (_, P, ph) = _rows("prefix_k", prefix[0], hsd, dev)
-            (pv, _, pvs, pvh), _ = _rows("prefix_v", prefix[1], hsd, dev, (1, P, ph))
-            if ph != Hk:
-                raise ValueError(f"prefix_k must have the {Hk} heads of k, got {ph}")
-            vp = (pk, pks, pkh, pv, pvs, pvh)
-        vg = (_NO_ROWS,) * 4
-        if grads is not None:
-            vg = (_rows("out_grad", grads[0], hsd, dev, mine)[0], _rows("dq", grads[1], hsd, dev, mine)[0],
-                  _rows("dk", grads[2], hsd, dev, keys)[0], _rows("dv", grads[3], hsd, dev, keys)[0])
+        dev = self.device
+        aq, ao, ak, av, (apk, apv), ag, sizes, P, size = _cross_form(
+            op, _hsd(layout), dev, _kind(q), _kind(out), _kind(k), _kind(v),
+            None if prefix is None else (_kind(prefix[0]), _kind(prefix[1])),
+            None if grads is None else tuple(_kind(g) for g in grads))
+        B, S, H = sizes[0], sizes[1], sizes[3]
         lens = 0 if kv_lens is None else _vector("kv_lens", kv_lens, torch.int32, (B,), dev)
         plse = 0 if lse is None else _vector("lse", lse, torch.float32, (B, H, S) if lse.dim() == 3 or B > 1 else (H, S),
                                              dev)
-        size = _cross_workspace(op, B, S, keys[1], P, H, Hk)
         ws = self._workspace(size, stream) if size else None
-        args = _CROSS.pack(*vq, *vo, *vk, *vv, B, S, keys[1], H, Hk, 128, scale, lens, plse, *vp, P, 0, *vg[0], *vg[1],
-                           *vg[2], *vg[3], ws.data_ptr() if size else 0, size)
-        self._check(call(self.ctx, args, self._raw_stream(stream)))
+        pk, pv = (0, 0) if prefix is None else (prefix[0].data_ptr(), prefix[1].data_ptr())
+        g0, g1, g2, g3 = (0, 0, 0, 0) if grads is None else (g.data_ptr() for g in grads)
+        args = _CROSS.pack(q.data_ptr(), *aq, out.data_ptr(), *ao, k.data_ptr(), *ak, v.data_ptr(), *av, *sizes, scale,
+                           lens, plse, pk, *apk, pv, *apv, P, 0, g0, *ag[0], g1, *ag[1], g2, *ag[2], g3, *ag[3],
+                           ws.data_ptr() if size else 0, size)
+        self._launch(call, args, stream)
 
     def cross_attn_fwd(self, *, q, k, v, out, scale, layout="SHD", kv_lens=None, lse=None, stream=None):
         """``out = softmax(scale q k^T) v`` against encoder states of another
@@ -325,34 +367,28 @@ class Runtime:
     def _norm(self, call, q, k, outs, q_norm, k_norm, eps, q_rope, k_rope, layout, stream, grads=None):
         import torch
 
-        hsd, dev = _hsd(layout), self.device
-        vq, mine = _rows("q", q, hsd, dev)
-        vk, keys = _rows("k", k, hsd, dev)
-        B, S, H = mine
-        if keys[0] != B:
-            raise ValueError(f"k must have the {B} members of q, got {keys[0]}")
+        dev = self.device
+        yq, yk = outs if grads is None else grads[2:4]
+        aq, ak, ayq, ayk, ag, sizes = _norm_form(
+            _hsd(layout), dev, _kind(q), _kind(k), _kind(yq), _kind(yk),
+            None if grads is None else (_kind(grads[0]), _kind(grads[1])))
+        B, S, N = sizes[:3]
         wq = _vector("q_norm", q_norm, torch.bfloat16, (128,), dev)
         wk = _vector("k_norm", k_norm, torch.bfloat16, (128,), dev)
         tq, hq, bq = self._rope_rows("q_rope", q_rope, B, S)
-        tk, hk, bk = self._rope_rows("k_rope", k_rope, B, keys[1])
-        size, ws, back, dw = 0, None, (_NO_ROWS,) * 4, (0, 0)
-        if grads is None:
-            names, given = ("q_out", "k_out"), outs
-        else:
-            names, given = ("dq", "dk"), grads[2:4]
+        tk, hk, bk = self._rope_rows("k_rope", k_rope, B, N)
+        yq, yk = (yq.data_ptr(), *ayq), (yk.data_ptr(), *ayk)
+        size, ws, fwd, back, dw = 0, None, (yq, yk), (_NO_ROWS,) * 4, (0, 0)
+        if grads is not None:
             size = _norm_workspace()
             ws = self._workspace(size, stream)
             dw = (_vector("dq_norm", grads[4], torch.float32, (128,), dev),
                   _vector("dk_norm", grads[5], torch.float32, (128,), dev))
-        yq, _ = _rows(names[0], given[0], hsd, dev, mine)
-        yk, _ = _rows(names[1], given[1], hsd, dev, keys)
-        fwd = (yq, yk)
-        if grads is not None:
-            back = (_rows("q_grad", grads[0], hsd, dev, mine)[0], yq, _rows("k_grad", grads[1], hsd, dev, keys)[0], yk)
             fwd = (_NO_ROWS, _NO_ROWS)
-        args = _NORM.pack(*vq, *fwd[0], *vk, *fwd[1], B, S, keys[1], H, keys[2], 128, wq, wk, tq, tk, bq, bk, hq, hk, eps,
-                          0, *back[0], *back[1], *back[2], *back[3], *dw, ws.data_ptr() if size else 0, size)
-        self._check(call(self.ctx, args, self._raw_stream(stream)))
+            back = (grads[0].data_ptr(), *ag[0]), yq, (grads[1].data_ptr(), *ag[1]), yk
+        args = _NORM.pack(q.data_ptr(), *aq, *fwd[0], k.data_ptr(), *ak, *fwd[1], *sizes, wq, wk, tq, tk, bq, bk, hq, hk,
+                          eps, 0, *back[0], *back[1], *back[2], *back[3], *dw, ws.data_ptr() if size else 0, size)
+        self._launch(call, args, stream)
 
     def qk_norm_rope_fwd(self, *, q, k, q_out, k_out, q_norm, k_norm, eps=1e-6, q_rope=None, k_rope=None,
                          layout="SHD", stream=None):

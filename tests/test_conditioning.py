@@ -219,10 +219,10 @@ def test_python_refuses_host_tensors_and_types(lib):
     """The tensor checks of the Python calls run before the library is entered."""
     import torch
 
-    from h3attention.runtime import _cross_workspace, _norm_workspace, _rows, _vector
+    from h3attention.runtime import _axes, _cross_workspace, _kind, _norm_workspace, _vector
 
     with pytest.raises(ValueError, match="must be bfloat16 on cuda:0"):
-        _rows("q", torch.zeros(2, 3, 128, dtype=torch.bfloat16), False, 0)
+        _axes("q", _kind(torch.zeros(2, 3, 128, dtype=torch.bfloat16)), False, 0)
     with pytest.raises(ValueError, match="must be a contiguous"):
         _vector("kv_lens", torch.zeros(2, dtype=torch.int64), torch.int32, (2,), 0)
     a = _cross(lib)
