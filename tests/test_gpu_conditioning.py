@@ -428,6 +428,36 @@ def test_norm_matches_64_bits(gpu, B, S, N, H, Hk, hq, hk, each, layout):
             _assert_within(n + " " + name, got, val[name], tol[name])
 
 
+def test_norm_gradient_against_differences(gpu):
+    """The gradients' products with a direction against central differences of
+    the plain loss in 64 bits: a second statement of the formula."""
+    import torch
+
+    g = _gen(35)
+    x, grad = _normal(g, 2, 30, 3, D), _normal(g, 2, 30, 3, D)
+    w, tab = _normal(g, D, mean=1.0, std=0.5), _rope(30, 48, 36)
+    dx, dk = torch.empty_like(x), torch.empty_like(x)
+    dw, dwk = torch.empty(D, device="cuda"), torch.empty(D, device="cuda")
+    _rt().qk_norm_rope_bwd(q=x, k=x, q_grad=grad, k_grad=grad, dq=dx, dk=dk, q_norm=w, k_norm=w, dq_norm=dw,
+                           dk_norm=dwk, eps=1e-5, q_rope=tab)
+    t = tab.double()[None, :, None]
+
+    def loss(x, w):
+        n = x * torch.rsqrt(x.square().mean(-1, keepdim=True) + 1e-5) * w
+        a, b, rest = n[..., :48], n[..., 48:96], n[..., 96:]
+        y = torch.cat([t[..., 0] * a + t[..., 1] * b, t[..., 2] * a + t[..., 3] * b, rest], -1)
+        return (y * grad.double()).sum()
+
+    at, h = [x.double(), w.double()], 1e-4
+    for i, got in enumerate((dx, dw)):
+        d = torch.randn_like(at[i])
+        up, down = ([v + s * h * d if j == i else v for j, v in enumerate(at)] for s in (1, -1))
+        want = ((loss(*up) - loss(*down)) / (2 * h)).item()
+        have = (got.double() * d).sum().item()
+        # every element is off by a rounding (u = 2^-8) of its own size, with signs that do not agree
+        assert abs(have - want) <= 8 * U * (got.double() * d).norm().item() + 1e-4 * abs(want), i
+
+
 def test_norm_in_place_and_strided(gpu):
     """Queries and keys as slices of one packed projection, normalised in place; gradients likewise."""
     import torch
