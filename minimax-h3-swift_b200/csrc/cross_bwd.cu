@@ -646,8 +646,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   const uint32_t tmem = alloc_tmem(warp, &bars->tmem_base);
   asm volatile("griddepcontrol.launch_dependents;");
-  // placed while the kernel before runs; nothing is read or written before its end
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // Placed while the kernel before runs.  What that one writes (-lse2, delta)
+  // is read, and anything written, after its end: the producer waits for it
+  // behind the first loads of inputs, the others here (38.6 us for 41.3 in a
+  // step of 3 x 257 x 8 rows; the same in dq_kernel cost the clip 2%).
+  if (warp >= 2) asm volatile("griddepcontrol.wait;" ::: "memory");
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     return mbar_wait(smem_u32(bar), parity, abort_flag, a.status, a.wait_limit_ns);
   };
@@ -684,6 +687,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           mbar_expect_tx(bar, kTileBytes + 1024);
           tma_tile(smem_u32(sG + i * kTileBytes), &tm_g, bar, 128 * qb, h * a.g_h, seg.b * a.g_b);
           const int64_t pad = (((int64_t)seg.b * a.n.heads + h) * a.q_blocks + qb) * 128;
+          if (ng == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
           bulk_512(smem_u32(bars->nl2[i]), a.nl2 + pad, bar);
           bulk_512(smem_u32(bars->delta[i]), a.delta + pad, bar);
           ++ng;
