@@ -38,9 +38,11 @@
 // cycles a key tile) and softmax (2,200, of them 1,024 of the MUFU units), and
 // from 1,024 keys on the power cap (1.4-1.6 GHz): 32,768 x 40 rows against 512
 // keys 345-385 us (0.9-1.0 PFLOP/s), against 4,096 2.45-2.75 ms (1.0-1.1).
-// Below 256 keys the units' turn-over: 128 keys 165 us, 4.1 TB/s.  Single: HBM
-// (64 members of 4,096 keys and 8 key heads: 184 us, 5.8 TB/s), dual: softmax
-// (32 members of 5 rows over 65,536 keys and 512 of their own: 114 us).
+// Below 256 keys the units' turn-over: 128 keys 160 us, 4.2 TB/s.  Single: HBM
+// (64 members of 4,096 keys and 8 key heads: 180 us, 6.0 TB/s; one token over
+// 65,536 keys: 56 us for 41 at the copy rate, the rest the start, whose code
+// and queries come from HBM behind the first keys, and the join).  Dual: as
+// dense (32 members of 5 rows over 65,536 keys and 512 of their own: 107 us).
 // Every wait is bounded (see attn_tc.cu).
 #include <algorithm>
 #include <climits>
@@ -56,8 +58,9 @@ constexpr int kThreads = 512;
 constexpr int kSms = 148;
 // What a unit of folded rows costs beside its key tiles, in key tiles: its
 // queries and its results pass through one buffer each.  24 members with 64
-// keys of their own over 65,536 shared ones: 151 us without it, 79 with 2, 76
-// with 4; 32 members with 100 over 8,192: 38, 40, 46.
+// keys of their own over 65,536 shared ones: 149 us without it, 75 with 2; 16
+// members of 4 x 14 rows with 300 over 4,000: 40 and 34; 32 members with 512
+// over 65,536: 107 and 111.
 constexpr int kUnitCost = 2;
 
 enum { kDense = 0, kSingle = 1, kDual = 2 };
@@ -285,6 +288,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) {
         SegIter<MODE> it(a);
         Seg s{};
+        [[maybe_unused]] const uint64_t once = evict_first();
         int ec = 0, r = 0, issued = 0;
         uint32_t ph = 0;
         bool ok = true;
@@ -318,17 +322,22 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!SINGLE && dense && i > 0) mbar_arrive(bar);
             mbar_expect_tx(bar, 2 * kTileBytes);
             const uint32_t dk = smem_u32(sKV + 2 * r * kTileBytes), dv = dk + kTileBytes;
+            // both half tiles; of folded rows each key tile is read once (a prefix
+            // of 65,536 keys, 1 row: 56 us, 61 with the tiles kept in L2 like
+            // any other load)
+            auto load = [&](uint32_t dst, const CUtensorMap* map, int tok, int h, int b) {
+#pragma unroll
+              for (int x = 0; x < 2; ++x)
+                if constexpr (dense) tma_load_4d(dst + x * kHalfBytes, map, bar, 64 * x, tok, h, b);
+                else tma_load_4d(dst + x * kHalfBytes, map, bar, 64 * x, tok, h, b, once);
+            };
             if (pre) {
-              tma_load_4d(dk, &tm_pk, bar, 0, 128 * j, s.hk * a.pk_h, 0);
-              tma_load_4d(dk + kHalfBytes, &tm_pk, bar, 64, 128 * j, s.hk * a.pk_h, 0);
-              tma_load_4d(dv, &tm_pv, bar, 0, 128 * j, s.hk * a.pv_h, 0);
-              tma_load_4d(dv + kHalfBytes, &tm_pv, bar, 64, 128 * j, s.hk * a.pv_h, 0);
+              load(dk, &tm_pk, 128 * j, s.hk * a.pk_h, 0);
+              load(dv, &tm_pv, 128 * j, s.hk * a.pv_h, 0);
             } else {
               const int tok = 128 * (j - s.npre);
-              tma_load_4d(dk, &tm_k, bar, 0, tok, s.hk * a.k_h, s.b * a.k_b);
-              tma_load_4d(dk + kHalfBytes, &tm_k, bar, 64, tok, s.hk * a.k_h, s.b * a.k_b);
-              tma_load_4d(dv, &tm_v, bar, 0, tok, s.hk * a.v_h, s.b * a.v_b);
-              tma_load_4d(dv + kHalfBytes, &tm_v, bar, 64, tok, s.hk * a.v_h, s.b * a.v_b);
+              load(dk, &tm_k, tok, s.hk * a.k_h, s.b * a.k_b);
+              load(dv, &tm_v, tok, s.hk * a.v_h, s.b * a.v_b);
             }
             ++issued;
             ++ec;
@@ -462,6 +471,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // latency, not HBM's.
         SegIter<MODE> it(a);
         Seg s{}, following{};
+        const uint64_t once = evict_first();  // (4% at 128-332 keys)
         int qn0 = 0, qn1 = 0, ec = 0;
         bool more = it.next(a, bars->lens, following);
         while (more) {
@@ -478,8 +488,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t bar = smem_u32(&bars->kv_full[ec % L::kRing]);
           auto load = [&](int t) {
             const uint32_t dst = smem_u32(sQ + t * kTileBytes);
-            tma_load_4d(dst, &tm_q, bar, 0, s.row0 + 128 * t, s.h * a.q_h, s.b * a.q_b);
-            tma_load_4d(dst + kHalfBytes, &tm_q, bar, 64, s.row0 + 128 * t, s.h * a.q_h, s.b * a.q_b);
+            tma_load_4d(dst, &tm_q, bar, 0, s.row0 + 128 * t, s.h * a.q_h, s.b * a.q_b, once);
+            tma_load_4d(dst + kHalfBytes, &tm_q, bar, 64, s.row0 + 128 * t, s.h * a.q_h, s.b * a.q_b, once);
           };
           if (!wait(&bars->q_empty[0], (qn0++ & 1) ^ 1)) break;
           mbar_expect_tx(bar, act1 ? 2 * kTileBytes : kTileBytes);
@@ -709,43 +719,47 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     };
     // Folded: the next segment's Q rows, once the last S has read this one's.
-    // 16 lanes take a row, 8 rows a pass of the 128 threads, 8 passes in
-    // flight; rows past the block are zero.  Swizzle: 16-byte chunk c of row r
-    // sits at c ^ (r & 7).
+    // 16 lanes take a row, 8 rows a pass of the 128 threads; rows past the
+    // block are zero.  All passes of both tiles are in flight together, by
+    // asynchronous copies: at the start every SM's first K/V loads queue at HBM,
+    // and four rounds of loads through registers took 13,000 cycles there.
+    // Swizzle: 16-byte chunk c of row r sits at c ^ (r & 7).
     auto gather = [&](const Seg& g, int t, int& qn) {
       if (!wait_w(&bars->q_empty[t], (qn & 1) ^ 1)) return false;
       ++qn;
-      const int c = lane & 15;
-      uint8_t* dst = sQ + t * kTileBytes + (c >> 3) * kHalfBytes;
-#pragma unroll 1
-      for (int r0 = 2 * q + (lane >> 4); r0 < 128; r0 += 64) {
-        uint4 v[8];
-#pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          const int row = g.row0 + 128 * t + r0 + 8 * x;
-          v[x] = make_uint4(0, 0, 0, 0);
-          if (row < g.row_end) {
-            const int tok = a.by_group(row), b = a.by_q_len(tok);
-            v[x] = *reinterpret_cast<const uint4*>(
-                a.q.at(b, tok - b * a.n.q_len, g.hk * a.n.group + (row - tok * a.n.group)) + 8 * c);
-          }
-        }
-#pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          const int r = r0 + 8 * x;
-          *reinterpret_cast<uint4*>(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[x];
-        }
+      const int c = lane & 15, first = 2 * q + (lane >> 4);
+      const uint32_t dst = smem_u32(sQ + t * kTileBytes + (c >> 3) * kHalfBytes) + (((c & 7) ^ (first & 7)) << 4);
+#pragma unroll 4
+      for (int r0 = first; r0 < 128; r0 += 8) {
+        const int row = g.row0 + 128 * t + r0;
+        const bool in = row < g.row_end;
+        const int tok = a.by_group(in ? row : g.row0), b = a.by_q_len(tok);
+        copy16_or_zero(dst + r0 * 128,
+                       a.q.at(b, tok - b * a.n.q_len, g.hk * a.n.group + ((in ? row : g.row0) - tok * a.n.group)) + 8 * c,
+                       in);
       }
-      fence_async_shared();
-      mbar_arrive(smem_u32(&bars->q_full[t]));
+      copies_commit();
       return true;
     };
     int qn0 = 0, qn1 = 0;
     auto gather_next = [&](SegIter<MODE> ahead) {
       Seg g{};
-      while (ahead.next(a, bars->lens, g))
-        if (g.n > 0)
-          return gather(g, 0, qn0) && (SINGLE || g.row0 + 128 >= g.row_end || gather(g, 1, qn1));
+      while (ahead.next(a, bars->lens, g)) {
+        if (g.n == 0) continue;
+        const bool two = !SINGLE && g.row0 + 128 < g.row_end;
+        if (!gather(g, 0, qn0)) return false;
+        if (two && !gather(g, 1, qn1)) return false;
+        if (two) copies_wait<1>();
+        else copies_wait<0>();
+        fence_async_shared();
+        mbar_arrive(smem_u32(&bars->q_full[0]));
+        if (two) {
+          copies_wait<0>();
+          fence_async_shared();
+          mbar_arrive(smem_u32(&bars->q_full[1]));
+        }
+        return true;
+      }
       return true;
     };
     if (!dense && !gather_next(it)) it.pos = it.end;
@@ -775,6 +789,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   out:
+    copies_wait<0>();
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     __syncwarp();
   }

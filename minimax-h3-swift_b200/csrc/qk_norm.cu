@@ -224,16 +224,6 @@ struct Cursor {
   }
 };
 
-__device__ __forceinline__ void copy16(void* dst, const uint16_t* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
-               : "memory");
-}
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copies_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 // HBM-bound, with bytes in flight and instructions not far behind.  A thread's
 // own 32 bytes a row run through a ring of six rows in shared memory that only
 // it reads (no barrier), 96 KB an SM; the table's entries stay in registers
@@ -258,8 +248,8 @@ __global__ void __launch_bounds__(kThreads, kCtas) qk_norm_fwd_kernel(const __gr
       if (in.more()) {
         if (in.live()) {
           const uint16_t* x = p.o.x.p + in.off[0];
-          copy16(&ring[slot][0][threadIdx.x], x + c0);
-          copy16(&ring[slot][1][threadIdx.x], x + c1);
+          copy16(smem_u32(&ring[slot][0][threadIdx.x]), x + c0);
+          copy16(smem_u32(&ring[slot][1][threadIdx.x]), x + c1);
         }
         in.next();
       }
@@ -340,10 +330,10 @@ __global__ void __launch_bounds__(kThreads, kCtas) qk_norm_bwd_kernel(const __gr
         if (in.more()) {
           if (in.live()) {
             const uint16_t *x = p.o.x.p + in.off[0], *go = p.o.g.p + in.off[1];
-            copy16(&sm.ring[slot][0][threadIdx.x], x + c0);
-            copy16(&sm.ring[slot][1][threadIdx.x], x + c1);
-            copy16(&sm.ring[slot][2][threadIdx.x], go + c0);
-            copy16(&sm.ring[slot][3][threadIdx.x], go + c1);
+            copy16(smem_u32(&sm.ring[slot][0][threadIdx.x]), x + c0);
+            copy16(smem_u32(&sm.ring[slot][1][threadIdx.x]), x + c1);
+            copy16(smem_u32(&sm.ring[slot][2][threadIdx.x]), go + c0);
+            copy16(smem_u32(&sm.ring[slot][3][threadIdx.x]), go + c1);
           }
           in.next();
         }
