@@ -35,6 +35,9 @@ struct DeviceGuard {
   }
 };
 
+// a b c > limit, for 32-bit numbers that are not negative.
+bool product_over(int64_t a, int64_t b, int64_t c, int64_t limit) { return c > 0 && (a * b > limit || a * b * c > limit); }
+
 // Normalises one [batch, tokens, heads, 128] operand.  Outputs may not have
 // two elements in one place.
 Refusal rows(const h3c_bview& v, int64_t batch, int64_t tokens, int64_t heads, bool output, const char* name,
@@ -68,6 +71,7 @@ Refusal rows(const h3c_bview& v, int64_t batch, int64_t tokens, int64_t heads, b
     for (const Axis& a : ax) {
       if (a.size == 1) continue;
       if (a.stride < extent) return no(H3C_ERR_INVALID_ARGUMENT, n + " overlaps itself");
+      if (a.stride > ((int64_t)1 << 46) / (a.size - 1)) return no(H3C_ERR_UNSUPPORTED, n + " spans 2^47 bytes or more");
       extent += (a.size - 1) * a.stride;
     }
   }
@@ -93,7 +97,8 @@ Refusal check_cross(const h3c_cross_args* a, int op, h3::CrossLaunch* L) {
   if (prefix && a->prefix_len < 0) return no(H3C_ERR_INVALID_ARGUMENT, "prefix_len must not be negative");
   const int64_t B = a->batch, P = prefix ? a->prefix_len : 0;
   // row and tile numbers are 32-bit in the kernels
-  if (B * a->heads * (int64_t)std::max(a->q_len, 1) > INT_MAX || B * a->heads * (((int64_t)a->kv_len + 127) / 128) > INT_MAX ||
+  if (product_over(B, a->heads, std::max(a->q_len, 1), INT_MAX) ||
+      product_over(B, a->heads, ((int64_t)a->kv_len + 127) / 128, INT_MAX) ||
       P + a->kv_len > INT_MAX - 256 || a->q_len > INT_MAX - 256)
     return no(H3C_ERR_UNSUPPORTED, "more than 2^31 rows");
   h3::CrossLaunch l{};
@@ -193,7 +198,7 @@ Refusal check_norm(const h3c_qk_norm_args* a, bool bwd, h3::QkNormLaunch* L) {
     if (o.table && (o.half <= 0 || o.half > 64)) return no(H3C_ERR_UNSUPPORTED, "rope half must be in [1, 64]");
     if (o.table && a->batch > 1 && (o.table_batch < 0 || (o.table_batch & 3)))
       return no(H3C_ERR_INVALID_ARGUMENT, "a rope batch stride must be a multiple of 4 and not negative");
-    if ((int64_t)a->batch * o.tokens * o.heads > INT_MAX - 65536) return no(H3C_ERR_UNSUPPORTED, "more than 2^31 rows");
+    if (product_over(a->batch, o.heads, o.tokens, INT_MAX - 65536)) return no(H3C_ERR_UNSUPPORTED, "more than 2^31 rows");
     const int64_t B = a->batch;
     H3_REFUSE(rows(i ? a->k : a->q, B, o.tokens, o.heads, false, i ? "k" : "q", &o.x));
     if (bwd) {

@@ -156,6 +156,21 @@ def test_norm_refusals(lib, path, value, status, why, ops):
             assert st == lib.H3C_OK, said
 
 
+def test_sizes_whose_products_pass_64_bits(lib):
+    """2^31 - 1 on three axes: 2^93 rows must not wrap to a number that passes."""
+    big = 2 ** 31 - 1
+    for a in (_cross(lib), _norm(lib)):
+        a.batch = a.heads = a.kv_heads = a.q_len = big
+        for op in (0, 1):
+            st, n, said = _ask(lib, a, op)
+            assert (st, n) == (lib.H3C_ERR_UNSUPPORTED, 0) and "2^31 rows" in said, said
+    a = _cross(lib, batch=1, kv_len=2 ** 20)
+    for v in (a.k, a.v, a.dk, a.dv):
+        v.token_stride = 2 ** 38
+    st, _, said = _ask(lib, a, 1)
+    assert st == lib.H3C_ERR_UNSUPPORTED and "dk spans 2^47 bytes" in said, said
+
+
 def test_null_arguments(lib):
     L = lib.load()
     n = C.c_size_t()
