@@ -79,8 +79,10 @@ def _axes(name, kind, hsd: bool, device: int, want=None):
 # types and device alone: a program makes the same call again and again, and
 # going through them took 3 of its 8 us in Python.
 @functools.lru_cache(maxsize=4096)
-def _cross_form(op, hsd, device, q, out, k, v, prefix, grads):
+def _cross_form(op, hsd, device, q, out, k, v, lens, lse, prefix, grads):
     """Strides and sizes of a call, in the order of its arguments."""
+    import torch
+
     aq, mine = _axes("q", q, hsd, device)
     ao, _ = _axes("out", out, hsd, device, mine)
     ak, keys = _axes("k", k, hsd, device)
@@ -88,6 +90,10 @@ def _cross_form(op, hsd, device, q, out, k, v, prefix, grads):
     (B, S, H), (_, N, Hk) = mine, keys
     if keys[0] != B:
         raise ValueError(f"k must have the {B} members of q, got {keys[0]}")
+    if lens is not None:
+        _check_vector("kv_lens", lens, torch.int32, (B,), device)
+    if lse is not None:
+        _check_vector("lse", lse, torch.float32, (B, H, S) if len(lse[0]) == 3 or B > 1 else (H, S), device)
     P, ap = 0, ((0, 0), (0, 0))
     if prefix is not None:
         if len(prefix[0][0]) != 3 or len(prefix[1][0]) != 3:
@@ -105,7 +111,9 @@ def _cross_form(op, hsd, device, q, out, k, v, prefix, grads):
 
 
 @functools.lru_cache(maxsize=4096)
-def _norm_form(hsd, device, q, k, yq, yk, grads):
+def _norm_form(hsd, device, q, k, yq, yk, q_norm, k_norm, q_rope, k_rope, grads):
+    import torch
+
     aq, mine = _axes("q", q, hsd, device)
     ak, keys = _axes("k", k, hsd, device)
     if keys[0] != mine[0]:
@@ -113,18 +121,51 @@ def _norm_form(hsd, device, q, k, yq, yk, grads):
     names = ("q_out", "k_out") if grads is None else ("dq", "dk")
     ayq, _ = _axes(names[0], yq, hsd, device, mine)
     ayk, _ = _axes(names[1], yk, hsd, device, keys)
+    _check_vector("q_norm", q_norm, torch.bfloat16, (128,), device)
+    _check_vector("k_norm", k_norm, torch.bfloat16, (128,), device)
+    hq, bq = _rope_form("q_rope", q_rope, mine[0], mine[1], device)
+    hk, bk = _rope_form("k_rope", k_rope, mine[0], keys[1], device)
     ag = None
     if grads is not None:
         ag = _axes("q_grad", grads[0], hsd, device, mine)[0], _axes("k_grad", grads[1], hsd, device, keys)[0]
-    return aq, ak, ayq, ayk, ag, (mine[0], mine[1], keys[1], mine[2], keys[2], 128)
+        _check_vector("dq_norm", grads[2], torch.float32, (128,), device)
+        _check_vector("dk_norm", grads[3], torch.float32, (128,), device)
+    return aq, ak, ayq, ayk, ag, (mine[0], mine[1], keys[1], mine[2], keys[2], 128), (bq, bk, hq, hk)
 
 
-def _vector(name, t, dtype, shape, device: int) -> int:
-    """Device pointer of a contiguous tensor of the given type and shape."""
-    if t.dtype is not dtype or t.get_device() != device or t.shape != shape or not t.is_contiguous():
+def _contiguous(size, stride) -> bool:
+    if 0 in size:
+        return True
+    n = 1
+    for axis, step in zip(reversed(size), reversed(stride)):
+        if axis != 1 and step != n:
+            return False
+        n *= axis
+    return True
+
+
+def _check_vector(name, kind, dtype, shape, device: int) -> None:
+    """Refuses what is not a contiguous tensor of the given type and shape."""
+    size, stride, given, where = kind
+    if given is not dtype or where != device or size != shape or not _contiguous(size, stride):
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape} on cuda:{device}, got "
-                         f"{t.dtype} {tuple(t.shape)} on {t.device}")
-    return t.data_ptr()
+                         f"{given} {tuple(size)} on {'the host' if where < 0 else f'cuda:{where}'}")
+
+
+def _rope_form(name, kind, batch: int, tokens: int, device: int):
+    """(half, batch stride) of a bf16 [S, half, 4] or [B, S, half, 4] table."""
+    import torch
+
+    if kind is None:
+        return 0, 0
+    shape, stride, dtype, where = kind
+    each = len(shape) == 4
+    if dtype is not torch.bfloat16 or where != device or not 3 <= len(shape) <= 4 or shape[-1] != 4 \
+            or shape[:-2] != ((batch, tokens) if each else (tokens,)) or not _contiguous(shape, stride):
+        raise ValueError(f"{name} must be a contiguous bfloat16 [{tokens}, half, 4] or [{batch}, {tokens}, half, 4] "
+                         f"tensor on cuda:{device}, got {dtype} {tuple(shape)} on "
+                         f"{'the host' if where < 0 else f'cuda:{where}'}")
+    return shape[-2], tokens * shape[-2] * 4 if each else 0
 
 
 def _hsd(layout: str) -> bool:
@@ -305,17 +346,13 @@ class Runtime:
             self._check(status)
 
     def _cross(self, op, call, q, k, v, out, layout, scale, kv_lens, lse, stream, prefix=None, grads=None):
-        import torch
-
-        dev = self.device
         aq, ao, ak, av, (apk, apv), ag, sizes, P, size = _cross_form(
-            op, _hsd(layout), dev, _kind(q), _kind(out), _kind(k), _kind(v),
+            op, _hsd(layout), self.device, _kind(q), _kind(out), _kind(k), _kind(v),
+            None if kv_lens is None else _kind(kv_lens), None if lse is None else _kind(lse),
             None if prefix is None else (_kind(prefix[0]), _kind(prefix[1])),
             None if grads is None else tuple(_kind(g) for g in grads))
-        B, S, H = sizes[0], sizes[1], sizes[3]
-        lens = 0 if kv_lens is None else _vector("kv_lens", kv_lens, torch.int32, (B,), dev)
-        plse = 0 if lse is None else _vector("lse", lse, torch.float32, (B, H, S) if lse.dim() == 3 or B > 1 else (H, S),
-                                             dev)
+        lens = 0 if kv_lens is None else kv_lens.data_ptr()
+        plse = 0 if lse is None else lse.data_ptr()
         ws = self._workspace(size, stream) if size else None
         pk, pv = (0, 0) if prefix is None else (prefix[0].data_ptr(), prefix[1].data_ptr())
         g0, g1, g2, g3 = (0, 0, 0, 0) if grads is None else (g.data_ptr() for g in grads)
@@ -350,44 +387,24 @@ class Runtime:
         self._cross(_lib.H3C_OP_PREFIX_FWD, self._packed.h3c_prefix_attn_fwd, q, k, v, out, layout, scale, kv_lens,
                     lse, stream, prefix=(prefix_k, prefix_v))
 
-    def _rope_rows(self, name, table, batch, tokens):
-        """(pointer, half, batch stride) of a bf16 [S, half, 4] or [B, S, half, 4] table."""
-        import torch
-
-        if table is None:
-            return 0, 0, 0
-        shape = table.shape
-        each = len(shape) == 4
-        if table.dtype is not torch.bfloat16 or table.get_device() != self.device or not 3 <= len(shape) <= 4 \
-                or shape[-1] != 4 or shape[:-2] != ((batch, tokens) if each else (tokens,)) or not table.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous bfloat16 [{tokens}, half, 4] or [{batch}, {tokens}, half, 4] "
-                             f"tensor on cuda:{self.device}, got {table.dtype} {tuple(shape)} on {table.device}")
-        return table.data_ptr(), shape[-2], tokens * shape[-2] * 4 if each else 0
-
     def _norm(self, call, q, k, outs, q_norm, k_norm, eps, q_rope, k_rope, layout, stream, grads=None):
-        import torch
-
-        dev = self.device
         yq, yk = outs if grads is None else grads[2:4]
-        aq, ak, ayq, ayk, ag, sizes = _norm_form(
-            _hsd(layout), dev, _kind(q), _kind(k), _kind(yq), _kind(yk),
-            None if grads is None else (_kind(grads[0]), _kind(grads[1])))
-        B, S, N = sizes[:3]
-        wq = _vector("q_norm", q_norm, torch.bfloat16, (128,), dev)
-        wk = _vector("k_norm", k_norm, torch.bfloat16, (128,), dev)
-        tq, hq, bq = self._rope_rows("q_rope", q_rope, B, S)
-        tk, hk, bk = self._rope_rows("k_rope", k_rope, B, N)
+        aq, ak, ayq, ayk, ag, sizes, ropes = _norm_form(
+            _hsd(layout), self.device, _kind(q), _kind(k), _kind(yq), _kind(yk), _kind(q_norm), _kind(k_norm),
+            None if q_rope is None else _kind(q_rope), None if k_rope is None else _kind(k_rope),
+            None if grads is None else tuple(_kind(grads[i]) for i in (0, 1, 4, 5)))
         yq, yk = (yq.data_ptr(), *ayq), (yk.data_ptr(), *ayk)
         size, ws, fwd, back, dw = 0, None, (yq, yk), (_NO_ROWS,) * 4, (0, 0)
         if grads is not None:
             size = _norm_workspace()
             ws = self._workspace(size, stream)
-            dw = (_vector("dq_norm", grads[4], torch.float32, (128,), dev),
-                  _vector("dk_norm", grads[5], torch.float32, (128,), dev))
+            dw = grads[4].data_ptr(), grads[5].data_ptr()
             fwd = (_NO_ROWS, _NO_ROWS)
             back = (grads[0].data_ptr(), *ag[0]), yq, (grads[1].data_ptr(), *ag[1]), yk
-        args = _NORM.pack(q.data_ptr(), *aq, *fwd[0], k.data_ptr(), *ak, *fwd[1], *sizes, wq, wk, tq, tk, bq, bk, hq, hk,
-                          eps, 0, *back[0], *back[1], *back[2], *back[3], *dw, ws.data_ptr() if size else 0, size)
+        args = _NORM.pack(q.data_ptr(), *aq, *fwd[0], k.data_ptr(), *ak, *fwd[1], *sizes, q_norm.data_ptr(),
+                          k_norm.data_ptr(), 0 if q_rope is None else q_rope.data_ptr(),
+                          0 if k_rope is None else k_rope.data_ptr(), *ropes, eps, 0, *back[0], *back[1], *back[2],
+                          *back[3], *dw, ws.data_ptr() if size else 0, size)
         self._launch(call, args, stream)
 
     def qk_norm_rope_fwd(self, *, q, k, q_out, k_out, q_norm, k_norm, eps=1e-6, q_rope=None, k_rope=None,

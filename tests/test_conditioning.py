@@ -234,12 +234,12 @@ def test_python_refuses_host_tensors_and_types(lib):
     """The tensor checks of the Python calls run before the library is entered."""
     import torch
 
-    from h3attention.runtime import _axes, _cross_workspace, _kind, _norm_workspace, _vector
+    from h3attention.runtime import _axes, _check_vector, _cross_workspace, _kind, _norm_workspace
 
     with pytest.raises(ValueError, match="must be bfloat16 on cuda:0"):
         _axes("q", _kind(torch.zeros(2, 3, 128, dtype=torch.bfloat16)), False, 0)
     with pytest.raises(ValueError, match="must be a contiguous"):
-        _vector("kv_lens", torch.zeros(2, dtype=torch.int64), torch.int32, (2,), 0)
+        _check_vector("kv_lens", _kind(torch.zeros(2, dtype=torch.int64)), torch.int32, (2,), 0)
     a = _cross(lib)
     for op in (0, 1, 2):
         assert _cross_workspace(op, 2, 5, 7, 3, 4, 2) == _ask(lib, a, op)[1]
