@@ -3,9 +3,9 @@
 //   P = 2^(scale log2(e) q.k - lse2);  delta_i = do_i.o_i;  dS = P (do v^T - delta)
 //   dq = scale dS k;  dk = scale dS^T q;  dv = P^T do   (sums over the heads of a group)
 //
-// (delta_i = sum_j P_ij dP_ij too, and is taken so up to 128 keys)
-// delta_kernel goes over do and out once; then two passes, so that every sum
-// has one owner and a fixed order (no atomics):
+// (delta_i = sum_j P_ij dP_ij too, and is taken so of members with up to 128
+// keys).  delta_kernel goes over do and out once, unless kv_len <= 128; then
+// two passes, so that every sum has one owner and a fixed order (no atomics):
 //   dq_kernel    a CTA holds 128 queries and walks the keys: S, dP, dq += dS K
 //   dkv_kernel   a CTA holds 128 keys and walks the queries of all heads of
 //                the group: S^T, dP^T, dv += P^T do, dk += dS^T Q
@@ -220,6 +220,11 @@ struct DqUnit {
   }
 };
 
+// ONE: no member has more than one block of keys.  delta_kernel is then not
+// needed: -lse2 is taken from lse (the next unit's a unit ahead) and left for
+// dkv_kernel together with delta.  Forward and gradient of 15,731 x 56 rows
+// and 77 keys: 484 us, with delta_kernel before it 564.
+template <bool ONE>
 __global__ void __launch_bounds__(kDqThreads, 1)
     dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
               const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_g,
@@ -321,11 +326,13 @@ __global__ void __launch_bounds__(kDqThreads, 1)
             bar = smem_u32(&bars->g_full);
             mbar_expect_tx(bar, kTileBytes);
             tma_tile(smem_u32(sG), &tm_g, bar, x.t0, x.h * a.g_h, x.b * a.g_b);
-            bar = smem_u32(&bars->n_full[ng & 1]);
-            mbar_expect_tx(bar, 1024);
-            const int64_t pad = ((int64_t)x.b * a.n.heads + x.h) * a.q_blocks * 128 + x.t0;
-            bulk_512(smem_u32(bars->nl2[ng & 1]), a.nl2 + pad, bar);
-            bulk_512(smem_u32(bars->delta[ng & 1]), a.delta + pad, bar);
+            if constexpr (!ONE) {
+              bar = smem_u32(&bars->n_full[ng & 1]);
+              mbar_expect_tx(bar, 1024);
+              const int64_t pad = ((int64_t)x.b * a.n.heads + x.h) * a.q_blocks * 128 + x.t0;
+              bulk_512(smem_u32(bars->nl2[ng & 1]), a.nl2 + pad, bar);
+              bulk_512(smem_u32(bars->delta[ng & 1]), a.delta + pad, bar);
+            }
             ++ng;
           }
         }
@@ -342,7 +349,7 @@ __global__ void __launch_bounds__(kDqThreads, 1)
           mbar_wait(smem_u32(&bars->v_full[x & 1]), (x >> 1) & 1, &zero, nullptr);
         if (qn) mbar_wait(smem_u32(&bars->q_full), (qn - 1) & 1, &zero, nullptr);
         if (ng) mbar_wait(smem_u32(&bars->g_full), (ng - 1) & 1, &zero, nullptr);
-        for (int x = max(0, ng - 2); x < ng; ++x)
+        for (int x = ONE ? ng : max(0, ng - 2); x < ng; ++x)
           mbar_wait(smem_u32(&bars->n_full[x & 1]), (x >> 1) & 1, &zero, nullptr);
       }
     } else if (warp == 1 || warp == 2) {
@@ -431,13 +438,29 @@ __global__ void __launch_bounds__(kDqThreads, 1)
     const uint64_t sl2 = dup2(a.scale * kLog2e);
     int e = 0, un = 0, n1 = 0;  // blocks, units, units of one block
     bool ok = true;
+    auto row_of = [&](const DqUnit& x) { return ((int64_t)x.b * a.n.heads + x.h) * a.q_blocks * 128 + x.t0 + r; };
+    auto lse_of = [&](int u) {  // rows past the queries: P is 0
+      if (u >= units) return 0.f;
+      const DqUnit x(a, bars->lens, u);
+      return x.t0 + r < a.n.q_len ? a.lse[((int64_t)x.b * a.n.heads + x.h) * a.n.q_len + x.t0 + r] : INFINITY;
+    };
+    [[maybe_unused]] float ahead = 0.f;
+    if constexpr (ONE) ahead = lse_of(blockIdx.x);
     for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
       const DqUnit x(a, bars->lens, u);
+      float nl2;
+      if constexpr (ONE) {
+        nl2 = ahead * -kLog2e;
+        ahead = lse_of(u + gridDim.x);
+      }
       if (x.n == 0) continue;
-      if (!(ok = wait_w(&bars->n_full[un & 1], (un >> 1) & 1))) break;
-      const uint64_t nl2x2 = dup2(bars->nl2[un & 1][r]);
       uint64_t ndelta = 0;
-      if (x.n > 1) ndelta = dup2(-bars->delta[un & 1][r]);
+      if constexpr (!ONE) {
+        if (!(ok = wait_w(&bars->n_full[un & 1], (un >> 1) & 1))) break;
+        nl2 = bars->nl2[un & 1][r];
+        if (x.n > 1) ndelta = dup2(-bars->delta[un & 1][r]);
+      }
+      const uint64_t nl2x2 = dup2(nl2);
       ++un;
       for (int j = 0; j < x.n; ++j, ++e) {
         if (!(ok = wait_w(&bars->s_full, e & 1))) break;
@@ -458,7 +481,7 @@ __global__ void __launch_bounds__(kDqThreads, 1)
         uint32_t d[64];
         load64(lane_base + 256 + 64 * w, d);
         const int valid = x.len - 128 * j - 64 * w;  // this half's
-        if (x.n == 1) {
+        if (ONE || x.n == 1) {
           // All keys are here, so delta is sum(P dP) in fp32 and not do.out:
           // the rounding of out shows in dS where keys are few (with one key
           // dS is 0: hence also the division by the weights' own sum).  Half 1
@@ -485,7 +508,8 @@ __global__ void __launch_bounds__(kDqThreads, 1)
             *all = own;
             fence_async_shared();
             mbar_arrive(smem_u32(&bars->sum_full[0]));
-            a.delta[((int64_t)x.b * a.n.heads + x.h) * a.q_blocks * 128 + x.t0 + r] = own;  // for dkv_kernel
+            a.delta[row_of(x)] = own;  // for dkv_kernel
+            if (ONE) a.nl2[row_of(x)] = nl2;
           }
           ++n1;
           ndelta = dup2(-own);
@@ -1006,19 +1030,27 @@ cudaError_t launch_cross_bwd(const CrossLaunch& L, cudaStream_t s, std::string* 
   if (n.kv_len && (!make_map4(&mk, L.k, n.kv_len, n.kv_heads, n.batch, err) ||
                    !make_map4(&mv, L.v, n.kv_len, n.kv_heads, n.batch, err)))
     return cudaErrorInvalidValue;
-  static std::once_flag once_q[64], once_kv[64];
-  static cudaError_t res_q[64], res_kv[64];
-  cudaError_t e = prepare(dq_kernel, kDqSmem, 128, once_q, res_q);
+  const bool one = n.kv_len > 0 && n.kv_len <= 128;
+  static std::once_flag once_q[2][64], once_kv[64];
+  static cudaError_t res_q[2][64], res_kv[64];
+  cudaError_t e = one ? prepare(dq_kernel<true>, kDqSmem, 128, once_q[1], res_q[1])
+                      : prepare(dq_kernel<false>, kDqSmem, 128, once_q[0], res_q[0]);
   if (e == cudaSuccess) e = prepare(dkv_kernel, kDkvSmem, 168, once_kv, res_kv);
   if (e != cudaSuccess) return e;
-  const int units = n.batch * n.heads * a.q_blocks;
+  const int units = n.batch * n.heads * a.q_blocks, dq_ctas = units < kSms ? units : kSms;
   const int ctas = n.kv_len ? dkv_ctas(n) : 0;
   const int groups = (n.heads + kHeads - 1) / kHeads * n.batch;
-  if (ctas) {
+  if (one) {
+    dq_kernel<true><<<dq_ctas, kDqThreads, kDqSmem, s>>>(mq, mk, mv, mg, a, units);
+    e = cudaGetLastError();
+  } else if (!ctas) {
+    dq_kernel<false><<<dq_ctas, kDqThreads, kDqSmem, s>>>(mq, mk, mv, mg, a, units);
+    e = cudaGetLastError();
+  } else {
     delta_kernel<<<dim3(a.q_blocks * 8, groups < 65535 ? groups : 65535), 256, 0, s>>>(a);
     e = cudaGetLastError();
+    if (e == cudaSuccess) e = launch_after(dq_kernel<false>, dq_ctas, kDqThreads, kDqSmem, s, mq, mk, mv, mg, a, units);
   }
-  if (e == cudaSuccess) e = launch_after(dq_kernel, units < kSms ? units : kSms, kDqThreads, kDqSmem, s, mq, mk, mv, mg, a, units);
   if (ctas && e == cudaSuccess) e = launch_after(dkv_kernel, ctas, kThreads, kDkvSmem, s, mq, mk, mv, mg, a);
   if (ctas > 1 && e == cudaSuccess) e = launch_after(dkv_join_kernel, dim3(ctas - 1, 32), 256, 0, s, a, ctas);
   return e;
