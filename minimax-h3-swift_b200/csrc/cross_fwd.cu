@@ -13,7 +13,7 @@
 // that is cut, or whose rows have two sources, leaves fp32 partial results
 // (o, m, l) that a second kernel joins in a fixed order.  Row blocks:
 //   dense   q_len >= 128: 2 x 128 tokens of one head, Q tiles by TMA; keys are
-//           the prefix's and then the member's own
+//           the prefix's and then the member's own (compiled twice: kShort)
 //   folded  q_len < 128: a row is (member, token, head of the group), so one
 //           K/V tile serves all query heads of its key head and, for the
 //           prefix, the whole batch; rows are gathered.  The
@@ -42,7 +42,7 @@
 // (64 members of 4,096 keys and 8 key heads: 180 us, 6.0 TB/s; one token over
 // 65,536 keys: 56 us for 41 at the copy rate, the rest the start, whose code
 // and queries come from HBM behind the first keys, and the join).  Dual: as
-// dense (32 members of 5 rows over 65,536 keys and 512 of their own: 107 us).
+// dense (32 members of 5 rows over 65,536 keys and 512 of their own: 104 us).
 // Every wait is bounded (see attn_tc.cu).
 #include <algorithm>
 #include <climits>
@@ -63,7 +63,10 @@ constexpr int kSms = 148;
 // over 65,536: 107 and 111.
 constexpr int kUnitCost = 2;
 
-enum { kDense = 0, kSingle = 1, kDual = 2 };
+// kShort: dense rows against few key tiles, see the mask of the last tile
+enum { kDense = 0, kSingle = 1, kDual = 2, kShort = 3 };
+constexpr int kShortTiles = 3;
+constexpr bool is_dense(int mode) { return mode == kDense || mode == kShort; }
 
 // The units of one source of keys: the prefix (folded rows only), or the
 // members' own keys (dense rows: the prefix's and their own).
@@ -135,8 +138,8 @@ struct SegIter {
     if (a.tpc) {
       do {
         if (pos >= end) return false;
-        const uint32_t pre = MODE == kDense ? 0 : a.units_p * a.src[0].pitch;
-        s.own = MODE == kDense || pos >= pre;
+        const uint32_t pre = is_dense(MODE) ? 0 : a.units_p * a.src[0].pitch;
+        s.own = is_dense(MODE) || pos >= pre;
         const Source& c = a.src[s.own];
         const uint32_t off = s.own ? pos - pre : pos;
         tiles = c.tiles;
@@ -145,12 +148,12 @@ struct SegIter {
         j1 = min(c.pitch, s.j0 + (int)(end - pos));
         s.slot = blockIdx.x - c.by_tpc(pos - s.j0);
         pos += j1 - s.j0;
-      } while (MODE != kDense && s.j0 >= tiles);
-      if (MODE != kDense) j1 = min(j1, tiles);
+      } while (!is_dense(MODE) && s.j0 >= tiles);
+      if (!is_dense(MODE)) j1 = min(j1, tiles);
     } else {
       if (pos >= end) return false;
-      s.own = MODE == kDense || (int)pos >= a.units_p;
-      s.unit = (int)pos - (MODE != kDense && s.own ? a.units_p : 0);
+      s.own = is_dense(MODE) || (int)pos >= a.units_p;
+      s.unit = (int)pos - (!is_dense(MODE) && s.own ? a.units_p : 0);
       tiles = a.src[s.own].tiles;
       s.j0 = 0;
       j1 = tiles;
@@ -167,7 +170,7 @@ struct SegIter {
       s.len = 0;
       s.npre = limit = a.np;
     } else {
-      if (MODE == kDense) {
+      if (is_dense(MODE)) {
         s.b = a.by_heads(x);
         s.h = x - s.b * a.n.heads;
         s.hk = a.by_group(s.h);
@@ -186,7 +189,7 @@ struct SegIter {
       limit = s.npre + ((s.len + 127) >> 7);
     }
     s.n = max(0, min(j1, limit) - s.j0);
-    s.direct = s.j0 == 0 && j1 == tiles && (MODE == kDense || !a.two_sources);
+    s.direct = s.j0 == 0 && j1 == tiles && (is_dense(MODE) || !a.two_sources);
     return true;
   }
   // valid keys of tile j of the segment's unit
@@ -233,7 +236,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                      const __grid_constant__ CUtensorMap tm_pv, const __grid_constant__ CUtensorMap tm_o,
                      const __grid_constant__ FwdArgs a) {
   using L = Layout<MODE>;
-  constexpr bool SINGLE = MODE == kSingle, dense = MODE == kDense;
+  constexpr bool SINGLE = MODE == kSingle, dense = is_dense(MODE);
   extern __shared__ __align__(1024) uint8_t smem[];
   if (!tiles_aligned(smem, a.status)) return;
   uint8_t* sQ = smem;
@@ -536,10 +539,24 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int c = 0; c < 8; ++c) H3_TMEM_LD16(tS + 16 * c, (&v[16 * c]));
         tmem_wait_ld();
+        // Keys past the end.  128 selects are 4 KB of code, with which a unit's
+        // code no longer stays in the instruction cache where each unit comes to
+        // them soon: there -inf is written to TMEM instead, in a loop, and the
+        // row loaded again.  15,731 x 56 rows against 77 keys 137 us (selects:
+        // 168), 332 keys 255 (275), 32 members with 512 keys over 65,536 shared
+        // 104 (115).  From four tiles on the selects are faster, since the code
+        // around them comes out faster: 16,384 keys 1,285 us (1,324 with the loop).
         if (valid < 128) {
+          if constexpr (MODE == kDense) {
 #pragma unroll
-          for (int c = 0; c < 128; ++c)
-            if (c >= valid) v[c] = __float_as_uint(-INFINITY);
+            for (int c = 0; c < 128; ++c)
+              if (c >= valid) v[c] = __float_as_uint(-INFINITY);
+          } else {
+            fill_columns(tS, valid, 128, __float_as_uint(-INFINITY));
+#pragma unroll
+            for (int c = 0; c < 8; ++c) H3_TMEM_LD16(tS + 16 * c, (&v[16 * c]));
+            tmem_wait_ld();
+          }
         }
         float mxa[8];
 #pragma unroll
@@ -1075,7 +1092,8 @@ cudaError_t launch_cross_fwd(const CrossLaunch& L, cudaStream_t s, std::string* 
   if (n.prefix_len && (!make_map4(&m[3], L.pk, n.prefix_len, n.kv_heads, 1, err) ||
                        !make_map4(&m[4], L.pv, n.prefix_len, n.kv_heads, 1, err)))
     return cudaErrorInvalidValue;
-  cudaError_t e = dense               ? launch_fwd<kDense>(a, p.ctas, m, s)
+  cudaError_t e = dense && a.src[1].tiles <= kShortTiles ? launch_fwd<kShort>(a, p.ctas, m, s)
+                  : dense             ? launch_fwd<kDense>(a, p.ctas, m, s)
                   : a.mode == kSingle ? launch_fwd<kSingle>(a, p.ctas, m, s)
                                       : launch_fwd<kDual>(a, p.ctas, m, s);
   if (e != cudaSuccess || !p.join) return e;

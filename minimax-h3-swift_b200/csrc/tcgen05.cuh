@@ -479,6 +479,21 @@ __device__ __forceinline__ void tma_prefetch_4d(const CUtensorMap* map, int c0, 
                : "memory");
 }
 
+// Columns [from, to) of the warp's lanes, to a multiple of 16; waits for it.
+__device__ __forceinline__ void fill_columns(uint32_t addr, int from, int to, uint32_t value) {
+  int c = from;
+#pragma unroll 1
+  for (; c & 15; ++c)
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(addr + c), "r"(value) : "memory");
+#pragma unroll 1
+  for (; c < to; c += 16)
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%1,%1,%1,%1,%1,%1,%1,%1,%1,%1,%1,%1,%1,%1,%1};" ::"r"(
+                     addr + c),
+                 "r"(value)
+                 : "memory");
+  tmem_wait_st();
+}
+
 // Orders this thread's shared-memory writes before later reads by TMA or MMA.
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
