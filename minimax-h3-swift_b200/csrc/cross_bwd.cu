@@ -465,6 +465,10 @@ __global__ void __launch_bounds__(kDqThreads, 1)
       for (int j = 0; j < x.n; ++j, ++e) {
         if (!(ok = wait_w(&bars->s_full, e & 1))) break;
         tc_fence_after();
+        const int valid = x.len - 128 * j - 64 * w;  // this half's
+        // (ONE: keys past the length weigh 0, in TMEM: each unit comes to the
+        // mask, and masks of registers are four times the code)
+        if (ONE && valid < 64) fill_columns(lane_base + 128 + 64 * w, max(valid, 0), 64, __float_as_uint(-INFINITY));
         uint32_t s[64];
         load64(lane_base + 128 + 64 * w, s);
         tc_fence_before();
@@ -478,9 +482,9 @@ __global__ void __launch_bounds__(kDqThreads, 1)
         }
         if (!(ok = wait_w(&bars->dp_full, e & 1))) break;
         tc_fence_after();
+        if (ONE && valid < 64) fill_columns(lane_base + 256 + 64 * w, max(valid, 0), 64, 0u);
         uint32_t d[64];
         load64(lane_base + 256 + 64 * w, d);
-        const int valid = x.len - 128 * j - 64 * w;  // this half's
         if (ONE || x.n == 1) {
           // All keys are here, so delta is sum(P dP) in fp32 and not do.out:
           // the rounding of out shows in dS where keys are few (with one key
@@ -491,7 +495,7 @@ __global__ void __launch_bounds__(kDqThreads, 1)
           float own = 0.f, ps = 0.f;
 #pragma unroll
           for (int c = 0; c < 64; ++c)
-            if (c < valid) {
+            if (ONE || c < valid) {
               own = fmaf(p[c], __uint_as_float(d[c]), own);
               ps += p[c];
             }
@@ -523,7 +527,7 @@ __global__ void __launch_bounds__(kDqThreads, 1)
                                    pair2(__float_as_uint(p[2 * c]), __float_as_uint(p[2 * c + 1])));
           pk[c] = pack_bf16(lo2(v), hi2(v));
         }
-        if (valid < 64) {  // keys past the length, whatever their values gave
+        if (!ONE && valid < 64) {  // keys past the length, whatever their values gave
 #pragma unroll
           for (int c = 0; c < 32; ++c) pk[c] = 2 * c + 1 < valid ? pk[c] : 2 * c < valid ? pk[c] & 0xffffu : 0u;
         }
