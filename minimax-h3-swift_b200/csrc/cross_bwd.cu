@@ -223,7 +223,8 @@ struct DqUnit {
 // ONE: no member has more than one block of keys.  delta_kernel is then not
 // needed: -lse2 is taken from lse (the next unit's a unit ahead) and left for
 // dkv_kernel together with delta.  Forward and gradient of 15,731 x 56 rows
-// and 77 keys: 484 us, with delta_kernel before it 564.
+// and 77 keys: 451 us; 479 with masks of registers, and 80 more with
+// delta_kernel before it.
 template <bool ONE>
 __global__ void __launch_bounds__(kDqThreads, 1)
     dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
@@ -467,7 +468,8 @@ __global__ void __launch_bounds__(kDqThreads, 1)
         tc_fence_after();
         const int valid = x.len - 128 * j - 64 * w;  // this half's
         // (ONE: keys past the length weigh 0, in TMEM: each unit comes to the
-        // mask, and masks of registers are four times the code)
+        // mask, and masks of registers are four times the code; where units have
+        // more blocks either takes the same time)
         if (ONE && valid < 64) fill_columns(lane_base + 128 + 64 * w, max(valid, 0), 64, __float_as_uint(-INFINITY));
         uint32_t s[64];
         load64(lane_base + 128 + 64 * w, s);
