@@ -645,6 +645,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto finish_box = [&](int t, bool has, float2 ml) {
       tc_fence_after();
       const int row0 = s.row0 + 128 * t + 32 * q;
+      // A warp without rows leaves both boxes alone: its waits below count on a
+      // store of every box that it fills.
+      if (row0 >= s.row_end) return;
       const float f = 1.0f / fmaxf(ml.y, 1e-30f);
       if (a.lse && row0 + lane < s.row_end)
         a.lse[((int64_t)s.b * a.n.heads + s.h) * a.n.q_len + row0 + lane] =
@@ -678,7 +681,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         fence_async_shared();
         __syncwarp();
-        if (lane == 0 && row0 < s.row_end)
+        if (lane == 0)
           tma_store_4d(&tm_o, smem_u32(box), 64 * p, row0, s.h * (a.out.h != 0), s.b * (a.out.b != 0));
       }
     };
