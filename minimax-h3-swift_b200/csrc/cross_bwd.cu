@@ -46,6 +46,7 @@ struct BwdArgs {
   int32_t q_blocks;
   int32_t* status;
   uint64_t wait_limit_ns;
+  int32_t drop_item;          // test hook: K tile (dq) and q tile (dk, dv) of each CTA that is never loaded
   int32_t q_b, q_h, k_b, k_h, v_b, v_h, g_b, g_h;
   Div by_blocks, by_heads, by_group;
 };
@@ -115,6 +116,7 @@ __device__ __forceinline__ void release_tmem(int warp, uint32_t tmem, volatile i
     if (*abort_flag) {
       volatile int32_t zero = 0;
       mbar_wait(smem_u32(done), 0, &zero, nullptr);
+      settle();
       __syncwarp();
     }
     tc_fence_after();
@@ -309,7 +311,8 @@ __global__ void __launch_bounds__(kDqThreads, 1)
                               (valid < 128 && x.len < a.n.kv_len ? valid << kZeroShift : 0);
           bar = smem_u32(&bars->k_full[kr]);
           mbar_expect_tx(bar, kTileBytes);
-          tma_tile(smem_u32(sK + kr * kTileBytes), &tm_k, bar, 128 * j, hk * a.k_h, x.b * a.k_b);
+          if (e != a.drop_item)
+            tma_tile(smem_u32(sK + kr * kTileBytes), &tm_k, bar, 128 * j, hk * a.k_h, x.b * a.k_b);
           ++e;
           if (++kr == 3) {
             kr = 0;
@@ -345,13 +348,13 @@ __global__ void __launch_bounds__(kDqThreads, 1)
       } else {  // abort: every load in flight lands before anyone may exit
         volatile int32_t zero = 0;
         for (int x = max(0, e - 3); x < e; ++x)
-          mbar_wait(smem_u32(&bars->k_full[x % 3]), (x / 3) & 1, &zero, nullptr);
+          mbar_wait(smem_u32(&bars->k_full[x % 3]), (x / 3) & 1, &zero, nullptr, kDrainNs);
         for (int x = max(0, nv - 2); x < nv; ++x)
-          mbar_wait(smem_u32(&bars->v_full[x & 1]), (x >> 1) & 1, &zero, nullptr);
-        if (qn) mbar_wait(smem_u32(&bars->q_full), (qn - 1) & 1, &zero, nullptr);
-        if (ng) mbar_wait(smem_u32(&bars->g_full), (ng - 1) & 1, &zero, nullptr);
+          mbar_wait(smem_u32(&bars->v_full[x & 1]), (x >> 1) & 1, &zero, nullptr, kDrainNs);
+        if (qn) mbar_wait(smem_u32(&bars->q_full), (qn - 1) & 1, &zero, nullptr, kDrainNs);
+        if (ng) mbar_wait(smem_u32(&bars->g_full), (ng - 1) & 1, &zero, nullptr, kDrainNs);
         for (int x = ONE ? ng : max(0, ng - 2); x < ng; ++x)
-          mbar_wait(smem_u32(&bars->n_full[x & 1]), (x >> 1) & 1, &zero, nullptr);
+          mbar_wait(smem_u32(&bars->n_full[x & 1]), (x >> 1) & 1, &zero, nullptr, kDrainNs);
       }
     } else if (warp == 1 || warp == 2) {
       // Two issuers, one of S and one of dP and dq, so that the waits of one
@@ -705,7 +708,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           bars->info[e & 7] = (it == seg.it0 ? kFirst : 0) | (it == seg.it1 - 1 ? kLast : 0);
           bar = smem_u32(&bars->q_full[qr]);
           mbar_expect_tx(bar, kTileBytes);
-          tma_tile(smem_u32(sQ + qr * kTileBytes), &tm_q, bar, 128 * qb, h * a.q_h, seg.b * a.q_b);
+          if (e != a.drop_item)
+            tma_tile(smem_u32(sQ + qr * kTileBytes), &tm_q, bar, 128 * qb, h * a.q_h, seg.b * a.q_b);
           ++e;
           if (++qr == 3) {
             qr = 0;
@@ -733,10 +737,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       } else {  // abort: every load in flight lands before anyone may exit
         volatile int32_t zero = 0;
         for (int x = max(0, e - 3); x < e; ++x)
-          mbar_wait(smem_u32(&bars->q_full[x % 3]), (x / 3) & 1, &zero, nullptr);
+          mbar_wait(smem_u32(&bars->q_full[x % 3]), (x / 3) & 1, &zero, nullptr, kDrainNs);
         for (int x = max(0, ng - 2); x < ng; ++x)
-          mbar_wait(smem_u32(&bars->g_full[x & 1]), (x >> 1) & 1, &zero, nullptr);
-        if (sn) mbar_wait(smem_u32(&bars->kv_full), (sn - 1) & 1, &zero, nullptr);
+          mbar_wait(smem_u32(&bars->g_full[x & 1]), (x >> 1) & 1, &zero, nullptr, kDrainNs);
+        if (sn) mbar_wait(smem_u32(&bars->kv_full), (sn - 1) & 1, &zero, nullptr, kDrainNs);
       }
     } else if (warp == 1) {
       // dv(e-1) S(e) dk(e-1) dP(e): the order keeps P^T (dS^T) in place until
@@ -1026,6 +1030,7 @@ cudaError_t launch_cross_bwd(const CrossLaunch& L, cudaStream_t s, std::string* 
   a.part = a.delta + rows;
   a.status = L.status;
   a.wait_limit_ns = L.wait_limit_ns;
+  a.drop_item = L.drop_item;
   a.q_b = L.q.b != 0, a.q_h = L.q.h != 0;
   a.k_b = L.k.b != 0, a.k_h = L.k.h != 0;
   a.v_b = L.v.b != 0, a.v_h = L.v.h != 0;

@@ -103,6 +103,7 @@ struct FwdArgs {
   float2* part_ml[2];
   int32_t* status;
   uint64_t wait_limit_ns;
+  int32_t drop_item;          // test hook: K/V entry of each CTA that is never loaded
   // 1 where an operand's tensor map has the axis, 0 where it is broadcast
   int32_t q_b, q_h, k_b, k_h, v_b, v_h, pk_h, pv_h;
 };
@@ -329,6 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             // of 65,536 keys, 1 row: 56 us, 61 with the tiles kept in L2 like
             // any other load)
             auto load = [&](uint32_t dst, const CUtensorMap* map, int tok, int h, int b) {
+              if (ec == a.drop_item) return;  // (the entry then never completes)
 #pragma unroll
               for (int x = 0; x < 2; ++x)
                 if constexpr (dense) tma_load_4d(dst + x * kHalfBytes, map, bar, 64 * x, tok, h, b);
@@ -359,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           // that the Q loader did not join never completes: a short limit)
           volatile int32_t zero = 0;
           for (int e = max(0, issued - L::kRing); e < issued; ++e, zero = 0)
-            mbar_wait(smem_u32(&bars->kv_full[e % L::kRing]), (e / L::kRing) & 1, &zero, nullptr, 10000000);
+            mbar_wait(smem_u32(&bars->kv_full[e % L::kRing]), (e / L::kRing) & 1, &zero, nullptr, kDrainNs);
         }
       }
     } else if (warp == 1) {
@@ -821,6 +823,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (bars->abort) {  // no MMA may still write TMEM when it is released
       volatile int32_t zero = 0;
       mbar_wait(smem_u32(&bars->done), 0, &zero, nullptr);
+      settle();
       __syncwarp();
     }
     tc_fence_after();
@@ -1080,6 +1083,7 @@ cudaError_t launch_cross_fwd(const CrossLaunch& L, cudaStream_t s, std::string* 
   }
   a.status = L.status;
   a.wait_limit_ns = L.wait_limit_ns;
+  a.drop_item = L.drop_item;
   a.q_b = L.q.b != 0, a.q_h = L.q.h != 0;
   a.k_b = L.k.b != 0, a.k_h = L.k.h != 0;
   a.v_b = L.v.b != 0, a.v_h = L.v.h != 0;

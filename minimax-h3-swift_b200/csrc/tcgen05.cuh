@@ -12,6 +12,7 @@ namespace h3 {
 constexpr int kTileBytes = 128 * 128 * 2;   // one 128x128 bf16 tile
 constexpr int kHalfBytes = kTileBytes / 2;  // one 128x64 swizzle box
 constexpr uint64_t kWaitLimitNs = 4000000000ull;  // 4 s
+constexpr uint64_t kDrainNs = 10000000ull;  // 10 ms, of a wait for the waiter's own copies (they take microseconds)
 
 // ------------------------------------------------------------- primitives
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -59,6 +60,13 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
       return false;
     }
   }
+}
+
+// After an abort, behind every role's end: a copy that one role had just issued
+// when another gave up lands before the block's shared memory is given back.
+__device__ __forceinline__ void settle() {
+  const uint64_t t0 = globaltimer();
+  for (int i = 0; i < 100000 && globaltimer() - t0 < 1000000; ++i) __nanosleep(1000);
 }
 
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
