@@ -272,9 +272,11 @@ h3c_status h3c_prologue(h3c_ctx* ctx, h3c_view x, h3c_view out, int32_t seq_len,
 h3c_status h3c_attn_fwd(h3c_ctx* ctx, const h3c_attn_args* args, void* stream);
 /* Bytes of workspace h3c_attn_fwd needs for these args. */
 h3c_status h3c_attn_workspace_size(const h3c_attn_args* args, size_t* bytes);
-/* Reads (and clears) the status word the attention kernel writes when one of
- * its bounded device waits gives up: H3C_OK, or H3C_ERR_TIMEOUT (the output
- * of that call is invalid; the context stays usable).  Synchronous.  The
+/* Reads (and clears) the status words the attention kernels write when one of
+ * their bounded device waits gives up: H3C_OK, or H3C_ERR_TIMEOUT (the output
+ * of that call is invalid; the context stays usable), with h3c_last_error
+ * naming the self-attention call, the conditioning calls or both.  Does not
+ * wait for calls still running on a non-blocking stream.  Synchronous.  The
  * bounded waits replace the reference's render-level cancellation
  * (Sources/MiniMaxH3/RenderEngine.swift:574-590) at the kernel level. */
 h3c_status h3c_device_status(h3c_ctx* ctx);
@@ -302,15 +304,16 @@ h3c_status h3c_attn_fwd_noalloc(const h3c_attn_args* args, void* stream, char* e
 h3c_status h3c_attn_fwd_noalloc_status(void);
 
 /* --- conditioning: cross attention, shared prefix, q/k norm ------------------ */
-/* These calls keep no state between them: scratch is the caller's
+/* These calls read nothing that another call leaves: scratch is the caller's
  * (`workspace`, device memory of at least the size the matching
  * *_workspace_size call gives, 256-byte aligned; its contents need not be
  * kept or cleared), so calls on several streams, host threads or captured
  * graphs are independent as long as each has its own workspace and outputs.
  * They are asynchronous on `stream`, allocate nothing and may be captured.
  * Results are deterministic: no sum depends on the order of atomics.  A
- * bounded device wait that gives up is reported by h3c_device_status, as for
- * h3c_attn_fwd. */
+ * bounded device wait that gives up (4 s) makes the output of its own call
+ * invalid and no other's; h3c_device_status reports it.  Nothing of a call on
+ * valid arguments reaches that bound. */
 
 /* A bf16 [batch, tokens, heads, 128] operand: element (b, s, h, d) sits at
  * ptr[b * batch_stride + s * token_stride + h * head_stride + d].  A stride of

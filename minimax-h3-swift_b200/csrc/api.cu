@@ -480,11 +480,17 @@ h3c_status h3c_attn_fwd_sync(h3c_ctx* ctx, const h3c_attn_args* args, void* stre
 h3c_status h3c_device_status(h3c_ctx* ctx) {
   if (!ctx) return H3C_ERR_INVALID_ARGUMENT;
   H3_CUDA_TRY(ctx, cudaSetDevice(ctx->device));
-  int32_t word = 0;
-  H3_CUDA_TRY(ctx, cudaMemcpy(&word, ctx->d_counter + 1, sizeof(word), cudaMemcpyDeviceToHost));
-  if (word == 0) return H3C_OK;
-  H3_CUDA_TRY(ctx, cudaMemset(ctx->d_counter + 1, 0, sizeof(int64_t)));
-  return fail(ctx, (h3c_status)word, "h3c_attn_fwd: a bounded device wait gave up (H3C_ERR_TIMEOUT); output invalid");
+  int64_t words[3] = {};  // [1] to [3]
+  H3_CUDA_TRY(ctx, cudaMemcpy(words, ctx->d_counter + 1, sizeof(words), cudaMemcpyDeviceToHost));
+  const int32_t attn = (int32_t)words[0], cond = (int32_t)words[2];
+  if (attn) H3_CUDA_TRY(ctx, cudaMemset(ctx->d_counter + 1, 0, sizeof(int64_t)));
+  if (cond) H3_CUDA_TRY(ctx, cudaMemset(ctx->d_counter + 3, 0, sizeof(int64_t)));
+  if (!attn && !cond) return H3C_OK;
+  const char* who = !cond   ? "h3c_attn_fwd"
+                    : !attn ? "h3c_cross_attn_fwd, h3c_cross_attn_bwd or h3c_prefix_attn_fwd"
+                            : "h3c_attn_fwd, and h3c_cross_attn_fwd, h3c_cross_attn_bwd or h3c_prefix_attn_fwd";
+  return fail(ctx, (h3c_status)(attn ? attn : cond),
+              std::string(who) + ": a bounded device wait gave up (H3C_ERR_TIMEOUT); output invalid");
 }
 
 h3c_status h3c_fill_normal_bf16(h3c_ctx* ctx, void* d_out, int64_t n, uint64_t seed, uint64_t stream_id, double mean,

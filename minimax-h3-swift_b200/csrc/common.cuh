@@ -18,7 +18,7 @@ struct h3c_ctx {
   cudaEvent_t workspace_done = nullptr;  // recorded after the last launch that read the workspace
   void* comm = nullptr;           // h3c_comm_state of the sequence-sharded path
   int64_t* d_counter = nullptr;   // small device scratch: [0] mask builder nnz, [1] kernel status word,
-                                  // [2] block-list validation flags
+                                  // [2] block-list validation flags, [3] status word of the conditioning calls
 };
 
 namespace h3 {

@@ -160,7 +160,7 @@ h3c_status cross_call(h3c_ctx* ctx, const h3c_cross_args* args, int op, const ch
   DeviceGuard guard(ctx->device);
   H3_CUDA_TRY(ctx, guard.err);
   L.ws = (uint8_t*)args->workspace;
-  L.status = (int32_t*)(ctx->d_counter + 1);
+  L.status = (int32_t*)(ctx->d_counter + 3);
   L.wait_limit_ns = h3::kWaitLimitNs;
   L.drop_item = -1;
   // Test hooks (fault injection on the host side), as those of h3c_attn_fwd; the

@@ -26,7 +26,7 @@ struct CrossLaunch {
   const int32_t* kv_lens;     // may be null
   float* lse;                 // may be null (forward)
   uint8_t* ws;
-  int32_t* status;            // status word of the context (bounded waits)
+  int32_t* status;            // the context's status word of these calls (bounded waits), written only
   uint64_t wait_limit_ns;
   int32_t drop_item;          // test hook: load of each CTA that its producer skips (-1: none)
 };

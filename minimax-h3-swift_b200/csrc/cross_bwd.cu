@@ -16,7 +16,7 @@
 // Roles of a CTA's 12 warps: 0 TMA producer, 1 MMA issuer, 2 TMEM owner (and
 // a second issuer in dq_kernel), 4-7 and 8-11 elementwise: each warpgroup takes
 // 64 of a tile's 128 columns of every row (thread = row = TMEM lane).  Every
-// wait is bounded (attn_tc.cu).
+// wait is bounded (attn_tc.cu; a CTA that gives up does so alone).
 //
 // dkv_kernel's work, all (key tile, query block) pairs in a row, is cut into
 // equal runs, one a CTA; a key tile that is cut leaves fp32 partial sums that
@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(kDqThreads, 1)
   // placed while the kernel before runs; nothing is read or written before its end
   asm volatile("griddepcontrol.wait;" ::: "memory");
   auto wait = [&](uint64_t* bar, uint32_t parity) {
-    return mbar_wait(smem_u32(bar), parity, abort_flag, a.status, a.wait_limit_ns);
+    return mbar_wait<false>(smem_u32(bar), parity, abort_flag, a.status, a.wait_limit_ns);
   };
   // Register split of the launch's 512 x 128: 128 x 48 + 256 x 176 + 128 x 112.
   if (warp < 4) {
@@ -685,7 +685,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // step of 3 x 257 x 8 rows; the same in dq_kernel cost the clip 2%).
   if (warp >= 2) asm volatile("griddepcontrol.wait;" ::: "memory");
   auto wait = [&](uint64_t* bar, uint32_t parity) {
-    return mbar_wait(smem_u32(bar), parity, abort_flag, a.status, a.wait_limit_ns);
+    return mbar_wait<false>(smem_u32(bar), parity, abort_flag, a.status, a.wait_limit_ns);
   };
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");

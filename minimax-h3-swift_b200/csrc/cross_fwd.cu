@@ -43,7 +43,7 @@
 // 65,536 keys: 56 us for 41 at the copy rate, the rest the start, whose code
 // and queries come from HBM behind the first keys, and the join).  Dual: as
 // dense (32 members of 5 rows over 65,536 keys and 512 of their own: 104 us).
-// Every wait is bounded (see attn_tc.cu).
+// Every wait is bounded (see attn_tc.cu; a CTA that gives up does so alone).
 #include <algorithm>
 #include <climits>
 #include <mutex>
@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = bars->tmem_base;
   asm volatile("griddepcontrol.launch_dependents;");
   auto wait = [&](uint64_t* bar, uint32_t parity) {
-    return mbar_wait(smem_u32(bar), parity, abort_flag, a.status, a.wait_limit_ns);
+    return mbar_wait<false>(smem_u32(bar), parity, abort_flag, a.status, a.wait_limit_ns);
   };
 
   // Register split of the launch's 512 x 128: 128 x 48 + 256 x 192 + 128 x 80.

@@ -39,7 +39,10 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
   return ok != 0;
 }
 
-// Bounded wait; false on abort/timeout.
+// Bounded wait; false on abort/timeout.  SHARED: launches share the status
+// word, and a wait that finds it set gives up; without, the word is only
+// written, so that calls beside or behind a failed one are not drawn in.
+template <bool SHARED = true>
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int32_t* abort_flag,
                                           int32_t* status, uint64_t limit_ns = kWaitLimitNs) {
   for (int i = 0; i < 64; ++i)
@@ -48,9 +51,10 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
   while (true) {
     if (mbar_try(bar, parity)) return true;
     if (*abort_flag) return false;
-    // another CTA's wait already gave up: stop instead of timing out again
-    // (one status word per launch, so a systematic stall ends in one limit)
-    if (status && *(volatile int32_t*)status != 0) {
+    // another CTA's wait already gave up: stop instead of timing out again, so
+    // that a systematic stall ends in one limit (a grid of at most a CTA an SM
+    // does so anyway)
+    if (SHARED && status && *(volatile int32_t*)status != 0) {
       *abort_flag = 1;
       return false;
     }

@@ -73,3 +73,59 @@ def test_dropped_load_of_a_prefix(gpu, monkeypatch, B, S):
     _times_out()
     base._rt().prefix_attn_fwd(**kw)
     base._check_attention(q, k, v, [200] * B, dict(out=out, lse=lse), prefix=(pk, pv))
+
+
+def test_a_failed_call_leaves_the_others_alone(gpu, monkeypatch):
+    """Calls beside and behind one whose waits ran out, before anyone has read
+    the status: right results, of the self-attention too; and the other way round."""
+    import torch
+
+    from h3attention import BlockList, H3CError, MaskSpec
+
+    rt = base._rt()
+    q, k, v, do = base._inputs(2, 2500, 400, 10, 5, 84)
+    want = base._run_cross(q, k, v, [400, 200], do)
+    lens = base._lens_tensor([400, 200])
+    g = torch.cuda.CUDAGraph()
+    replayed, lse = torch.empty_like(q), torch.empty(2, 10, 2500, device="cuda")
+    with torch.cuda.graph(g):
+        rt.cross_attn_fwd(q=q, k=k, v=v, out=replayed, lse=lse, kv_lens=lens, scale=base.SCALE)
+    bl = BlockList.build(MaskSpec(seq_len=1024, frames=4, height=16, width=16, n_random=1, seed=3))
+    x = base._inputs(1, 1024, 1024, 2, 2, 85)[:3]
+    out = torch.empty_like(x[0][0])
+    kw = dict(q=x[0][0], k=x[1][0], v=x[2][0], out=out, layout="SHD", scale=base.SCALE, blocks=bl.on(gpu))
+    rt.attn_fwd_sync(**kw)
+    attended = out.clone()
+
+    def others_are_right():
+        again = base._run_cross(q, k, v, [400, 200], do)
+        assert all(torch.equal(again[n], want[n]) for n in again)
+        replayed.fill_(7.0)
+        g.replay()
+        assert torch.equal(replayed, want["out"])
+
+    fails, beside = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with _dropped(monkeypatch, 0), torch.cuda.stream(fails):
+        base._run_cross(q, k, v, None)
+    with torch.cuda.stream(beside):
+        again = base._run_cross(q, k, v, [400, 200], do)
+    torch.cuda.synchronize()
+    assert all(torch.equal(again[n], want[n]) for n in again)
+    others_are_right()
+    out.fill_(7.0)
+    rt.attn_fwd(**kw)
+    torch.cuda.synchronize()
+    assert torch.equal(out, attended)
+    with pytest.raises(H3CError, match="^(?!.*h3c_attn_fwd).*h3c_cross_attn_fwd"):
+        rt.device_status()
+    rt.device_status()
+
+    with _dropped(monkeypatch, 3):
+        rt.attn_fwd(**kw)
+    torch.cuda.synchronize()
+    others_are_right()
+    with pytest.raises(H3CError, match="^(?!.*h3c_cross_attn_fwd).*h3c_attn_fwd"):
+        rt.device_status()
+    rt.attn_fwd_sync(**kw)
+    assert torch.equal(out, attended)
