@@ -4,7 +4,9 @@
  * This is the boundary a Swift `CUDABackend: H3AttentionBackend` (module
  * CH3Cuda) or any ctypes / cffi caller binds.  Plain pointers and sizes only;
  * no C++ or torch types.  Every call returns an h3c_status and never aborts;
- * h3c_last_error() gives the message of the last failure on a context.
+ * h3c_last_error() gives the message of the last failure on a context (of the
+ * calling thread's last one, where it had one there), valid until the thread's
+ * next failure or h3c_last_error().
  *
  * What each entry point replaces in the reference (MiniMax-H3-Swift):
  *   h3c_attn_fwd          H3AttentionBackend.attend + AttentionLayer.sdpa

@@ -210,7 +210,11 @@ h3c_status h3c_device_free(h3c_ctx* ctx, void* ptr) {
   return H3C_OK;
 }
 
-const char* h3c_last_error(const h3c_ctx* ctx) { return ctx ? ctx->err.c_str() : kNullCtxError; }
+const char* h3c_last_error(const h3c_ctx* ctx) try {
+  return ctx ? ctx->err.c_str() : kNullCtxError;
+} catch (const std::exception&) {
+  return "h3c: no host memory for the message";
+}
 
 h3c_status h3c_device_info(h3c_ctx* ctx, h3c_devinfo* info) {
   if (!ctx || !info) return fail(ctx, H3C_ERR_INVALID_ARGUMENT, "h3c_device_info: null argument");

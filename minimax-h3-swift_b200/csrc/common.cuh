@@ -5,13 +5,61 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+#include <mutex>
 #include <string>
 
 #include "h3cuda.h"
 
+namespace h3 {
+
+// The text of a context's last failure.  Host threads may fail at once: each
+// reads that of its own last failure, or, where that was on another context or
+// there was none, the context's.
+class LastError {
+ public:
+  LastError& operator=(const std::string& s) {
+    Mine& m = mine();
+    m.id = id_;
+    m.text = s;
+    std::lock_guard<std::mutex> hold(lock_);
+    text_ = s;
+    return *this;
+  }
+  // valid until the thread's next failure or c_str()
+  const char* c_str() const {
+    Mine& m = mine();
+    if (m.id != id_) {
+      std::lock_guard<std::mutex> hold(lock_);
+      m.id = 0;
+      m.text = text_;
+    }
+    return m.text.c_str();
+  }
+
+ private:
+  struct Mine {
+    uint64_t id = 0;
+    std::string text;
+  };
+  static Mine& mine() {
+    thread_local Mine m;
+    return m;
+  }
+  static uint64_t next() {
+    static std::atomic<uint64_t> n{0};
+    return ++n;
+  }
+  const uint64_t id_ = next();
+  mutable std::mutex lock_;
+  std::string text_;
+};
+
+}  // namespace h3
+
 struct h3c_ctx {
   int device = 0;
-  std::string err;
+  h3::LastError err;
   cudaDeviceProp prop{};
   void* workspace = nullptr;      // normalised keys/queries of the fused path
   size_t workspace_bytes = 0;
