@@ -76,6 +76,10 @@ __device__ __forceinline__ uint64_t mul_2(uint64_t a, uint64_t b) {
 __device__ __forceinline__ float lo2(uint64_t v) { return __uint_as_float((uint32_t)v); }
 __device__ __forceinline__ float hi2(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
 
+// What dq and dk are scaled by.  The softmax over one key is 1 whatever its
+// logit: what rounding left of dS there (a few rows in a million) is taken out.
+__device__ __forceinline__ float ds_scale(const BwdArgs& a, int len) { return len == 1 ? 0.f : a.scale; }
+
 __device__ __forceinline__ void tma_tile(uint32_t dst, const CUtensorMap* m, uint32_t bar, int tok, int h, int b) {
   tma_load_4d(dst, m, bar, 0, tok, h, b);
   tma_load_4d(dst + kHalfBytes, m, bar, 64, tok, h, b);
@@ -561,6 +565,7 @@ __global__ void __launch_bounds__(kDqThreads, 1)
         if (!wait_w(&bars->dq_full, un & 1)) break;
         ++un;
         tc_fence_after();
+        const float f = ds_scale(a, x.len);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           uint32_t v[32];
@@ -569,7 +574,7 @@ __global__ void __launch_bounds__(kDqThreads, 1)
           tmem_wait_ld();
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            k[16 * c + i] = pack_bf16(__uint_as_float(v[2 * i]) * a.scale, __uint_as_float(v[2 * i + 1]) * a.scale);
+            k[16 * c + i] = pack_bf16(__uint_as_float(v[2 * i]) * f, __uint_as_float(v[2 * i + 1]) * f);
         }
         tc_fence_before();
         mbar_arrive(smem_u32(&bars->dq_empty));
@@ -883,7 +888,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool head = seg.it0 > 0, tail = seg.it1 < seg.steps;
       const int key = seg.tile * 128 + r;
       const bool valid = key < seg.len, live = key < a.n.kv_len;
-      const float f = w ? 1.0f : a.scale;
+      const float f = w ? 1.0f : ds_scale(a, seg.len);
       const Rows& out = w ? a.dv : a.dk;
       uint16_t* go = live ? out.at(seg.b, key, seg.hk) : nullptr;
       float4* po = reinterpret_cast<float4*>(a.part + (((int64_t)blockIdx.x * 2 + (head ? 0 : 1)) * 2 + w) * 16384);
@@ -941,7 +946,7 @@ __global__ void __launch_bounds__(256) dkv_join_kernel(const __grid_constant__ B
     sum.z += v.z;
     sum.w += v.w;
   }
-  const float f = which ? 1.0f : a.scale;
+  const float f = which ? 1.0f : ds_scale(a, own.len);
   uint2 o = make_uint2(pack_bf16(sum.x * f, sum.y * f), pack_bf16(sum.z * f, sum.w * f));
   if (key >= own.len) o = make_uint2(0, 0);
   *reinterpret_cast<uint2*>((which ? a.dv : a.dk).at(own.b, key, own.hk) + 4 * cg) = o;

@@ -27,3 +27,31 @@ def test_dense_rows_beside_units_of_part_tiles(gpu, B, S, N, H, lens):
     for _ in range(30):
         again = base._run_cross(q, k, v, lens)
         assert torch.equal(again["out"], first["out"]) and torch.equal(again["lse"], first["lse"])
+
+
+@pytest.mark.parametrize("N", [1, 77, 128, 129, 600])
+@pytest.mark.parametrize("std", [1.0, 4.0])
+def test_gradient_of_a_lone_key_is_zero(gpu, N, std):
+    """The softmax over one key is 1 whatever its logit: dq and dk are 0 to the
+    last bit, dv is the sum of do.  q_len * heads large enough that a key tile
+    of the member is cut among blocks, too."""
+    import torch
+
+    for seed in range(90, 94):
+        B, S, H, Hk = 3, 700, 6, 2
+        lens = [1, N, 1]
+        q, k, v, do = base._inputs(B, S, N, H, Hk, seed, std=std)
+        got = base._run_cross(q, k, v, lens, do)
+        base._check_attention(q, k, v, lens, got, do, one_block=N <= 128)
+        for b in (0, 2):
+            assert (got["dq"][b] == 0).all(), (seed, b, got["dq"][b].abs().max().item())
+            assert (got["dk"][b] == 0).all(), (seed, b, got["dk"][b].abs().max().item())
+
+
+@pytest.mark.parametrize("N", [1, 200])
+def test_gradient_of_a_lone_key_is_zero_in_millions_of_rows(gpu, N):
+    """P dP / P is dP in all but a few rows in a million, whose dS is a last
+    bit of dP: those too come out as 0."""
+    q, k, v, do = base._inputs(1, 65536, N, 40, 40, 3, std=4.0)
+    got = base._run_cross(q, k, v, [1], do)
+    assert (got["dq"] == 0).all() and (got["dk"] == 0).all()
