@@ -162,12 +162,12 @@ h3c_status cross_call(h3c_ctx* ctx, const h3c_cross_args* args, int op, const ch
   L.ws = (uint8_t*)args->workspace;
   L.status = (int32_t*)(ctx->d_counter + 3);
   L.wait_limit_ns = h3::kWaitLimitNs;
-  L.drop_item = -1;
-  // Test hooks (fault injection on the host side), as those of h3c_attn_fwd; the
-  // load to drop is read only beside a shorter bound.
+  L.stall = -1;
+  // Test hooks (fault injection on the host side): a shorter bound, as that of
+  // h3c_attn_fwd, and beside it a barrier that waits for bytes that never come.
   if (const char* w = getenv("H3C_TEST_WAIT_LIMIT_NS")) {
     L.wait_limit_ns = strtoull(w, nullptr, 10);
-    if (const char* d = getenv("H3C_TEST_DROP_ITEM")) L.drop_item = atoi(d);
+    if (const char* b = getenv("H3C_TEST_STALL_BARRIER")) L.stall = atoi(b);
   }
   std::string why;
   cudaError_t e = op == H3C_OP_CROSS_BWD ? h3::launch_cross_bwd(L, (cudaStream_t)stream, &why)

@@ -28,7 +28,7 @@ struct CrossLaunch {
   uint8_t* ws;
   int32_t* status;            // the context's status word of these calls (bounded waits), written only
   uint64_t wait_limit_ns;
-  int32_t drop_item;          // test hook: load of each CTA that its producer skips (-1: none)
+  int32_t stall;              // test hook: barrier of each CTA that never completes (-1: none)
 };
 
 // n / d for n < 2^31, d >= 1: m = ceil(2^(31 + s) / d) with 2^s >= d.

@@ -46,7 +46,7 @@ struct BwdArgs {
   int32_t q_blocks;
   int32_t* status;
   uint64_t wait_limit_ns;
-  int32_t drop_item;          // test hook: K tile (dq) and q tile (dk, dv) of each CTA that is never loaded
+  int32_t stall;              // test hook: barrier (from q_full, kv_full on) that never completes
   int32_t q_b, q_h, k_b, k_h, v_b, v_h, g_b, g_h;
   Div by_blocks, by_heads, by_group;
 };
@@ -265,6 +265,7 @@ __global__ void __launch_bounds__(kDqThreads, 1)
     mbar_init(smem_u32(&bars->dq_full), 1);
     mbar_init(smem_u32(&bars->dq_empty), 128);
     mbar_init(smem_u32(&bars->done), 2);
+    if (a.stall >= 0 && &bars->q_full + a.stall <= &bars->ds_full[1]) mbar_stall(smem_u32(&bars->q_full + a.stall));
     bars->abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -275,7 +276,7 @@ __global__ void __launch_bounds__(kDqThreads, 1)
   // placed while the kernel before runs; nothing is read or written before its end
   asm volatile("griddepcontrol.wait;" ::: "memory");
   auto wait = [&](uint64_t* bar, uint32_t parity) {
-    return mbar_wait<false>(smem_u32(bar), parity, abort_flag, a.status, a.wait_limit_ns);
+    return mbar_wait_alone(smem_u32(bar), parity, abort_flag, a.status, a.wait_limit_ns);
   };
   // Register split of the launch's 512 x 128: 128 x 48 + 256 x 176 + 128 x 112.
   if (warp < 4) {
@@ -315,8 +316,7 @@ __global__ void __launch_bounds__(kDqThreads, 1)
                               (valid < 128 && x.len < a.n.kv_len ? valid << kZeroShift : 0);
           bar = smem_u32(&bars->k_full[kr]);
           mbar_expect_tx(bar, kTileBytes);
-          if (e != a.drop_item)
-            tma_tile(smem_u32(sK + kr * kTileBytes), &tm_k, bar, 128 * j, hk * a.k_h, x.b * a.k_b);
+          tma_tile(smem_u32(sK + kr * kTileBytes), &tm_k, bar, 128 * j, hk * a.k_h, x.b * a.k_b);
           ++e;
           if (++kr == 3) {
             kr = 0;
@@ -679,6 +679,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(smem_u32(&bars->acc_full), 1);
     mbar_init(smem_u32(&bars->acc_empty), 256);
     mbar_init(smem_u32(&bars->done), 1);
+    if (a.stall >= 0 && &bars->kv_full + a.stall <= &bars->done) mbar_stall(smem_u32(&bars->kv_full + a.stall));
     bars->abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -690,7 +691,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // step of 3 x 257 x 8 rows; the same in dq_kernel cost the clip 2%).
   if (warp >= 2) asm volatile("griddepcontrol.wait;" ::: "memory");
   auto wait = [&](uint64_t* bar, uint32_t parity) {
-    return mbar_wait<false>(smem_u32(bar), parity, abort_flag, a.status, a.wait_limit_ns);
+    return mbar_wait_alone(smem_u32(bar), parity, abort_flag, a.status, a.wait_limit_ns);
   };
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
@@ -713,8 +714,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           bars->info[e & 7] = (it == seg.it0 ? kFirst : 0) | (it == seg.it1 - 1 ? kLast : 0);
           bar = smem_u32(&bars->q_full[qr]);
           mbar_expect_tx(bar, kTileBytes);
-          if (e != a.drop_item)
-            tma_tile(smem_u32(sQ + qr * kTileBytes), &tm_q, bar, 128 * qb, h * a.q_h, seg.b * a.q_b);
+          tma_tile(smem_u32(sQ + qr * kTileBytes), &tm_q, bar, 128 * qb, h * a.q_h, seg.b * a.q_b);
           ++e;
           if (++qr == 3) {
             qr = 0;
@@ -1035,7 +1035,7 @@ cudaError_t launch_cross_bwd(const CrossLaunch& L, cudaStream_t s, std::string* 
   a.part = a.delta + rows;
   a.status = L.status;
   a.wait_limit_ns = L.wait_limit_ns;
-  a.drop_item = L.drop_item;
+  a.stall = L.stall;
   a.q_b = L.q.b != 0, a.q_h = L.q.h != 0;
   a.k_b = L.k.b != 0, a.k_h = L.k.h != 0;
   a.v_b = L.v.b != 0, a.v_h = L.v.h != 0;

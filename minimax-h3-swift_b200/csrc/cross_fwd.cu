@@ -103,7 +103,7 @@ struct FwdArgs {
   float2* part_ml[2];
   int32_t* status;
   uint64_t wait_limit_ns;
-  int32_t drop_item;          // test hook: K/V entry of each CTA that is never loaded
+  int32_t stall;              // test hook: barrier (from Barriers::q_full on) that never completes
   // 1 where an operand's tensor map has the axis, 0 where it is broadcast
   int32_t q_b, q_h, k_b, k_h, v_b, v_h, pk_h, pv_h;
 };
@@ -265,6 +265,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(smem_u32(&bars->v_empty[r]), 1);
     }
     mbar_init(smem_u32(&bars->done), 1);
+    if (a.stall >= 0 && bars->q_full + a.stall <= &bars->done) mbar_stall(smem_u32(bars->q_full + a.stall));
     bars->abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -281,7 +282,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = bars->tmem_base;
   asm volatile("griddepcontrol.launch_dependents;");
   auto wait = [&](uint64_t* bar, uint32_t parity) {
-    return mbar_wait<false>(smem_u32(bar), parity, abort_flag, a.status, a.wait_limit_ns);
+    return mbar_wait_alone(smem_u32(bar), parity, abort_flag, a.status, a.wait_limit_ns);
   };
 
   // Register split of the launch's 512 x 128: 128 x 48 + 256 x 192 + 128 x 80.
@@ -330,7 +331,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             // of 65,536 keys, 1 row: 56 us, 61 with the tiles kept in L2 like
             // any other load)
             auto load = [&](uint32_t dst, const CUtensorMap* map, int tok, int h, int b) {
-              if (ec == a.drop_item) return;  // (the entry then never completes)
 #pragma unroll
               for (int x = 0; x < 2; ++x)
                 if constexpr (dense) tma_load_4d(dst + x * kHalfBytes, map, bar, 64 * x, tok, h, b);
@@ -647,9 +647,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto finish_box = [&](int t, bool has, float2 ml) {
       tc_fence_after();
       const int row0 = s.row0 + 128 * t + 32 * q;
-      // A warp without rows leaves both boxes alone: its waits below count on a
-      // store of every box that it fills.
-      if (row0 >= s.row_end) return;
       const float f = 1.0f / fmaxf(ml.y, 1e-30f);
       if (a.lse && row0 + lane < s.row_end)
         a.lse[((int64_t)s.b * a.n.heads + s.h) * a.n.q_len + row0 + lane] =
@@ -657,7 +654,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
       for (int p = 0; p < 2; ++p) {
         uint8_t* box = stage + p * 4096;
-        if (lane == 0) tma_store_wait_read<1>();  // the box two stores ago has been read
+        if (lane == 0) tma_store_wait_read<1>();  // the box two groups ago has been read
         __syncwarp();
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -683,8 +680,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         fence_async_shared();
         __syncwarp();
-        if (lane == 0)
-          tma_store_4d(&tm_o, smem_u32(box), 64 * p, row0, s.h * (a.out.h != 0), s.b * (a.out.b != 0));
+        if (lane == 0) {
+          if (row0 < s.row_end)
+            tma_store_4d(&tm_o, smem_u32(box), 64 * p, row0, s.h * (a.out.h != 0), s.b * (a.out.b != 0));
+          tma_store_commit();  // a group for every box that was filled, empty or not: the waits count them
+        }
       }
     };
     // any other rows of tile t: O of half t (f0) and, where has1, of half 1
@@ -1083,7 +1083,7 @@ cudaError_t launch_cross_fwd(const CrossLaunch& L, cudaStream_t s, std::string* 
   }
   a.status = L.status;
   a.wait_limit_ns = L.wait_limit_ns;
-  a.drop_item = L.drop_item;
+  a.stall = L.stall;
   a.q_b = L.q.b != 0, a.q_h = L.q.h != 0;
   a.k_b = L.k.b != 0, a.k_h = L.k.h != 0;
   a.v_b = L.v.b != 0, a.v_h = L.v.h != 0;

@@ -27,6 +27,11 @@ __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
 }
 
+// Bytes that never come: the barrier's phase does not complete (a test hook).
+__device__ __forceinline__ void mbar_stall(uint32_t bar) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], 16;" ::"r"(bar) : "memory");
+}
+
 __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
@@ -39,10 +44,7 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
   return ok != 0;
 }
 
-// Bounded wait; false on abort/timeout.  SHARED: launches share the status
-// word, and a wait that finds it set gives up; without, the word is only
-// written, so that calls beside or behind a failed one are not drawn in.
-template <bool SHARED = true>
+// Bounded wait; false on abort/timeout.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int32_t* abort_flag,
                                           int32_t* status, uint64_t limit_ns = kWaitLimitNs) {
   for (int i = 0; i < 64; ++i)
@@ -51,10 +53,9 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
   while (true) {
     if (mbar_try(bar, parity)) return true;
     if (*abort_flag) return false;
-    // another CTA's wait already gave up: stop instead of timing out again, so
-    // that a systematic stall ends in one limit (a grid of at most a CTA an SM
-    // does so anyway)
-    if (SHARED && status && *(volatile int32_t*)status != 0) {
+    // another CTA's wait already gave up: stop instead of timing out again
+    // (one status word per launch, so a systematic stall ends in one limit)
+    if (status && *(volatile int32_t*)status != 0) {
       *abort_flag = 1;
       return false;
     }
@@ -63,6 +64,31 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
       if (status) atomicExch(status, (int32_t)H3C_ERR_TIMEOUT);
       return false;
     }
+  }
+}
+
+// The same for calls whose status word is only written, so that those beside
+// or behind a failed one are not drawn in (a grid of at most a CTA an SM ends in
+// one limit all the same).  From the 65th try on a try every 200 ns: polls
+// without a pause take issue slots from the warps that are waited for (16,384
+// keys, 4,096 x 40 rows: 1,180 us; 1,325 without, 1,310 and 1,370 with nanosleep
+// and with the suspension that try_wait can be given).
+__device__ __forceinline__ bool mbar_wait_alone(uint32_t bar, uint32_t parity, volatile int32_t* abort_flag,
+                                                int32_t* status, uint64_t limit_ns) {
+  for (int i = 0; i < 64; ++i)
+    if (mbar_try(bar, parity)) return true;
+  const uint64_t t0 = globaltimer();
+  while (true) {
+    if (mbar_try(bar, parity)) return true;
+    if (*abort_flag) return false;
+    uint64_t now = globaltimer();
+    if (now - t0 > limit_ns) {
+      *abort_flag = 1;
+      atomicExch(status, (int32_t)H3C_ERR_TIMEOUT);
+      return false;
+    }
+    const uint64_t next = now + 200;
+    while (now < next) now = globaltimer();
   }
 }
 
@@ -443,14 +469,15 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
-// 4D tiled TMA store from shared memory (this thread's bulk group), and the
-// wait until at most N of the thread's groups still read shared memory.
+// 4D tiled TMA store from shared memory, the end of a bulk group of this
+// thread's stores, and the wait until at most N of its groups still read shared
+// memory.
 __device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2, int c3) {
   asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(map),
                "r"(src), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
                : "memory");
-  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
+__device__ __forceinline__ void tma_store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void tma_store_wait_read() {
   asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
