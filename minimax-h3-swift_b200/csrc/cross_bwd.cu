@@ -197,6 +197,7 @@ __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ BwdA
 // 1,024 of the MUFU units between two TMEM round trips).
 struct __align__(16) DqBarriers {
   float nl2[2][128], delta[2][128];  // by unit parity
+  float weights[128];                // half 1's share of a row's sum of P
   uint64_t q_full, q_empty, g_full, g_empty;
   uint64_t k_full[3], k_empty[3], v_full[2], v_empty[2];
   uint64_t n_full[2];                // -lse2 and delta of unit u on [u & 1]
@@ -495,12 +496,11 @@ __global__ void __launch_bounds__(kDqThreads, 1)
         uint32_t d[64];
         load64(lane_base + 256 + 64 * w, d);
         if (ONE || x.n == 1) {
-          // All keys are here, so delta is sum(P dP) in fp32 and not do.out:
-          // the rounding of out shows in dS where keys are few (with one key
-          // dS is 0: hence also the division by the weights' own sum).  Half 1
-          // hands its sum over in the place of delta, half 0 the whole one in
-          // that of -lse2, which both have read; the places are the unit's
-          // until dp_empty.
+          // All keys are here, so delta is sum(P dP) / sum(P) in fp32 and not
+          // do.out: the rounding of out shows in dS where keys are few, and
+          // that of lse in a weight near 1.  Half 1 hands its sum of P dP over
+          // in the place of delta, half 0 delta in that of -lse2, which both
+          // have read; the places are the unit's until dp_empty.
           float own = 0.f, ps = 0.f;
 #pragma unroll
           for (int c = 0; c < 64; ++c)
@@ -511,13 +511,15 @@ __global__ void __launch_bounds__(kDqThreads, 1)
           float *other = &bars->delta[(un - 1) & 1][r], *all = &bars->nl2[(un - 1) & 1][r];
           if (w == 1) {
             *other = own;
+            bars->weights[r] = ps;
             fence_async_shared();
             mbar_arrive(smem_u32(&bars->sum_full[1]));
             if (!(ok = wait_w(&bars->sum_full[0], n1 & 1))) break;
             own = *all;
           } else {
             if (!(ok = wait_w(&bars->sum_full[1], n1 & 1))) break;
-            own = x.len > 64 ? own + *other : ps > 0.f ? own / ps : 0.f;
+            ps += bars->weights[r];
+            own = ps > 0.f ? (own + *other) / ps : 0.f;
             *all = own;
             fence_async_shared();
             mbar_arrive(smem_u32(&bars->sum_full[0]));

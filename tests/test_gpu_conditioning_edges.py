@@ -55,3 +55,34 @@ def test_gradient_of_a_lone_key_is_zero_in_millions_of_rows(gpu, N):
     q, k, v, do = base._inputs(1, 65536, N, 40, 40, 3, std=4.0)
     got = base._run_cross(q, k, v, [1], do)
     assert (got["dq"] == 0).all() and (got["dk"] == 0).all()
+
+
+@pytest.mark.parametrize("N", [128, 300])
+def test_gradient_of_rows_with_one_key_of_weight(gpu, N):
+    """Rows whose every other weight is 0 in fp32, with logits of 5,792 to 11,585:
+    lse is off by 2^-24 of that, so the one weight by up to 2^-9, but dS is 0.  With up to
+    128 keys delta is P dP / P, two roundings from dP: dS is at most 2^-22 |dP| then.
+    dk takes dP from a product of its own: its 128 additions are off by at most
+    2^-23 of the sum of magnitudes each, 2^-16 in all, as is the first one's."""
+    import torch
+
+    lens, S, H = [128, 100, 65, 64, 20], 200, 2
+    B = len(lens)
+    _, _, v, do = base._inputs(B, S, N, H, H, 95)
+    g = base._gen(96)
+    k = torch.where(torch.rand(B, N, H, base.D, device="cuda", generator=g) < 0.5, -32.0, 32.0).to(torch.bfloat16)
+    at = torch.stack([torch.randint(0, n, (S,), device="cuda", generator=g) for n in lens])
+    member = torch.arange(B, device="cuda")[:, None]
+    size = torch.randint(64, 129, (B, S, H, 1), device="cuda", generator=g) / 128
+    q, hot = (k[member, at] * size).to(torch.bfloat16), v[member, at]
+    got = base._run_cross(q, k, v, lens, do)
+    assert torch.equal(got["out"], hot)
+    dp, mag = (do.double() * hot.double()).sum(-1), (do.double().abs() * hot.double().abs()).sum(-1)
+    bound = 32 * base.SCALE * (2.0 ** -22 * dp.abs())[..., None]
+    over = (got["dq"].double().abs() - bound).amax((1, 2, 3))
+    assert (over <= 0).all(), over.tolist()
+    rows = torch.zeros(B, N, H, device="cuda", dtype=torch.float64)
+    for b in range(B):
+        rows[b].index_add_(0, at[b], 2.0 ** -22 * dp[b].abs() + 2.0 ** -15 * mag[b])
+    over = (got["dk"].double().abs() - 32 * base.SCALE * rows[..., None]).amax((1, 2, 3))
+    assert (over <= 0).all(), over.tolist()
