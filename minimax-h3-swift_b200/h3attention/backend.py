@@ -334,9 +334,13 @@ def cross_sdpa(q, k, v, head_dim: int, kv_lens=None):
     ``[B, S, H, D]``, ``k`` and ``v`` ``[N, Hk, D]`` (with ``q``'s batch axis;
     H a multiple of Hk), bf16 in, ``[S, H*D]`` (``[B, S, H*D]``) out.
     ``kv_lens`` (int32 ``[B]`` on the device) counts each member's valid keys;
-    a member without any gives zeros."""
+    a member without any gives zeros.  Forward only: operands that want a
+    gradient are refused unless gradients are off."""
     import torch
 
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (q, k, v)):
+        raise ValueError("cross_sdpa gives no gradients: call it under torch.no_grad(), or Runtime.cross_attn_fwd and "
+                         "cross_attn_bwd from a torch.autograd.Function")
     if not isinstance(q, torch.Tensor) or not q.is_cuda:
         raise ValueError("q must be a CUDA tensor")
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
