@@ -341,6 +341,8 @@ def cross_sdpa(q, k, v, head_dim: int, kv_lens=None):
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (q, k, v)):
         raise ValueError("cross_sdpa gives no gradients: call it under torch.no_grad(), or Runtime.cross_attn_fwd and "
                          "cross_attn_bwd from a torch.autograd.Function")
+    if isinstance(q, torch.Tensor) and q.dim() and q.shape[-1] != head_dim:
+        raise ValueError(f"q must have head_dim {head_dim}, got {q.shape[-1]}")
     if not isinstance(q, torch.Tensor) or not q.is_cuda:
         raise ValueError("q must be a CUDA tensor")
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)

@@ -20,3 +20,11 @@ def test_cross_sdpa_refuses_to_lose_a_gradient(which):
         cross_sdpa(*x, 128)
     with torch.no_grad(), pytest.raises(ValueError, match="must be a CUDA tensor"):
         cross_sdpa(*x, 128)
+
+
+def test_cross_sdpa_refuses_another_head_dim():
+    """The scale follows from head_dim: one that is not the operands' would scale wrongly."""
+    from h3attention import cross_sdpa
+
+    with pytest.raises(ValueError, match="head_dim 64, got 128"):
+        cross_sdpa(*_operands(), 64)
