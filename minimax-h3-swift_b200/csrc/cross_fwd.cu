@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = bars->tmem_base;
   asm volatile("griddepcontrol.launch_dependents;");
   auto wait = [&](uint64_t* bar, uint32_t parity) {
-    return mbar_wait_alone(smem_u32(bar), parity, abort_flag, a.status, a.wait_limit_ns);
+    return mbar_wait_alone<dense>(smem_u32(bar), parity, abort_flag, a.status, a.wait_limit_ns);
   };
 
   // Register split of the launch's 512 x 128: 128 x 48 + 256 x 192 + 128 x 80.

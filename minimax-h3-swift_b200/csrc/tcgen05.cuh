@@ -69,10 +69,13 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
 
 // The same for calls whose status word is only written, so that those beside
 // or behind a failed one are not drawn in (a grid of at most a CTA an SM ends in
-// one limit all the same).  From the 65th try on a try every 200 ns: polls
-// without a pause take issue slots from the warps that are waited for (16,384
-// keys, 4,096 x 40 rows: 1,180 us; 1,325 without, 1,310 and 1,370 with nanosleep
-// and with the suspension that try_wait can be given).
+// one limit all the same).  PACED: from the 65th try on a try every 200 ns, as
+// polls without a pause take issue slots from the warps that are waited for
+// (dense rows against 16,384 keys, 4,096 x 40: 1,180 us; 1,325 without, 1,310
+// and 1,370 with nanosleep and with the suspension that try_wait can be given).
+// Folded rows wait for HBM or for few warps, and are faster without (32 members
+// over 65,536 keys and 512 of their own: 102.5 us, 106.5 with).
+template <bool PACED = true>
 __device__ __forceinline__ bool mbar_wait_alone(uint32_t bar, uint32_t parity, volatile int32_t* abort_flag,
                                                 int32_t* status, uint64_t limit_ns) {
   for (int i = 0; i < 64; ++i)
@@ -87,8 +90,10 @@ __device__ __forceinline__ bool mbar_wait_alone(uint32_t bar, uint32_t parity, v
       atomicExch(status, (int32_t)H3C_ERR_TIMEOUT);
       return false;
     }
-    const uint64_t next = now + 200;
-    while (now < next) now = globaltimer();
+    if constexpr (PACED) {
+      const uint64_t next = now + 200;
+      while (now < next) now = globaltimer();
+    }
   }
 }
 
