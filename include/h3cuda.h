@@ -335,7 +335,10 @@ enum { H3C_OP_CROSS_FWD = 0, H3C_OP_CROSS_BWD = 1, H3C_OP_PREFIX_FWD = 2 };
  * attend to its first kv_lens[b] keys (clamped to [0, kv_len]; NULL: all),
  * after the shared prefix where there is one; key and value rows past that
  * length are not used whatever they hold (NaN included).  A row without keys
- * gives an output of 0, a log-sum-exp of -inf and no gradient. */
+ * gives an output of 0, a log-sum-exp of -inf and no gradient.  Logits
+ * (scale q.k) are fp32 and must stay below 2^30 in magnitude, beyond that rows
+ * can come out as NaN; lse is fp32 too, so the gradient's weights are off by
+ * 2^-23 of its magnitude.  Where a member has one key, dq and dk are 0. */
 typedef struct h3c_cross_args {
   h3c_bview q, out;           /* [batch, q_len, heads, 128]; out may not overlap an input */
   h3c_bview k, v;             /* [batch, kv_len, kv_heads, 128] */

@@ -3,8 +3,8 @@
 //   P = 2^(scale log2(e) q.k - lse2);  delta_i = do_i.o_i;  dS = P (do v^T - delta)
 //   dq = scale dS k;  dk = scale dS^T q;  dv = P^T do   (sums over the heads of a group)
 //
-// (delta_i = sum_j P_ij dP_ij too, and is taken so of members with up to 128
-// keys).  delta_kernel goes over do and out once, unless kv_len <= 128; then
+// (delta_i = sum_j P_ij dP_ij / sum_j P_ij too, and is taken so of members with
+// up to 128 keys).  delta_kernel goes over do and out once, unless kv_len <= 128; then
 // two passes, so that every sum has one owner and a fixed order (no atomics):
 //   dq_kernel    a CTA holds 128 queries and walks the keys: S, dP, dq += dS K
 //   dkv_kernel   a CTA holds 128 keys and walks the queries of all heads of

@@ -37,12 +37,12 @@
 // What bounds it: dense, the alternation of each half's products (1,024
 // cycles a key tile) and softmax (2,200, of them 1,024 of the MUFU units), and
 // from 1,024 keys on the power cap (1.4-1.6 GHz): 32,768 x 40 rows against 512
-// keys 345-385 us (0.9-1.0 PFLOP/s), against 4,096 2.45-2.75 ms (1.0-1.1).
-// Below 256 keys the units' turn-over: 128 keys 160 us, 4.2 TB/s.  Single: HBM
-// (64 members of 4,096 keys and 8 key heads: 180 us, 6.0 TB/s; one token over
-// 65,536 keys: 56 us for 41 at the copy rate, the rest the start, whose code
+// keys 340 us (1.0 PFLOP/s), against 4,096 2.4-2.5 ms (1.1).
+// Below 256 keys the units' turn-over: 128 keys 165 us, 4.1 TB/s.  Single: HBM
+// (64 members of 4,096 keys and 8 key heads: 184 us, 5.8 TB/s; one token over
+// 65,536 keys: 59 us for 41 at the copy rate, the rest the start, whose code
 // and queries come from HBM behind the first keys, and the join).  Dual: as
-// dense (32 members of 5 rows over 65,536 keys and 512 of their own: 104 us).
+// dense (32 members of 5 rows over 65,536 keys and 512 of their own: 103 us).
 // Every wait is bounded (see attn_tc.cu; a CTA that gives up does so alone).
 #include <algorithm>
 #include <climits>
